@@ -30,6 +30,18 @@ class CandleQError(RuntimeError):
     pass
 
 
+class KvCache(C.Structure):
+    """cq_kv_cache"""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("state", C.c_void_p)] + \
+        [(n, C.c_int) for n in ("layers", "pages", "kv_heads", "page_size", "head_dim", "max_seqs", "max_pages", "elem")]
+
+
+class PrefixPlan(C.Structure):
+    """cq_prefix_plan"""
+    _fields_ = [(n, C.c_int) for n in ("batch", "queries", "heads", "groups", "row_tile", "ctas", "shared_items")] + \
+        [("n_ints", C.c_int64), ("n_floats", C.c_int64), ("ints", C.c_void_p), ("scratch", C.c_void_p)]
+
+
 _lib = None
 
 
@@ -145,6 +157,22 @@ def lib() -> C.CDLL:
             getattr(L, f"launch_mmvq_gguf_quantize_q8_1_{el}").argtypes = [vp, vp, i32, i32, i32, vp]
             for t in TYPE_NAME.values():
                 getattr(L, f"launch_mmvq_gguf_{t}_{el}_plain").argtypes = [vp, vp, vp, i32, i32, i32, i32, i32, vp]
+        kvp, planp = C.POINTER(KvCache), C.POINTER(PrefixPlan)
+        L.cq_kv_state_ints.argtypes, L.cq_kv_state_ints.restype = [i32] * 3, C.c_size_t
+        L.cq_kv_reset.argtypes = L.cq_kv_compact.argtypes = [kvp, vp]
+        L.cq_kv_reserve.argtypes = [kvp, vp, i32, i32, vp]
+        L.cq_kv_fork.argtypes = [kvp, vp, vp, i32, i32, vp]
+        L.cq_kv_free.argtypes = [kvp, vp, i32, vp]
+        L.cq_kv_append.argtypes = [kvp, i32, vp, i32, i32, vp, vp, vp, i32, i32, i64, i64, i64, vp, vp, i32, i32, vp, vp]
+        L.cq_kv_take_fault.argtypes, L.cq_kv_take_fault.restype = [kvp, vp], i32
+        L.cq_prefix_plan_shape.argtypes, L.cq_prefix_plan_shape.restype = [kvp, planp, vp, vp], i32
+        L.cq_prefix_plan_update.argtypes = [kvp, planp, vp, vp]
+        L.cq_prefix_attention.argtypes = [kvp, i32, planp, vp, i64, vp, C.c_float, vp]
+        for f in (L.cq_kv_reset, L.cq_kv_compact, L.cq_kv_reserve, L.cq_kv_fork, L.cq_kv_free, L.cq_kv_append, L.cq_prefix_plan_update, L.cq_prefix_attention,
+                  L.cq_token_logprobs):
+            f.restype = None
+        L.cq_token_logprobs_scratch_bytes.argtypes, L.cq_token_logprobs_scratch_bytes.restype = [i32] * 3, C.c_size_t
+        L.cq_token_logprobs.argtypes = [vp, i32, i64, i32, i32, vp, i32, vp, vp, vp, vp, vp, vp]
         i64p, sz = C.POINTER(C.c_int64), C.c_size_t
         L.cqh_last_error.restype = C.c_char_p
         L.cqh_qtensor_load.argtypes = [i32, vp, sz, i64p, i32, i32, C.POINTER(vp)]

@@ -1,0 +1,527 @@
+// Pages of a KV cache: reserving, forking, freeing and compacting them, and the store of new keys and values.
+//
+// The bookkeeping (reference counts, lengths, tables) lives on the device, so that a decode step that grows its sequences, or forks
+// one, is a sequence of launches that a graph can hold.  One CTA does it: a pool has some thousands of pages, and a page's number
+// depends on all that are taken before it.  What it decides, a second kernel copies with the whole device.
+#include <cstdio>
+
+#include "kv_cache.cuh"
+
+namespace cq_kv {
+
+bool cache_ok(const cq_kv_cache *c, const char *who) {
+    char msg[160];
+    const char *why = nullptr;
+    int status = CQ_ERR_BAD_ARG;
+    if (!c || !c->k || !c->v || !c->state) why = "null pointer";
+    else if (c->layers <= 0 || c->pages <= 0 || c->kv_heads <= 0 || c->max_seqs <= 0 || c->max_pages <= 0) why = "sizes must be positive";
+    else if (c->elem != CQ_F32 && c->elem != CQ_F16 && c->elem != CQ_BF16) why = "element type must be f32, f16 or bf16";
+    else if (((uintptr_t)c->k | (uintptr_t)c->v | (uintptr_t)c->state) & 15) why = "k, v and state must be 16-byte aligned";
+    else {
+        status = CQ_ERR_UNSUPPORTED;
+        if (c->page_size != 16 && c->page_size != 32 && c->page_size != 64 && c->page_size != 128) why = "page_size must be 16, 32, 64 or 128";
+        else if (c->head_dim != 64 && c->head_dim != 128) why = "head_dim must be 64 or 128";
+        else if (c->max_seqs > 65536 || (int64_t)c->max_seqs * c->max_pages > (1 << 28) || (int64_t)c->max_pages * c->page_size > (1 << 30))
+            why = "at most 65536 slots, 2^28 table entries and 2^30 positions";
+        // rows of head_dim elements of one layer are numbered in 32 bits
+        else if ((int64_t)c->pages * c->kv_heads * c->page_size > INT32_MAX || (int64_t)c->pages * c->layers * c->kv_heads > (1 << 26))
+            why = "at most 2^31 rows in a layer and 2^26 pages over all layers and heads";
+    }
+    if (!why) return true;
+    std::snprintf(msg, sizeof msg, "%s: %s", who, why);
+    cq_set_status(status, msg);
+    return false;
+}
+
+}  // namespace cq_kv
+
+namespace {
+using namespace cq_kv;
+
+constexpr int kMeta = 1024;
+
+// Sum of `v` over the threads before this one; `total` over all.
+__device__ __forceinline__ int block_scan(int v, int *sums, int &total) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    int x = v;
+#pragma unroll
+    for (int m = 1; m < 32; m <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, x, m);
+        if (lane >= m) x += y;
+    }
+    __syncthreads();                    // the sums of the call before have been read
+    if (lane == 31) sums[warp] = x;
+    __syncthreads();
+    int w = sums[lane];
+#pragma unroll
+    for (int m = 1; m < 32; m <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, w, m);
+        if (lane >= m) w += y;
+    }
+    total = __shfl_sync(0xffffffffu, w, 31);
+    const int before = __shfl_sync(0xffffffffu, w, (warp + 31) & 31);
+    return x - v + (warp ? before : 0);
+}
+
+__device__ __forceinline__ int pages_of(int len, int page) { return (len + page - 1) / page; }
+
+// The `total` lowest free pages into copies[3 f + 1]; false when there are fewer.
+__device__ bool take_free(const State &s, int total, int *sums) {
+    int found = 0;
+    for (int p0 = 0; p0 < s.pages && found < total; p0 += 4 * kMeta) {
+        const int p = p0 + 4 * threadIdx.x;
+        int r[4] = {1, 1, 1, 1};
+        if (p + 3 < s.pages) {
+            const int4 q = *reinterpret_cast<const int4 *>(s.refs + p);
+            r[0] = q.x; r[1] = q.y; r[2] = q.z; r[3] = q.w;
+        } else
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (p + i < s.pages) r[i] = s.refs[p + i];
+        int mine = 0, all;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) mine += r[i] == 0;
+        int f = found + block_scan(mine, sums, all);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (r[i] == 0) {
+                if (f < total) s.copies[3 * (size_t)f + 1] = p + i;
+                ++f;
+            }
+        found += all;
+    }
+    __syncthreads();
+    return found >= total;
+}
+
+// Whether the pages in the row of a slot of length `len` are in the pool and taken; one warp.
+__device__ __forceinline__ bool row_ok(const State &s, int slot, int len, int lane) {
+    bool ok = true;
+    for (int j = lane; j < pages_of(len, s.page); j += 32) {
+        const int p = s.tables[(size_t)slot * s.max_pages + j];
+        ok = ok && p >= 0 && p < s.pages && s.refs[p] > 0;
+    }
+    return __all_sync(0xffffffffu, ok);
+}
+
+enum MetaOp { kReserve, kFork, kFree };
+
+// Three passes: everything is checked; the pages each slot needs are numbered in the order of the list; then the state changes.
+template <int OP>
+__global__ void __launch_bounds__(kMeta) kv_meta_kernel(const cq_kv_cache cache, const int *__restrict__ slots, const int *__restrict__ dst, int n, int arg) {
+    extern __shared__ unsigned seen[];              // one bit per slot
+    __shared__ int sums[32], err;
+    const State s = state_of(cache);
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, cap = s.max_pages * s.page;
+    cq_pdl_wait();
+    for (int i = tid; i < (s.max_seqs + 31) / 32; i += kMeta) seen[i] = 0;
+    if (tid == 0) {
+        err = s.header[0] ? -1 : 0;
+        s.header[1] = 0;
+    }
+    __syncthreads();
+    const int stop = err;
+    __syncthreads();                                // read by all before any thread adds to it
+    if (stop) return;
+    auto in_range = [&](int slot) { return slot >= 0 && slot < s.max_seqs; };
+    auto fail = [&](int code) { atomicMax(&err, code); };
+    const int *changed = OP == kFork ? dst : slots;
+    for (int i = tid; i < n; i += kMeta) {
+        const int slot = changed[i];
+        if (!in_range(slot) || (OP == kFork && !in_range(slots[i]))) { fail(kBadSlot); continue; }
+        const unsigned bit = 1u << (slot & 31);
+        if (atomicOr(&seen[slot >> 5], bit) & bit) fail(kBadSlot);
+        const int len = s.lens[slot];
+        if (len < 0 || len > cap) fail(kBadPage);
+        if (OP == kFork && len != 0) fail(kOccupied);
+        if (OP == kReserve && (int64_t)len + arg > cap) fail(kTooLong);
+        if (OP == kFork) {
+            const int from = s.lens[slots[i]];
+            if (from < 0 || from > cap) fail(kBadPage);
+        }
+    }
+    __syncthreads();
+    if (!err && OP != kReserve)
+        for (int i = warp; i < n; i += kMeta / 32) {
+            const int slot = slots[i];
+            if (OP == kFork && (seen[slot >> 5] >> (slot & 31) & 1)) { fail(kBadSlot); continue; }
+            if (!row_ok(s, slot, s.lens[slot], lane)) fail(kBadPage);
+        }
+    __syncthreads();
+    int total = 0;
+    if (!err && OP != kFree) {
+        for (int i0 = 0; i0 < n; i0 += kMeta) {
+            const int i = i0 + tid;
+            int need = 0, all;
+            if (i < n) {
+                const int len = s.lens[slots[i]];
+                if (OP == kReserve) need = pages_of(len + arg, s.page) - pages_of(len, s.page);
+                else need = arg ? pages_of(len, s.page) : (len % s.page ? 1 : 0);
+            }
+            const int at = total + block_scan(need, sums, all);
+            if (i < n) s.offsets[i] = at;
+            total += all;
+        }
+        // more than the pool has: take_free would not need to look, and its list would not hold them
+        if (total > s.pages || !take_free(s, total, sums)) fail(kNoPages);
+    }
+    __syncthreads();
+    if (err) {
+        if (tid == 0) s.header[0] = err;
+        return;
+    }
+    for (int i = warp; i < n; i += kMeta / 32) {
+        const int slot = slots[i], len = s.lens[slot];
+        int *row = s.tables + (size_t)slot * s.max_pages;
+        __syncwarp();
+        if (OP == kReserve) {
+            const int have = pages_of(len, s.page), need = pages_of(len + arg, s.page) - have;
+            for (int j = lane; j < need; j += 32) {
+                const int p = s.copies[3 * (size_t)(s.offsets[i] + j) + 1];
+                row[have + j] = p;
+                s.refs[p] = 1;
+            }
+            if (lane == 0) s.lens[slot] = len + arg;
+        } else if (OP == kFree) {
+            for (int j = lane; j < pages_of(len, s.page); j += 32) {
+                atomicSub(&s.refs[row[j]], 1);
+                row[j] = -1;
+            }
+            if (lane == 0) s.lens[slot] = 0;
+        } else {
+            int *to = s.tables + (size_t)dst[i] * s.max_pages;
+            const int shared = arg ? 0 : len / s.page;
+            for (int j = lane; j < pages_of(len, s.page); j += 32) {
+                const int p = row[j];
+                if (j < shared) {
+                    to[j] = p;
+                    atomicAdd(&s.refs[p], 1);
+                } else {
+                    int *c = s.copies + 3 * (size_t)(s.offsets[i] + j - shared);
+                    c[0] = p;
+                    c[2] = min(s.page, len - j * s.page);
+                    to[j] = c[1];
+                    s.refs[c[1]] = 1;
+                }
+            }
+            if (lane == 0) s.lens[dst[i]] = len;
+        }
+    }
+    if (OP == kFork && tid == 0) s.header[1] = total;
+}
+
+// Live pages are counted, then the free ones below that number meet the live ones at or above it, both in ascending order.
+__global__ void __launch_bounds__(kMeta) kv_compact_kernel(const cq_kv_cache cache) {
+    __shared__ int sums[32], stop;
+    const State s = state_of(cache);
+    const int tid = threadIdx.x;
+    cq_pdl_wait();
+    if (tid == 0) {
+        stop = s.header[0];
+        s.header[1] = 0;
+    }
+    __syncthreads();
+    if (stop) return;
+    int mine = 0, live;
+    for (int p = tid; p < s.pages; p += kMeta) mine += s.refs[p] > 0;
+    block_scan(mine, sums, live);
+    int holes = 0, movers = 0;
+    for (int p0 = 0; p0 < s.pages; p0 += kMeta) {
+        const int p = p0 + tid;
+        const bool used = p < s.pages && s.refs[p] > 0;
+        const bool hole = p < live && !used, mover = p >= live && used;
+        int nh, nm;
+        const int ah = block_scan(hole, sums, nh), am = block_scan(mover, sums, nm);
+        if (hole) s.copies[3 * (size_t)(holes + ah) + 1] = p;
+        if (mover) {
+            s.copies[3 * (size_t)(movers + am)] = p;
+            s.copies[3 * (size_t)(movers + am) + 2] = s.page;
+        }
+        if (p >= live && p < s.pages) s.map[p] = -1;
+        holes += nh;
+        movers += nm;
+    }
+    __syncthreads();
+    for (int m = tid; m < movers; m += kMeta) {         // as many as holes: both are live - (live pages below `live`)
+        const int from = s.copies[3 * (size_t)m], to = s.copies[3 * (size_t)m + 1];
+        s.refs[to] = s.refs[from];
+        s.refs[from] = 0;
+        s.map[from] = to;
+    }
+    __syncthreads();
+    if (tid == 0) {
+        s.header[1] = movers;
+        s.header[2] = live;
+    }
+}
+
+// The listed copies over all layers, keys and values.  A warp moves pieces of kPiece bytes, eight 16-byte loads of a lane in flight
+// before the first store.  REMAP: the table entries of moved pages follow (compaction).
+constexpr int kPiece = 4096, kCopyThreads = 256;
+template <bool REMAP>
+__global__ void __launch_bounds__(kCopyThreads) kv_copy_kernel(const cq_kv_cache cache) {
+    const State s = state_of(cache);
+    const int lane = threadIdx.x & 31;
+    cq_pdl_wait();
+    const int n = s.header[1];
+    if (n == 0) return;
+    const int row_bytes = cache.head_dim * elem_bytes(cache.elem);
+    const unsigned pieces = (unsigned)(s.page * row_bytes + kPiece - 1) / kPiece, heads = cache.kv_heads;
+    const unsigned per_copy = 2u * cache.layers * heads * pieces;
+    const int64_t page_bytes = (int64_t)s.page * row_bytes;
+    const unsigned total = (unsigned)n * per_copy, warps = gridDim.x * (kCopyThreads / 32);
+    for (unsigned u = blockIdx.x * (kCopyThreads / 32) + (threadIdx.x >> 5); u < total; u += warps) {
+        const unsigned c = u / per_copy, r = u % per_copy, seg = r / pieces, piece = r % pieces, layer_kv = seg / heads, head = seg % heads;
+        const int bytes = min(s.copies[3 * (size_t)c + 2] * row_bytes - (int)piece * kPiece, kPiece);
+        if (bytes <= 0) continue;
+        uint8_t *pool = reinterpret_cast<uint8_t *>(layer_kv & 1 ? cache.v : cache.k);
+        const int64_t layer = (int64_t)(layer_kv >> 1) * cache.pages;
+        const uint4 *from = reinterpret_cast<const uint4 *>(pool + ((layer + s.copies[3 * (size_t)c]) * heads + head) * page_bytes + piece * kPiece) + lane;
+        uint4 *to = reinterpret_cast<uint4 *>(pool + ((layer + s.copies[3 * (size_t)c + 1]) * heads + head) * page_bytes + piece * kPiece) + lane;
+        uint4 w[kPiece / 512];
+#pragma unroll
+        for (int i = 0; i < kPiece / 512; ++i)
+            if (i * 512 + lane * 16 < bytes) w[i] = from[32 * i];
+#pragma unroll
+        for (int i = 0; i < kPiece / 512; ++i)
+            if (i * 512 + lane * 16 < bytes) to[32 * i] = w[i];
+    }
+    if constexpr (REMAP) {
+        const int live = s.header[2];
+        const int64_t entries = (int64_t)s.max_seqs * s.max_pages;
+        for (int64_t e = (int64_t)blockIdx.x * kCopyThreads + threadIdx.x; e < entries; e += (int64_t)gridDim.x * kCopyThreads) {
+            const int p = s.tables[e];
+            if (p >= live && p < s.pages) s.tables[e] = s.map[p];
+        }
+    }
+}
+
+__global__ void __launch_bounds__(256) kv_reset_kernel(const cq_kv_cache cache) {
+    cq_pdl_wait();
+    const State s = state_of(cache);
+    const int64_t n = (int64_t)state_ints(s.pages, s.max_seqs, s.max_pages), t0 = s.tables - s.header, t1 = s.offsets - s.header;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) s.header[i] = i >= t0 && i < t1 ? -1 : 0;
+}
+
+// ---- new keys and values ----
+template <typename T, int N> struct alignas(sizeof(T) * N < 16 ? sizeof(T) * N : 16) Vec { T v[N]; };
+__device__ __forceinline__ float to_f(float x) { return x; }
+__device__ __forceinline__ float to_f(__half x) { return __half2float(x); }
+__device__ __forceinline__ float to_f(__nv_bfloat16 x) { return __bfloat162float(x); }
+template <typename T> __device__ __forceinline__ T from_f(float x);
+template <> __device__ __forceinline__ float from_f<float>(float x) { return x; }
+template <> __device__ __forceinline__ __half from_f<__half>(float x) { return __float2half_rn(x); }
+template <> __device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
+
+struct AppendArgs {
+    const int *slots;
+    const void *q, *k, *v;
+    void *q_out;
+    const float *cosv, *sinv;
+    int64_t q_stride, k_stride, v_stride;
+    int layer, batch, t, hq, max_pos, neox;
+};
+
+// A thread takes four rotary pairs of one head: eight consecutive elements (interleaved), or four and the four half a head further.
+// grid.x covers the heads of q, k and v of a row, grid.y the rows; one read and one write of each element, which is the bound.
+template <typename In, typename T>
+__global__ void __launch_bounds__(128) kv_append_kernel(const cq_kv_cache cache, const AppendArgs a) {
+    extern __shared__ unsigned seen[];
+    const State s = state_of(cache);
+    cq_pdl_launch_dependents();
+    cq_pdl_wait();
+    const bool stopped = __syncthreads_or(s.header[0]) != 0;        // other CTAs may add a fault: one answer for this one
+    if (blockIdx.x == 0 && blockIdx.y == 0 && !stopped) {           // a slot named twice would have two writers for its positions
+        for (int i = threadIdx.x; i < (s.max_seqs + 31) / 32; i += 128) seen[i] = 0;
+        __syncthreads();
+        for (int i = threadIdx.x; i < a.batch; i += 128) {
+            const int slot = a.slots[i];
+            if (slot >= 0 && slot < s.max_seqs && (atomicOr(&seen[slot >> 5], 1u << (slot & 31)) >> (slot & 31) & 1)) atomicCAS(s.header, kOk, kBadSlot);
+        }
+    }
+    const int d = cache.head_dim, per = d / 8, hkv = cache.kv_heads, hq = a.q ? a.hq : 0;
+    const int unit = blockIdx.x * 128 + threadIdx.x, head = unit / per, x = unit % per;
+    if (head >= hq + 2 * hkv) return;
+    const int first = a.neox ? 4 * x : 8 * x, second = a.neox ? first + d / 2 : first + 4;
+    for (int64_t row = blockIdx.y; row < (int64_t)a.batch * a.t; row += gridDim.y) {
+        const int b = (int)(row / a.t), slot = a.slots[b];
+        int pos = -1, page = -1, code = kBadSlot;
+        if (stopped) code = -1;
+        else if (slot >= 0 && slot < s.max_seqs) {
+            pos = s.lens[slot] - a.t + (int)(row % a.t);
+            code = kBadPosition;
+            if (pos >= 0 && pos < s.max_pages * s.page && (!a.cosv || pos < a.max_pos)) {
+                page = s.tables[(size_t)slot * s.max_pages + pos / s.page];
+                code = page >= 0 && page < s.pages ? kOk : kBadPage;
+            }
+        }
+        const bool is_q = head < hq, is_v = head >= hq + hkv;
+        if (code > kOk && x == 0) atomicCAS(s.header, kOk, code);
+        if (code != kOk && !is_q) continue;
+        const In *src = reinterpret_cast<const In *>(is_q ? a.q : is_v ? a.v : a.k) + row * (is_q ? a.q_stride : is_v ? a.v_stride : a.k_stride) +
+                        (int64_t)(is_q ? head : is_v ? head - hq - hkv : head - hq) * d;
+        const Vec<In, 4> lo = *reinterpret_cast<const Vec<In, 4> *>(src + first), hi = *reinterpret_cast<const Vec<In, 4> *>(src + second);
+        Vec<T, 4> out_lo, out_hi;
+        if (is_v || !a.cosv) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) { out_lo.v[i] = from_f<T>(to_f(lo.v[i])); out_hi.v[i] = from_f<T>(to_f(hi.v[i])); }
+        } else {
+            float4 c = make_float4(0.f, 0.f, 0.f, 0.f), n = c;
+            if (code == kOk) {
+                c = *reinterpret_cast<const float4 *>(a.cosv + (int64_t)pos * (d / 2) + 4 * x);
+                n = *reinterpret_cast<const float4 *>(a.sinv + (int64_t)pos * (d / 2) + 4 * x);
+            }
+            const float cs[4] = {c.x, c.y, c.z, c.w}, sn[4] = {n.x, n.y, n.z, n.w};
+            float p0[4], p1[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                p0[i] = a.neox ? to_f(lo.v[i]) : i < 2 ? to_f(lo.v[2 * (i & 1)]) : to_f(hi.v[2 * (i & 1)]);
+                p1[i] = a.neox ? to_f(hi.v[i]) : i < 2 ? to_f(lo.v[2 * (i & 1) + 1]) : to_f(hi.v[2 * (i & 1) + 1]);
+            }
+            float r0[4], r1[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {               // the operations of cq_rope_store_kv_f32
+                r0[i] = __fmaf_rn(p0[i], cs[i], -__fmul_rn(p1[i], sn[i]));
+                r1[i] = __fmaf_rn(p0[i], sn[i], __fmul_rn(p1[i], cs[i]));
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                out_lo.v[i] = from_f<T>(a.neox ? r0[i] : i & 1 ? r1[i >> 1] : r0[i >> 1]);
+                out_hi.v[i] = from_f<T>(a.neox ? r1[i] : i & 1 ? r1[2 + (i >> 1)] : r0[2 + (i >> 1)]);
+            }
+        }
+        T *dst;
+        if (is_q) {
+            if (code != kOk)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) out_lo.v[i] = out_hi.v[i] = from_f<T>(0.0f);
+            dst = reinterpret_cast<T *>(a.q_out) + (row * hq + head) * d;
+        } else {
+            const int h = is_v ? head - hq - hkv : head - hq;
+            dst = reinterpret_cast<T *>(is_v ? cache.v : cache.k) +
+                  ((((int64_t)a.layer * s.pages + page) * hkv + h) * s.page + pos % s.page) * d;
+        }
+        *reinterpret_cast<Vec<T, 4> *>(dst + first) = out_lo;
+        *reinterpret_cast<Vec<T, 4> *>(dst + second) = out_hi;
+    }
+}
+
+template <typename In, typename T> void append_launch(const cq_kv_cache &c, const AppendArgs &a, cudaStream_t st) {
+    const int units = ((a.q ? a.hq : 0) + 2 * c.kv_heads) * (c.head_dim / 8);
+    const int64_t rows = (int64_t)a.batch * a.t;
+    cq_launch_k(kv_append_kernel<In, T>, dim3((units + 127) / 128, (unsigned)(rows < 65535 ? rows : 65535)), dim3(128), (size_t)(c.max_seqs + 31) / 32 * 4, st,
+                c, a);
+}
+
+bool slots_ok(const cq_kv_cache *c, const int *a, const int *b, int n, const char *who) {
+    if (!cache_ok(c, who)) return false;
+    if (!a || !b || n < 0 || n > c->max_seqs) {
+        char msg[160];
+        std::snprintf(msg, sizeof msg, "%s: null list, or more slots than the cache has", who);
+        cq_set_status(CQ_ERR_BAD_ARG, msg);
+        return false;
+    }
+    return true;
+}
+size_t seen_bytes(const cq_kv_cache *c) { return (size_t)(c->max_seqs + 31) / 32 * 4; }
+
+}  // namespace
+
+extern "C" size_t cq_kv_state_ints(int pages, int max_seqs, int max_pages) {
+    return pages > 0 && max_seqs > 0 && max_pages > 0 ? state_ints(pages, max_seqs, max_pages) : 0;
+}
+
+extern "C" void cq_kv_reset(const cq_kv_cache *cache, void *stream) {
+    if (!cache_ok(cache, "kv_reset")) return;
+    const int64_t n = (int64_t)state_ints(cache->pages, cache->max_seqs, cache->max_pages);
+    cq_launch_k(kv_reset_kernel, dim3((unsigned)(n / 1024 < 1 ? 1 : n / 1024 < 1024 ? n / 1024 : 1024)), dim3(256), 0, (cudaStream_t)stream, *cache);
+    cq_check_launch("kv_reset");
+}
+
+extern "C" void cq_kv_reserve(const cq_kv_cache *cache, const int *slots, int n, int tokens, void *stream) {
+    if (!slots_ok(cache, slots, slots, n, "kv_reserve")) return;
+    if (tokens < 0) { cq_set_status(CQ_ERR_BAD_ARG, "kv_reserve: negative number of tokens"); return; }
+    if (n == 0 || tokens == 0) return;
+    cq_launch_k(kv_meta_kernel<kReserve>, dim3(1), dim3(kMeta), seen_bytes(cache), (cudaStream_t)stream, *cache, slots, nullptr, n, tokens);
+    cq_check_launch("kv_reserve");
+}
+
+extern "C" void cq_kv_fork(const cq_kv_cache *cache, const int *src, const int *dst, int n, int deep, void *stream) {
+    if (!slots_ok(cache, src, dst, n, "kv_fork")) return;
+    if (n == 0) return;
+    cq_launch_k(kv_meta_kernel<kFork>, dim3(1), dim3(kMeta), seen_bytes(cache), (cudaStream_t)stream, *cache, src, dst, n, deep ? 1 : 0);
+    cq_launch_k(kv_copy_kernel<false>, dim3(cq_sm_count() * 8), dim3(kCopyThreads), 0, (cudaStream_t)stream, *cache);
+    cq_check_launch("kv_fork");
+}
+
+extern "C" void cq_kv_free(const cq_kv_cache *cache, const int *slots, int n, void *stream) {
+    if (!slots_ok(cache, slots, slots, n, "kv_free")) return;
+    if (n == 0) return;
+    cq_launch_k(kv_meta_kernel<kFree>, dim3(1), dim3(kMeta), seen_bytes(cache), (cudaStream_t)stream, *cache, slots, nullptr, n, 0);
+    cq_check_launch("kv_free");
+}
+
+extern "C" void cq_kv_compact(const cq_kv_cache *cache, void *stream) {
+    if (!cache_ok(cache, "kv_compact")) return;
+    cq_launch_k(kv_compact_kernel, dim3(1), dim3(kMeta), 0, (cudaStream_t)stream, *cache);
+    cq_launch_k(kv_copy_kernel<true>, dim3(cq_sm_count() * 8), dim3(kCopyThreads), 0, (cudaStream_t)stream, *cache);
+    cq_check_launch("kv_compact");
+}
+
+extern "C" void cq_kv_append(const cq_kv_cache *cache, int layer, const int *slots, int batch, int t, const void *q, const void *k, const void *v, int in_elem,
+                             int hq, int64_t q_stride, int64_t k_stride, int64_t v_stride, const float *cosv, const float *sinv, int max_pos, int neox,
+                             void *q_out, void *stream) {
+    if (!slots_ok(cache, slots, slots, batch, "kv_append")) return;
+    if (!k || !v || t <= 0 || layer < 0 || layer >= cache->layers || !q != !q_out || (q && hq <= 0) || !cosv != !sinv || (cosv && max_pos <= 0) ||
+        (in_elem != CQ_F32 && in_elem != CQ_F16 && in_elem != CQ_BF16)) {
+        cq_set_status(CQ_ERR_BAD_ARG, "kv_append: null pointer, layer, head count, or element type out of range");
+        return;
+    }
+    const int es = elem_bytes(in_elem);
+    const int64_t width = (int64_t)cache->kv_heads * cache->head_dim, q_width = (int64_t)hq * cache->head_dim;
+    if (((k_stride | v_stride) * es) % 16 || (q && (q_stride * es) % 16) || k_stride < width || v_stride < width || (q && q_stride < q_width) ||
+        (((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)q_out | (uintptr_t)cosv | (uintptr_t)sinv) & 15)) {
+        cq_set_status(CQ_ERR_BAD_ARG, "kv_append: rows must be 16-byte aligned and not overlap");
+        return;
+    }
+    if (q && q == q_out && (in_elem != cache->elem || (q_stride != q_width && (int64_t)batch * t > 1))) {
+        cq_set_status(CQ_ERR_BAD_ARG, "kv_append: q_out may be q only with the same type and rows without gaps");
+        return;
+    }
+    if (batch == 0) return;
+    const AppendArgs a{slots, q, k, v, q_out, cosv, sinv, q_stride, k_stride, v_stride, layer, batch, t, hq, max_pos, neox};
+    cudaStream_t st = (cudaStream_t)stream;
+    switch (in_elem * 3 + cache->elem) {
+        case 0: append_launch<float, float>(*cache, a, st); break;
+        case 1: append_launch<float, __half>(*cache, a, st); break;
+        case 2: append_launch<float, __nv_bfloat16>(*cache, a, st); break;
+        case 3: append_launch<__half, float>(*cache, a, st); break;
+        case 4: append_launch<__half, __half>(*cache, a, st); break;
+        case 5: append_launch<__half, __nv_bfloat16>(*cache, a, st); break;
+        case 6: append_launch<__nv_bfloat16, float>(*cache, a, st); break;
+        case 7: append_launch<__nv_bfloat16, __half>(*cache, a, st); break;
+        default: append_launch<__nv_bfloat16, __nv_bfloat16>(*cache, a, st);
+    }
+    cq_check_launch("kv_append");
+}
+
+extern "C" int cq_kv_take_fault(const cq_kv_cache *cache, void *stream) {
+    if (!cache_ok(cache, "kv_take_fault")) return -1;
+    static const char *const text[] = {"", "a slot is out of range, named twice, or source and destination at once", "out of pages",
+                                       "a sequence would be longer than its table", "fork into a slot that is not empty", "a table names a page that is not there",
+                                       "a position before the sequence, or past its table or the rotary tables"};
+    int fault = 0;
+    const int zero = 0;
+    cudaStream_t st = (cudaStream_t)stream;
+    if (cudaMemcpyAsync(&fault, cache->state, sizeof fault, cudaMemcpyDeviceToHost, st) != cudaSuccess || cudaStreamSynchronize(st) != cudaSuccess ||
+        (fault && (cudaMemcpyAsync(cache->state, &zero, sizeof zero, cudaMemcpyHostToDevice, st) != cudaSuccess || cudaStreamSynchronize(st) != cudaSuccess))) {
+        cq_check_launch("kv_take_fault");
+        return -1;
+    }
+    if (fault) {
+        char msg[160];
+        std::snprintf(msg, sizeof msg, "kv cache: %s", fault > 0 && fault <= kBadPosition ? text[fault] : "unknown fault");
+        cq_set_status(CQ_ERR_BAD_ARG, msg);
+    }
+    return fault;
+}

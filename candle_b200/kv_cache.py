@@ -1,0 +1,230 @@
+"""A KV cache in pages, and the attention of a decode batch that reads it.
+
+candle's quantized models keep one tensor [batch, heads, positions, head_dim] per layer (candle-transformers/src/models/quantized_llama.rs:235-245): every
+sequence has its own copy of all it has read, and all have one length.  Here sequences ("slots") have their own lengths, their keys and values lie in pages
+of one pool, and a sequence that goes on from another one shares its full pages:
+
+    cache = PagedKvCache(layers, pages, page_size, kv_heads, head_dim, max_seqs, max_len)
+    cache.reserve([0], n)                               # positions for a prompt of n tokens
+    q = cache.append(layer, [0], k, v, q=q, rotary=(cos, sin))
+    cache.fork([0] * 7, range(1, 8))                    # seven more continuations of it
+    plan = cache.attention_plan(8, heads)               # one group: all eight share a prefix
+    ...                                                 # per step:
+    cache.reserve(slots, 1); plan.update(slots)
+    out = cache.attention(layer, q, plan)               # per layer
+
+Nothing here synchronises or looks at the device's numbers: a step can be captured into a CUDA graph (slots given as an int32 tensor).  What the device finds
+wrong - no page left, a slot named twice, ... - leaves the cache as it was, stops every later change, and is raised by `check()`.  Calls on one cache
+are ordered by the caller: one stream, or events between several.
+"""
+from __future__ import annotations
+
+import ctypes as C
+import math
+
+import numpy as np
+import torch
+
+from . import capi
+from .capi import CandleQError
+
+_ELEM = {torch.float32: capi.F32, torch.float16: capi.F16, torch.bfloat16: capi.BF16}
+
+
+class PagedKvCache:
+    """`pages` pages of `page_size` (16, 32, 64, 128) positions for all layers; at most `max_seqs` sequences of at most `max_len` positions.  `k`, `v`:
+    [layers, pages, kv_heads, page_size, head_dim]; `refs` [pages], `lens` [max_seqs] and `tables` [max_seqs, max_pages] (-1 behind a sequence's pages) are views
+    of the bookkeeping, int32.  `pools`: the two tensors, where the caller has made them."""
+
+    def __init__(self, layers: int, pages: int, page_size: int, kv_heads: int, head_dim: int, max_seqs: int, max_len: int, dtype: torch.dtype = torch.float32,
+                 device="cuda:0", pools=None):
+        self.device = torch.device(device)
+        if self.device.type != "cuda":
+            raise CandleQError("PagedKvCache needs a CUDA device: there is no CPU path")
+        if dtype not in _ELEM:
+            raise CandleQError(f"Expected f32/f16/bf16, got {dtype}")
+        if page_size <= 0 or max_len <= 0:
+            raise CandleQError("PagedKvCache: page_size and max_len must be positive")
+        max_pages = -(-max_len // page_size)
+        shape = (layers, pages, kv_heads, page_size, head_dim)
+        if min(shape) <= 0 or max_seqs <= 0:
+            raise CandleQError("PagedKvCache: sizes must be positive")
+        if pools is None:
+            pools = (torch.zeros(shape, dtype=dtype, device=self.device), torch.zeros(shape, dtype=dtype, device=self.device))
+        for t in pools:
+            if t.shape != shape or t.dtype != dtype or t.device != pools[0].device or not t.is_cuda or not t.is_contiguous():
+                raise CandleQError(f"PagedKvCache: the pools must be contiguous CUDA tensors {list(shape)} of {dtype}")
+        self.k, self.v = pools
+        self.device = self.k.device
+        lib = capi.lib()
+        # rounded up, so that a view of everything keeps its alignment
+        self.state = torch.zeros(capi.pad(lib.cq_kv_state_ints(pages, max_seqs, max_pages), 4), dtype=torch.int32, device=self.device)
+        self._c = capi.KvCache(self.k.data_ptr(), self.v.data_ptr(), self.state.data_ptr(), layers, pages, kv_heads, page_size, head_dim, max_seqs, max_pages,
+                               _ELEM[dtype])
+        self._p = C.byref(self._c)
+        self.layers, self.pages, self.page_size, self.kv_heads, self.head_dim = layers, pages, page_size, kv_heads, head_dim
+        self.max_seqs, self.max_len, self.dtype = max_seqs, max_pages * page_size, dtype
+        at = 16
+        self.refs, at = self.state[at:at + pages], at + pages
+        self.lens, at = self.state[at:at + max_seqs], at + max_seqs
+        self.tables = self.state[at:at + max_seqs * max_pages].view(max_seqs, max_pages)
+        self.reset()
+
+    # ---- helpers ----
+    def _call(self, fn, *args) -> None:
+        with capi.on_device(self.device):
+            fn(self._p, *args, capi.stream_of(self.device))
+        capi.check("PagedKvCache")
+
+    def slot_list(self, slots) -> torch.Tensor:
+        """Slots as the device reads them: int32, contiguous, on the cache's device.  Such a tensor is taken as it is."""
+        if not isinstance(slots, torch.Tensor):
+            slots = [slots] if isinstance(slots, int) else list(slots)
+            if any(not 0 <= int(s) < self.max_seqs for s in slots):
+                raise CandleQError(f"PagedKvCache: slots are 0 .. {self.max_seqs - 1}")
+            slots = torch.tensor(slots, dtype=torch.int32)
+        if slots.dim() != 1 or slots.is_floating_point() or slots.dtype == torch.bool:
+            raise CandleQError("PagedKvCache: slots must be a list of whole numbers")
+        if slots.numel() > self.max_seqs:
+            raise CandleQError(f"PagedKvCache: {slots.numel()} slots named, the cache has {self.max_seqs}")
+        return slots.to(device=self.device, dtype=torch.int32).contiguous()
+
+    # ---- pages ----
+    def reset(self) -> None:
+        """Every slot empty, every page free, no fault."""
+        self._call(capi.lib().cq_kv_reset)
+
+    def reserve(self, slots, tokens: int) -> None:
+        """`tokens` more positions for each of the slots.  The lowest free pages are taken, in the order of the list."""
+        s = self.slot_list(slots)
+        if tokens < 0 or tokens > self.max_len:
+            raise CandleQError(f"PagedKvCache.reserve: {tokens} tokens, a sequence holds 0 .. {self.max_len}")
+        self._call(capi.lib().cq_kv_reserve, s.data_ptr(), s.numel(), tokens)
+
+    def fork(self, src, dst) -> None:
+        """The empty slots dst[i] go on from src[i] (one source may be named many times): full pages are shared, a part-full last page is copied."""
+        self._fork(src, dst, 0)
+
+    def copy(self, src, dst) -> None:
+        """Like `fork`, with pages of their own for all positions."""
+        self._fork(src, dst, 1)
+
+    def _fork(self, src, dst, deep: int) -> None:
+        a, b = self.slot_list(src), self.slot_list(dst)
+        if a.numel() != b.numel():
+            raise CandleQError("PagedKvCache.fork: one destination for each source")
+        self._call(capi.lib().cq_kv_fork, a.data_ptr(), b.data_ptr(), a.numel(), deep)
+
+    def free(self, slots) -> None:
+        """The slots become empty; pages that no other slot shares are free."""
+        s = self.slot_list(slots)
+        self._call(capi.lib().cq_kv_free, s.data_ptr(), s.numel())
+
+    def compact(self) -> None:
+        """Moves the live pages to the front of the pool (n live pages: the numbers 0 .. n - 1), tables included."""
+        self._call(capi.lib().cq_kv_compact)
+
+    def check(self) -> None:
+        """Raises if a call since the last check found a fault on the device (synchronises the stream)."""
+        with capi.on_device(self.device):
+            fault = capi.lib().cq_kv_take_fault(self._p, capi.stream_of(self.device))
+        if fault:
+            capi.check("PagedKvCache")
+            raise CandleQError("PagedKvCache: the state could not be read")
+
+    # ---- keys and values ----
+    def _rows(self, t: torch.Tensor, name: str, batch: int, heads: int | None, tokens: int | None):
+        """`t` as [batch, tokens, heads, head_dim] with heads side by side and aligned rows at one distance; (tensor, row distance)."""
+        if t.dim() != 4 or t.shape[0] != batch or t.shape[3] != self.head_dim or (heads is not None and t.shape[2] != heads) or \
+                (tokens is not None and t.shape[1] != tokens) or t.device != self.device:
+            raise CandleQError(f"PagedKvCache: {name} must be [batch, tokens, heads, {self.head_dim}] on {self.device}, got {list(t.shape)}")
+        es, d = t.element_size(), self.head_dim
+        stride = t.stride(1) if t.shape[1] > 1 else t.stride(0)
+        if t.stride(3) != 1 or (t.shape[2] > 1 and t.stride(2) != d) or stride < t.shape[2] * d or (t.shape[0] > 1 and t.stride(0) != stride * t.shape[1]) or \
+                stride * es % 16 or t.data_ptr() % 16:
+            t = t.contiguous() if not t.is_contiguous() else t.clone()
+            stride = t.shape[2] * d
+        return t, stride
+
+    def append(self, layer: int, slots, k: torch.Tensor, v: torch.Tensor, q: torch.Tensor | None = None, rotary=None, neox: bool = False):
+        """Keys and values [batch, tokens, kv_heads, head_dim] (f32, f16, bf16) of the last `tokens` positions of the slots, which `reserve` has added.  With
+        `rotary` = (cos, sin), each [positions, head_dim / 2] f32, k and q are rotated at their sequence's own positions: pairs (2i, 2i + 1), with `neox`
+        (i, i + head_dim / 2).  Returns q [batch, tokens, heads, head_dim] in the cache's type, or None."""
+        s = self.slot_list(slots)
+        if not 0 <= layer < self.layers:
+            raise CandleQError(f"PagedKvCache.append: layer {layer} of {self.layers}")
+        if k.dtype not in _ELEM or v.dtype != k.dtype or (q is not None and q.dtype != k.dtype):
+            raise CandleQError("PagedKvCache.append: q, k and v must be of one type, f32, f16 or bf16")
+        b = s.numel()
+        if b == 0 or k.dim() != 4 or k.shape[1] == 0:
+            raise CandleQError("PagedKvCache.append: no slots or no tokens")
+        k, ks = self._rows(k, "k", b, self.kv_heads, None)
+        v, vs = self._rows(v, "v", b, self.kv_heads, k.shape[1])
+        qs, out, heads = 0, None, 0
+        if q is not None:
+            q, qs = self._rows(q, "q", b, None, k.shape[1])
+            heads = q.shape[2]
+            out = torch.empty(q.shape, dtype=self.dtype, device=self.device)
+        cos = sin = None
+        if rotary is not None:
+            cos, sin = rotary
+            for t in (cos, sin):
+                if t.dtype != torch.float32 or t.dim() != 2 or t.shape[1] != self.head_dim // 2 or t.shape[0] != cos.shape[0] or t.shape[0] == 0 or \
+                        not t.is_contiguous() or t.device != self.device or t.data_ptr() % 16:
+                    raise CandleQError(f"PagedKvCache.append: rotary tables must be contiguous, aligned f32 [positions, {self.head_dim // 2}] on {self.device}")
+        ptr = lambda t: None if t is None else t.data_ptr()
+        self._call(capi.lib().cq_kv_append, layer, s.data_ptr(), b, k.shape[1], ptr(q), k.data_ptr(), v.data_ptr(), _ELEM[k.dtype], heads, qs, ks, vs, ptr(cos),
+                   ptr(sin), 0 if cos is None else cos.shape[0], int(neox), ptr(out))
+        return out
+
+    # ---- attention ----
+    def attention_plan(self, batch: int, heads: int, queries: int = 1, groups=None) -> "AttentionPlan":
+        """What `attention` needs for a batch of this shape: `queries` tokens of each of `batch` sequences.  `groups`: how many neighbouring sequences go on from
+        the same prompt, a list that adds up to `batch`; None: all of them."""
+        return AttentionPlan(self, batch, heads, queries, groups)
+
+    def attention(self, layer: int, q: torch.Tensor, plan: "AttentionPlan", scale: float | None = None) -> torch.Tensor:
+        """softmax(scale q K^T) V of the last `queries` positions of the plan's slots, each over the positions up to its own; scale: 1 / sqrt(head_dim).
+        q: [batch, queries, heads, head_dim] of the cache's type.  A sequence without positions gives zeros."""
+        if plan.cache is not self:
+            raise CandleQError("PagedKvCache.attention: the plan belongs to another cache")
+        if not 0 <= layer < self.layers:
+            raise CandleQError(f"PagedKvCache.attention: layer {layer} of {self.layers}")
+        if not plan.updated:
+            raise CandleQError("PagedKvCache.attention: the plan has no slots yet (AttentionPlan.update)")
+        if q.dtype != self.dtype:
+            raise CandleQError(f"PagedKvCache.attention: q must be of the cache's type, {self.dtype}")
+        q, stride = self._rows(q, "q", plan.batch, plan.heads, plan.queries)
+        out = torch.empty((plan.batch, plan.queries, plan.heads, self.head_dim), dtype=self.dtype, device=self.device)
+        self._call(capi.lib().cq_prefix_attention, layer, plan._p, q.data_ptr(), stride, out.data_ptr(), 1.0 / math.sqrt(self.head_dim) if scale is None else scale)
+        return out
+
+
+class AttentionPlan:
+    """The division of a batch's attention into pieces, and the room for their results.  `update(slots)` makes it for the lengths and tables as they are, once a
+    step; all layers use it.  One plan serves one stream at a time."""
+
+    def __init__(self, cache: PagedKvCache, batch: int, heads: int, queries: int, groups):
+        groups = [batch] if groups is None else [int(g) for g in groups]
+        if any(g <= 0 for g in groups) or sum(groups) != batch:
+            raise CandleQError(f"attention_plan: groups {groups} must be positive and add up to the batch of {batch}")
+        self.cache, self.batch, self.heads, self.queries, self.updated = cache, batch, heads, queries, False
+        self._c = capi.PrefixPlan(batch=batch, queries=queries, heads=heads, groups=len(groups))
+        self._p = C.byref(self._c)
+        sizes = np.array(groups, dtype=np.int32)
+        shapes = np.zeros(3 * (len(groups) + 1), dtype=np.int32)
+        with capi.on_device(cache.device):
+            if capi.lib().cq_prefix_plan_shape(cache._p, self._p, sizes.ctypes.data, shapes.ctypes.data):
+                capi.check("attention_plan")
+        self._ints = torch.zeros(self._c.n_ints, dtype=torch.int32, device=cache.device)
+        self._scratch = torch.empty(self._c.n_floats, dtype=torch.float32, device=cache.device)
+        self._ints[16:16 + shapes.size].copy_(torch.from_numpy(shapes))
+        self._c.ints, self._c.scratch = self._ints.data_ptr(), self._scratch.data_ptr()
+
+    def update(self, slots) -> None:
+        s = self.cache.slot_list(slots)
+        if s.numel() != self.batch:
+            raise CandleQError(f"AttentionPlan.update: {s.numel()} slots for a batch of {self.batch}")
+        self._slots = s             # read on the device after this returns
+        self.cache._call(capi.lib().cq_prefix_plan_update, self._p, s.data_ptr())
+        self.updated = True

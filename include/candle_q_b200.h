@@ -405,6 +405,86 @@ void cq_qknorm_rope_store_kv_f32(float *q, float *k, const float *v, const float
  * since the last query (synchronises the device, clears the flag, sets status 1). */
 int cq_glue_position_overflow_flag(void);
 
+/* ------------------------------------------------------------------------------------------------
+ * Paged KV cache: sequences of their own lengths over one pool of pages, pages shared by the sequences that go on from the
+ * same prompt.  (candle's quantized models keep one [batch, heads, positions, dim] tensor per layer,
+ * candle-transformers/src/models/quantized_llama.rs:235-245; no counterpart for the pages.)
+ *   k, v  : [layers, pages, kv_heads, page_size, head_dim], 16-byte aligned; elem: 0 f32, 1 f16, 2 bf16; page_size 16, 32, 64 or
+ *           128; head_dim 64 or 128.
+ *   state : cq_kv_state_ints() ints, zero before the first call except the tables (-1); cq_kv_reset writes that.  In it, in this
+ *           order: 16 ints of header, refs[pages] (sequences that hold a page), lens[max_seqs], tables[max_seqs][max_pages] (the
+ *           pages of a sequence in order, -1 behind them), and working room.
+ * A slot is a row of lens / tables; an empty one has length 0.  Lists of slots are device ints.  All of it is stream-ordered,
+ * nothing synchronises, and a call can be captured into a graph; calls on one cache are ordered by the caller.
+ * What only the device can see is checked there, before anything is changed: a slot out of range or named twice, too few free
+ * pages, a sequence beyond max_pages, a fork into an occupied slot, a page number out of range.  The call then does nothing,
+ * leaves its fault in header[0], and so does every later call that would change the cache until cq_kv_take_fault has
+ * read it.
+ *   cq_kv_reserve : `tokens` more positions for each slot; pages are taken lowest number first, in the order of the list.
+ *   cq_kv_fork    : slot dst[i] (empty) goes on from src[i]: the full pages are shared, a last page that is only part full is
+ *                   copied into a fresh one, its valid rows alone.  deep != 0: all pages are copied, none shared.
+ *                   dst and src have no slot in common.
+ *   cq_kv_free    : the slots become empty; a page that no sequence holds any more is free.
+ *   cq_kv_compact : live pages move to the front of the pool: those numbered n = (live pages) or higher into the free ones
+ *                   below n, both in ascending order; all tables follow.
+ *   cq_kv_append  : the last t positions of each slot (reserved before) get keys and values; with cosv / sinv
+ *                   ([max_pos, head_dim / 2] f32) q and k are rotated at those positions first - pairs (2i, 2i+1), neox != 0:
+ *                   (i, i + head_dim / 2).  q, k, v: batch * t rows of q_stride / k_stride / v_stride elements of type
+ *                   in_elem, heads side by side, rows 16-byte aligned; q_out: [batch, t, hq, head_dim] of the cache's type
+ *                   (it may be q itself where type and stride agree).  q and q_out may be null.  Sums in f32, one rounding.
+ *                   A row that cannot be stored gives q_out zeros and a fault.
+ *   cq_kv_take_fault : the fault of the cache (0: none; 1 slot, 2 out of pages, 3 too long, 4 occupied, 5 page number, 6 position),
+ *                   which is cleared; synchronises the stream and sets the status.  -1: the CUDA call failed. */
+typedef struct cq_kv_cache {
+    void *k, *v;
+    int *state;
+    int layers, pages, kv_heads, page_size, head_dim, max_seqs, max_pages, elem;
+} cq_kv_cache;
+size_t cq_kv_state_ints(int pages, int max_seqs, int max_pages);
+void cq_kv_reset(const cq_kv_cache *cache, void *stream);
+void cq_kv_reserve(const cq_kv_cache *cache, const int *slots, int n, int tokens, void *stream);
+void cq_kv_fork(const cq_kv_cache *cache, const int *src, const int *dst, int n, int deep, void *stream);
+void cq_kv_free(const cq_kv_cache *cache, const int *slots, int n, void *stream);
+void cq_kv_compact(const cq_kv_cache *cache, void *stream);
+void cq_kv_append(const cq_kv_cache *cache, int layer, const int *slots, int batch, int t, const void *q, const void *k, const void *v, int in_elem,
+                  int hq, int64_t q_stride, int64_t k_stride, int64_t v_stride, const float *cosv, const float *sinv, int max_pos, int neox,
+                  void *q_out, void *stream);
+int cq_kv_take_fault(const cq_kv_cache *cache, void *stream);
+
+/* Attention of a decode batch over the pages of a cache, with the pages that sequences share read once for all of them:
+ * out[b, t] = softmax(scale q K^T) V over the first len_b - queries + 1 + t positions of slot b (a context without positions gives
+ * zeros), query heads in groups of heads / kv_heads per KV head.  The batch is cut into `groups` runs of neighbouring sequences; the pages that all
+ * sequences of a run have in common at their start are found on the device, by comparing the tables.
+ *   cq_prefix_plan_shape  : fills row_tile, ctas, shared_items, n_ints, n_floats of a plan whose batch, queries, heads and groups are set, and `shapes`
+ *                           (host, 3 * (groups + 1) ints, or null).  group_sizes: host, sequences per group, null for one group or groups of one.  Host
+ *                           only; 0 or, with the status set, 1.  The caller then gives the plan `ints` (device, n_ints) and `scratch` (device, n_floats),
+ *                           32-byte aligned, and copies `shapes` to ints + 16.
+ *   cq_prefix_plan_update : the plan for the slots' lengths and tables as they are when it runs; once a step, for all layers.
+ *   cq_prefix_attention   : one layer.  q: batch * queries rows of q_stride elements of the cache's type, heads side by side, 16-byte aligned;
+ *                           out: [batch, queries, heads, head_dim] of that type.  Scores, sums and the join in f32; 16-bit types: the weights are
+ *                           rounded to the type for the second product.  The order of additions depends on the plan (lengths, tables, group sizes) and the device.
+ * A plan and its scratch serve one stream at a time.  At most 4096 queries and 32 query heads per KV head.  A slot or page number out of range is a fault of the
+ * cache (cq_kv_take_fault) and reads nothing. */
+typedef struct cq_prefix_plan {
+    int batch, queries, heads, groups;
+    int row_tile, ctas, shared_items;
+    int64_t n_ints, n_floats;
+    int *ints;
+    float *scratch;
+} cq_prefix_plan;
+int cq_prefix_plan_shape(const cq_kv_cache *cache, cq_prefix_plan *plan, const int *group_sizes, int *shapes);
+void cq_prefix_plan_update(const cq_kv_cache *cache, const cq_prefix_plan *plan, const int *slots, void *stream);
+void cq_prefix_attention(const cq_kv_cache *cache, int layer, const cq_prefix_plan *plan, const void *q, int64_t q_stride, void *out, float scale,
+                         void *stream);
+
+/* From rows of logits (row_stride elements apart, any alignment): logprob[r] of tokens[r] (both null: none asked for), the entropy of the row's
+ * distribution in nats, and its `top` (0 .. 32, at most vocab) most probable tokens, [rows, top], descending, the lower index first among equals.  Sums
+ * and results in f32, one read of the logits.  A token < 0: 0; >= vocab: NaN.  A row with a NaN or +inf, or nothing but -inf: NaN, ids -1.
+ * scratch: cq_token_logprobs_scratch_bytes bytes (0: sizes not covered), 16-byte aligned.  The 16-byte units that hold a row's ends are read whole. */
+size_t cq_token_logprobs_scratch_bytes(int rows, int vocab, int top);
+void cq_token_logprobs(const void *logits, int elem, int64_t row_stride, int rows, int vocab, const int64_t *tokens, int top, float *logprob,
+                       float *entropy, float *top_logprobs, int64_t *top_ids, void *scratch, void *stream);
+
 /* 1 (default): decode-path kernels (quantize, GEMV, glue, attention) are launched as programmatic dependents of their
  * predecessor in the stream, so their prologue and first weight copies overlap its tail; 0: plain launches. */
 void cq_set_pdl(int on);
