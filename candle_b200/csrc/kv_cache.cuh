@@ -10,7 +10,7 @@
 namespace cq_kv {
 
 constexpr int kHeader = 16;             // ints; [0] fault code, [1] copies listed by the last page operation
-enum Fault : int { kOk = 0, kBadSlot = 1, kNoPages = 2, kTooLong = 3, kOccupied = 4, kBadPage = 5, kBadPosition = 6 };
+enum Fault : int { kOk = 0, kBadSlot = 1, kNoPages = 2, kTooLong = 3, kOccupied = 4, kBadPage = 5, kBadPosition = 6, kTimeout = 7 };
 
 struct State {
     int *header, *refs, *lens, *tables, *offsets, *copies, *map;        // copies: (source, destination, rows) per page

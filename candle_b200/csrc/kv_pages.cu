@@ -509,7 +509,7 @@ extern "C" int cq_kv_take_fault(const cq_kv_cache *cache, void *stream) {
     if (!cache_ok(cache, "kv_take_fault")) return -1;
     static const char *const text[] = {"", "a slot is out of range, named twice, or source and destination at once", "out of pages",
                                        "a sequence would be longer than its table", "fork into a slot that is not empty", "a table names a page that is not there",
-                                       "a position before the sequence, or past its table or the rotary tables"};
+                                       "a position before the sequence, or past its table or the rotary tables", "a wait inside the attention gave up"};
     int fault = 0;
     const int zero = 0;
     cudaStream_t st = (cudaStream_t)stream;
@@ -520,8 +520,8 @@ extern "C" int cq_kv_take_fault(const cq_kv_cache *cache, void *stream) {
     }
     if (fault) {
         char msg[160];
-        std::snprintf(msg, sizeof msg, "kv cache: %s", fault > 0 && fault <= kBadPosition ? text[fault] : "unknown fault");
-        cq_set_status(CQ_ERR_BAD_ARG, msg);
+        std::snprintf(msg, sizeof msg, "kv cache: %s", fault > 0 && fault <= kTimeout ? text[fault] : "unknown fault");
+        cq_set_status(fault == kTimeout ? CQ_ERR_TIMEOUT : CQ_ERR_BAD_ARG, msg);
     }
     return fault;
 }

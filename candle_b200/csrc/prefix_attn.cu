@@ -276,7 +276,7 @@ bool plan_ready(const cq_prefix_plan *p, const Shape &s, const char *who) {
 extern "C" int cq_prefix_plan_shape(const cq_kv_cache *cache, cq_prefix_plan *plan, const int *group_sizes, int *shapes) {
     Shape s;
     if (!shape_ok(cache, plan, "prefix_plan_shape", s)) return 1;
-    s.row_tile = plan->row_tile = 32;
+    s.row_tile = plan->row_tile = s.elem == CQ_F32 ? 32 : 128;
     s.ctas = plan->ctas = 2 * cq_sm_count();
     int64_t items = 0, seqs = 0;
     for (int g = 0; g < plan->groups; ++g) {
@@ -314,7 +314,8 @@ extern "C" void cq_prefix_attention(const cq_kv_cache *cache, int layer, const c
     }
     const Call c = call_of(plan, s);
     cudaStream_t st = (cudaStream_t)stream;
-    simt_launch(c, *cache, layer, q, q_stride, scale, st);
+    if (s.elem == CQ_F32) simt_launch(c, *cache, layer, q, q_stride, scale, st);
+    else if (!mma_launch(c, *cache, layer, q, q_stride, scale, st)) return;
     if (s.head_dim == 128) join_launch<128>(c, out, st);
     else join_launch<64>(c, out, st);
     cq_check_launch("prefix_attention");

@@ -86,5 +86,6 @@ __host__ __device__ inline int64_t part_of(const Shape &s, int shared, int item,
 
 // One CTA's kernel for all segments, by element type (prefix_attn_simt.cu, prefix_attn_mma.cu).
 void simt_launch(const Call &c, const cq_kv_cache &cache, int layer, const void *q, int64_t q_stride, float scale, cudaStream_t st);
+bool mma_launch(const Call &c, const cq_kv_cache &cache, int layer, const void *q, int64_t q_stride, float scale, cudaStream_t st);
 
 }  // namespace cq_attn

@@ -1,0 +1,351 @@
+// Segments of the shared-prefix attention (prefix_attn.cuh) on the tensor cores: f16 and bf16 caches.
+//
+// A tile is 128 rows x 128 keys.  S = Q K^T goes to tensor memory; thread r of the softmax warps owns row r, reads it there, and writes the weights
+// 2^(s c - m), c = scale log2 e, back over it in 16 bits as the first operand of O += P V.  m is the row's maximum so far, kept until a score passes
+// it by 2^8 (weights up to 256 are as good as any, the sum has the same factor): O is then scaled in tensor memory, which happens in the first tiles
+// only.  The sum adds the weights as rounded, so that rounding moves weight between keys but not the total.
+//
+// Keys and values come by tiled TMA copies, one box per page and 64 dims, 128-byte swizzle: K as it is for the first product (rows of K major), V
+// for the second with the rows as its K dimension (N major).  Rows of a tile behind the last key hold whatever the page or the tile before left
+// there: their scores are masked, their values set to zero before the second product, since 0 x NaN is not 0.
+//
+// Warps: 0-3 softmax (TMEM lanes 32 w ..), 4 copies, 5 MMA.  Within a CTA the products and the softmax of a tile follow one another (the weights lie where
+// the scores were: 256 columns a CTA); two CTAs per SM fill each other's gaps.
+#include <cuda.h>
+
+#include <mutex>
+
+#include "prefix_attn.cuh"
+#include "prompt_f16.cuh"
+
+namespace {
+using namespace cq_attn;
+using namespace cq_prompt;
+
+constexpr int kThreads = 192, kCols = 256, kHalfBytes = 128 * 128;       // a half: 128 rows of 64 elements
+constexpr int kS = 0, kO = 128;                                                          // columns of scores / weights and of outputs
+
+struct Bars { uint64_t q, k, v, s, p, o; };      // operands there (q, k, v), scores there (and Q, K free), weights there, outputs there (and V free)
+
+template <int D> struct Tiles {
+    uint8_t q[D / 64][kHalfBytes], k[D / 64][kHalfBytes], v[D / 64][kHalfBytes];
+    Bars bar;
+    uint32_t tmem;
+    int abort;
+};
+
+// 128-byte swizzle, 8-row groups 1024 bytes apart.  K-major operands ignore the low word's upper half; N-major ones find there the distance
+// between blocks of 64 columns.
+__device__ __forceinline__ uint64_t desc_sw(uint32_t lo) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(lo), "r"((1024u >> 4) | (1u << 14) | (2u << 29)));
+    return r;
+}
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+                 ::"r"(d), "l"(desc_sw(a)), "l"(desc_sw(b)), "r"(idesc), "r"(acc) : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+                 ::"r"(d), "r"(a), "l"(desc_sw(b)), "r"(idesc), "r"(acc) : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&v)[16]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+                 ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]),
+                 "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]) : "memory");
+}
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&v)[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+        "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};"
+        ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]),
+        "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]),
+        "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31]) : "memory");
+}
+__device__ __forceinline__ float ex2(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+// two weights in the type's 16 bits, and their sum as rounded
+template <bool BF16> __device__ __forceinline__ uint32_t pack(float a, float b, float &sum) {
+    uint32_t w;
+    if constexpr (BF16) {
+        asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(b), "f"(a));
+        sum += __uint_as_float(w << 16) + __uint_as_float(w & 0xffff0000u);
+    } else {
+        asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(b), "f"(a));
+        const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w));
+        sum += f.x + f.y;
+    }
+    return w;
+}
+
+template <int D, bool BF16>
+__global__ void __launch_bounds__(kThreads, 2) prefix_mma_kernel(const cq_kv_cache cache, const Call call, const __grid_constant__ CUtensorMap k_map,
+                                                                 const __grid_constant__ CUtensorMap v_map, const uint8_t *__restrict__ q, int64_t q_stride, float c) {
+    extern __shared__ uint8_t raw[];
+    Tiles<D> &sm = *reinterpret_cast<Tiles<D> *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
+    const cq_kv::State st = cq_kv::state_of(cache);
+    const Plan &pl = call.plan;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, page = st.page;
+    constexpr uint32_t kIdescQK = (1u << 4) | (BF16 ? (1u << 7) | (1u << 10) : 0u) | (128u >> 3) << 17 | (128u >> 4) << 24;
+    constexpr uint32_t kIdescPV = (1u << 4) | (BF16 ? (1u << 7) | (1u << 10) : 0u) | (1u << 16) | ((uint32_t)D >> 3) << 17 | (128u >> 4) << 24;
+    volatile int *abort_flag = &sm.abort;
+    if (tid == 0) {
+        cq_mbar_init(&sm.bar.q, 4); cq_mbar_init(&sm.bar.k, 1); cq_mbar_init(&sm.bar.v, 1);
+        cq_mbar_init(&sm.bar.s, 1); cq_mbar_init(&sm.bar.p, 4); cq_mbar_init(&sm.bar.o, 1);
+        sm.abort = 0;
+        cq_fence_mbar_init();
+    }
+    if (warp == 5) {
+        tmem_alloc(&sm.tmem, kCols);
+        tmem_relinquish();
+        tc_fence_before();
+    }
+    cq_pdl_launch_dependents();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = sm.tmem;
+    cq_pdl_wait();
+    const int chunk = pl.header[1];
+    int left = min(pl.header[0] - (int)blockIdx.x * chunk, chunk);
+    int at = left > 0 ? pl.first[blockIdx.x] : 0;
+    bool ok = true;
+    if (warp < 4) {
+        const int per = call.sh.per_kv(), row = warp * 32 + lane;
+        const uint32_t mine = tmem + ((uint32_t)(warp * 32) << 16);
+        unsigned tile = 0;              // parity of the barriers
+        for (; ok && left > 0; ++at) {
+            const Segment seg = pl.segments[at];
+            if (seg.tiles == 0) continue;
+            left -= seg.tiles;
+            // Q: all rows of the segment by the four warps; rows behind them keep what was there, and nobody reads their results
+            const uint8_t *src = q + (int64_t)seg.head * per * D * 2;
+            for (int i = tid; i < seg.rows * (D / 8); i += 128) {
+                const int r = i / (D / 8), x = i % (D / 8), n = seg.row0 + r;
+                const uint4 w = *reinterpret_cast<const uint4 *>(src + ((int64_t)(n / per) * q_stride + (int64_t)(n % per) * D + x * 8) * 2);
+                *reinterpret_cast<uint4 *>(&sm.q[x >> 3][r * 128 + ((x & 7) ^ (r & 7)) * 16]) = w;
+            }
+            fence_proxy_async_smem();
+            arrive_warp(&sm.bar.q, lane);
+            const bool active = warp * 32 < seg.rows;
+            float m = -INFINITY, l = 0.0f;
+            for (int j = 0; j < seg.tiles; ++j, ++tile) {
+                const int n = seg.key1 - seg.key0 - j * kKeyTile;          // keys of this tile, if fewer than 128
+                if (!(ok = wait_warp(&sm.bar.s, tile & 1, abort_flag))) break;
+                tc_fence_after();
+                if (active) {
+                    uint32_t s[32];
+                    float mx = -INFINITY;
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) {
+                        tmem_ld32(mine + kS + 32 * x, s);
+                        tmem_ld_wait();
+                        if (n >= 32 * (x + 1)) {
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) mx = fmaxf(mx, __uint_as_float(s[i]));
+                        } else {
+#pragma unroll
+                            for (int i = 0; i < 32; ++i)
+                                if (32 * x + i < n) mx = fmaxf(mx, __uint_as_float(s[i]));
+                        }
+                    }
+                    mx *= c;
+                    if (j == 0) m = mx;
+                    else {
+                        const bool up = mx > m + 8.0f;          // from -inf as well
+                        if (__any_sync(0xffffffffu, up)) {
+                            const float f = up ? ex2(m - mx) : 1.0f;
+                            if (up) m = mx;
+                            l *= f;
+#pragma unroll
+                            for (int x = 0; x < D / 32; ++x) {
+                                tmem_ld32(mine + kO + 32 * x, s);
+                                tmem_ld_wait();
+#pragma unroll
+                                for (int i = 0; i < 32; ++i) s[i] = __float_as_uint(__uint_as_float(s[i]) * f);
+                                tmem_st32(mine + kO + 32 * x, s);
+                            }
+                        }
+                    }
+                    const float base = m == -INFINITY ? 0.0f : m;
+                    float sum0 = 0.0f, sum1 = 0.0f;
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) {
+                        tmem_ld32(mine + kS + 32 * x, s);
+                        tmem_ld_wait();
+                        uint32_t w[16];
+                        if (n >= 32 * (x + 1)) {
+#pragma unroll
+                            for (int i = 0; i < 16; ++i)
+                                w[i] = pack<BF16>(ex2(__fmaf_rn(__uint_as_float(s[2 * i]), c, -base)), ex2(__fmaf_rn(__uint_as_float(s[2 * i + 1]), c, -base)),
+                                                  i & 1 ? sum1 : sum0);
+                        } else {
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) {
+                                const float a = 32 * x + 2 * i < n ? ex2(__fmaf_rn(__uint_as_float(s[2 * i]), c, -base)) : 0.0f;
+                                const float b = 32 * x + 2 * i + 1 < n ? ex2(__fmaf_rn(__uint_as_float(s[2 * i + 1]), c, -base)) : 0.0f;
+                                w[i] = pack<BF16>(a, b, i & 1 ? sum1 : sum0);
+                            }
+                        }
+                        tmem_st16(mine + kS + 16 * x, w);       // over scores that this thread has read
+                    }
+                    l += sum0 + sum1;
+                    tmem_st_wait();
+                    tc_fence_before();
+                }
+                if (n < kKeyTile) {
+                    if (!(ok = wait_warp(&sm.bar.v, tile & 1, abort_flag))) break;
+                    for (int i = tid; i < (kKeyTile - n) * (D / 8); i += 128) {
+                        const int r = n + i / (D / 8), x = i % (D / 8);
+                        *reinterpret_cast<uint4 *>(&sm.v[x >> 3][r * 128 + (x & 7) * 16]) = make_uint4(0, 0, 0, 0);
+                    }
+                    fence_proxy_async_smem();
+                }
+                arrive_warp(&sm.bar.p, lane);
+            }
+            if (!ok || !(ok = wait_warp(&sm.bar.o, (tile - 1) & 1, abort_flag))) break;
+            tc_fence_after();
+            if (active) {
+                float *to = call.o + (int64_t)(seg.part + row) * D;
+#pragma unroll
+                for (int x = 0; x < D / 32; ++x) {
+                    uint32_t s[32];
+                    tmem_ld32(mine + kO + 32 * x, s);
+                    tmem_ld_wait();
+                    if (row < seg.rows)
+#pragma unroll
+                        for (int i = 0; i < 8; ++i)
+                            *reinterpret_cast<uint4 *>(to + 32 * x + 4 * i) = make_uint4(s[4 * i], s[4 * i + 1], s[4 * i + 2], s[4 * i + 3]);
+                }
+                if (row < seg.rows) call.ml[seg.part + row] = make_float2(m, l);
+                tc_fence_before();
+            }
+        }
+    } else if (warp == 4) {
+        unsigned tile = 0, k_sent = 0, v_sent = 0;
+        for (; ok && left > 0; ++at) {
+            const Segment seg = pl.segments[at];
+            if (seg.tiles == 0) continue;
+            left -= seg.tiles;
+            const int *table = st.tables + (size_t)seg.slot * st.max_pages;
+            for (int j = 0; j < seg.tiles; ++j, ++tile) {
+                const int key = seg.key0 + j * kKeyTile + lane * page;           // a lane takes a page
+                int id = -1;
+                if (lane * page < kKeyTile && key < seg.key1) {
+                    id = table[key / page];
+                    if (id < 0 || id >= st.pages) { id = -1; atomicCAS(st.header, cq_kv::kOk, cq_kv::kBadPage); }
+                }
+                const unsigned bytes = (unsigned)__popc(__ballot_sync(0xffffffffu, id >= 0)) * page * D * 2;
+                const int y = (id * cache.kv_heads + seg.head) * page;
+                if (tile > 0 && !(ok = wait_warp(&sm.bar.s, (tile - 1) & 1, abort_flag))) break;
+                if (lane == 0) cq_mbar_expect_tx(&sm.bar.k, bytes);
+                __syncwarp();
+                if (id >= 0)
+#pragma unroll
+                    for (int h = 0; h < D / 64; ++h) cq_tmap::load_2d(&sm.k[h][lane * page * 128], &k_map, 64 * h, y, &sm.bar.k);
+                ++k_sent;
+                if (tile > 0 && !(ok = wait_warp(&sm.bar.o, (tile - 1) & 1, abort_flag))) break;
+                if (lane == 0) cq_mbar_expect_tx(&sm.bar.v, bytes);
+                __syncwarp();
+                if (id >= 0)
+#pragma unroll
+                    for (int h = 0; h < D / 64; ++h) cq_tmap::load_2d(&sm.v[h][lane * page * 128], &v_map, 64 * h, y, &sm.bar.v);
+                ++v_sent;
+            }
+        }
+        if (!ok) {                      // leaving early: not before what is on its way has come
+            if (k_sent) (void)cq_mbar_wait_bounded(&sm.bar.k, (k_sent - 1) & 1);
+            if (v_sent) (void)cq_mbar_wait_bounded(&sm.bar.v, (v_sent - 1) & 1);
+        }
+    } else {
+        unsigned tile = 0, segment = 0, s_sent = 0, o_sent = 0;
+        const uint32_t qa = uniform(cq_smem_u32(&sm.q[0][0]) >> 4), ka = uniform(cq_smem_u32(&sm.k[0][0]) >> 4), va = uniform(cq_smem_u32(&sm.v[0][0]) >> 4);
+        const uint32_t t0 = uniform(tmem);
+        for (; ok && left > 0; ++at) {
+            const int tiles = (int)uniform((uint32_t)pl.segments[at].tiles);
+            if (tiles == 0) continue;
+            left -= tiles;
+            if (!(ok = wait_warp(&sm.bar.q, segment++ & 1, abort_flag))) break;
+            for (int j = 0; j < tiles; ++j, ++tile) {
+                if (!(ok = wait_warp(&sm.bar.k, tile & 1, abort_flag))) break;
+                if (tile > 0 && !(ok = wait_warp(&sm.bar.o, (tile - 1) & 1, abort_flag))) break;      // the weights before have been read
+                tc_fence_after();
+                if (elect_one()) {
+#pragma unroll
+                    for (int x = 0; x < D / 16; ++x) {
+                        const uint32_t off = (x >> 2) * (kHalfBytes >> 4) + (x & 3) * 2;
+                        mma_ss(t0 + kS, qa + off, ka + off, kIdescQK, x > 0);
+                    }
+                    tc_commit(&sm.bar.s);
+                }
+                __syncwarp();
+                ++s_sent;
+                if (!(ok = wait_warp(&sm.bar.v, tile & 1, abort_flag)) || !(ok = wait_warp(&sm.bar.p, tile & 1, abort_flag))) break;
+                tc_fence_after();
+                if (elect_one()) {
+#pragma unroll
+                    for (int x = 0; x < 8; ++x)
+                        mma_ts(t0 + kO, t0 + kS + 8 * x, (va + x * (2048 >> 4)) | (uint32_t)(kHalfBytes >> 4) << 16, kIdescPV, j > 0 || x > 0);
+                    tc_commit(&sm.bar.o);
+                }
+                __syncwarp();
+                ++o_sent;
+            }
+        }
+        if (!ok) {                      // nor before the products have ended
+            if (s_sent) (void)cq_mbar_wait_bounded(&sm.bar.s, (s_sent - 1) & 1);
+            if (o_sent) (void)cq_mbar_wait_bounded(&sm.bar.o, (o_sent - 1) & 1);
+        }
+    }
+    if (!ok && lane == 0) atomicCAS(st.header, cq_kv::kOk, cq_kv::kTimeout);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (warp == 5) tmem_dealloc(tmem, kCols);
+}
+
+// One layer of a pool as rows of D elements; box: one page x 64 elements, 128-byte swizzle.
+bool pool_map(const void *base, int64_t rows, int d, int page, CUtensorMap &out) {
+    using Encode = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *, const cuuint32_t *,
+                                const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+    static const Encode encode = [] {
+        void *fn = nullptr;
+        cudaDriverEntryPointQueryResult res;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &res) != cudaSuccess || res != cudaDriverEntryPointSuccess) {
+            (void)cudaGetLastError();
+            fn = nullptr;
+        }
+        return (Encode)fn;
+    }();
+    if (!encode) return false;
+    const cuuint64_t dims[2] = {(cuuint64_t)d, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)d * 2};
+    const cuuint32_t box[2] = {64, (cuuint32_t)page}, one[2] = {1, 1};
+    return encode(&out, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, const_cast<void *>(base), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int D, bool BF16>
+void launch(const Call &c, const cq_kv_cache &cache, const CUtensorMap &k, const CUtensorMap &v, const void *q, int64_t q_stride, float scale, cudaStream_t st) {
+    constexpr int smem = (int)sizeof(Tiles<D>) + 1024;
+    cudaFuncSetAttribute(prefix_mma_kernel<D, BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    cq_launch_k(prefix_mma_kernel<D, BF16>, dim3(c.sh.ctas), dim3(kThreads), smem, st, cache, c, k, v, (const uint8_t *)q, q_stride,
+                (float)(scale * 1.4426950408889634));
+}
+
+}  // namespace
+
+bool cq_attn::mma_launch(const Call &c, const cq_kv_cache &cache, int layer, const void *q, int64_t q_stride, float scale, cudaStream_t st) {
+    const int64_t rows = (int64_t)cache.pages * cache.kv_heads * cache.page_size, offset = rows * layer * cache.head_dim * 2;
+    CUtensorMap k, v;
+    if (!pool_map((const uint8_t *)cache.k + offset, rows, cache.head_dim, cache.page_size, k) ||
+        !pool_map((const uint8_t *)cache.v + offset, rows, cache.head_dim, cache.page_size, v)) {
+        cq_set_status(CQ_ERR_CUDA, "prefix_attention: cuTensorMapEncodeTiled is not available or refused the pool");
+        return false;
+    }
+    const bool bf16 = c.sh.elem == CQ_BF16;
+    if (c.sh.head_dim == 128) bf16 ? launch<128, true>(c, cache, k, v, q, q_stride, scale, st) : launch<128, false>(c, cache, k, v, q, q_stride, scale, st);
+    else bf16 ? launch<64, true>(c, cache, k, v, q, q_stride, scale, st) : launch<64, false>(c, cache, k, v, q, q_stride, scale, st);
+    return true;
+}
