@@ -38,7 +38,7 @@ class KvCache(C.Structure):
 
 class PrefixPlan(C.Structure):
     """cq_prefix_plan"""
-    _fields_ = [(n, C.c_int) for n in ("batch", "queries", "heads", "groups", "row_tile", "ctas", "shared_items")] + \
+    _fields_ = [(n, C.c_int) for n in ("batch", "queries", "heads", "groups", "ctas", "shared_items")] + \
         [("n_ints", C.c_int64), ("n_floats", C.c_int64), ("ints", C.c_void_p), ("scratch", C.c_void_p)]
 
 

@@ -3,17 +3,17 @@
 // A row is one query of one head; the rows of a KV head are numbered (sequence * queries + query) * group + head in group, so the
 // rows of consecutive sequences are consecutive.  Two kinds of items cover all (row, key) pairs:
 //   shared : up to `row_tile` rows of one group of sequences x one KV head x the keys of the pages that all of them share;
-//   own    : the rows of one query x one KV head x the keys behind these pages.
-// An item is a number of key tiles; the tiles of all items form one line, which the `ctas` CTAs take in equal parts.  A part of an
-// item that one CTA takes is a segment; it leaves (maximum, sum, unnormalised output) per row, and a second kernel joins a row's
-// segments in the order of their keys:  m = max m_i,  l = sum 2^(m_i - m) l_i,  o = sum 2^(m_i - m) o_i / l.
+//   own    : up to `own_rows` rows of one query x one KV head x the keys behind these pages.
+// An item is a number of units (128 keys of a shared item, `own_step` keys of an own one); the units of all items of a kind form a line, which
+// its workers (CTAs for the shared items; CTAs or warps for the own ones) take in equal parts.  A part of an item that one worker takes
+// is a segment; it leaves (maximum, sum, unnormalised output) per row, and a second kernel joins a row's segments in the order of their keys:
+// m = max m_i,  l = sum 2^(m_i - m) l_i,  o = sum 2^(m_i - m) o_i / l.
 #pragma once
 #include "kv_cache.cuh"
 
 namespace cq_attn {
 
-constexpr int kKeyTile = 128;
-constexpr int kMaxQueries = 1 << 16;        // sequences x queries of a call
+constexpr int kKeyTile = 128;       // keys of a shared unit
 
 struct Segment {            // 32 bytes
     int row0, rows;         // rows of the KV head
@@ -21,33 +21,40 @@ struct Segment {            // 32 bytes
     int slot;               // whose table holds the pages
     int key0, key1;         // positions [key0, key1), key0 a multiple of the page size
     int part;               // first row of the partial results
-    int tiles;
+    int units;
 };
-struct Query { int start, tiles, len, group; };         // its first own tile on the line, tiles per head, context length; group -1: no shared keys
-struct Group { int start, tiles, shared, slot; };       // first tile, tiles per item, shared positions, a slot whose table holds them
+struct Query {              // 32 bytes
+    int len, group;         // context length; group with shared keys, or -1
+    int start, units;       // its first own unit on the line, units per item
+    int query0, item0, row_tiles, pad;          // of its group
+};
+struct Group { int start, units, shared, slot; };       // first unit, units per item, shared positions, a slot whose table holds them
 struct GroupShape { int query0, item0, row_tiles; };    // from the sizes of the groups alone
 
 struct Shape {
     int batch, queries, heads, kv_heads, groups, head_dim, elem;
-    int row_tile, ctas;
+    int row_tile, ctas, own_rows, own_step, own_workers;
     __host__ __device__ int per_kv() const { return heads / kv_heads; }
     __host__ __device__ int n_queries() const { return batch * queries; }
+    __host__ __device__ int own_tiles() const { return (per_kv() + own_rows - 1) / own_rows; }
+    __host__ __device__ int own_slot() const { return per_kv() < own_rows ? per_kv() : own_rows; }      // rows of a partial result
+    __host__ __device__ int own_items() const { return n_queries() * kv_heads * own_tiles(); }          // query, then head, then row tile
 };
 
-// The plan's ints.  header: [0] tiles in all, [1] tiles per CTA
+// One kind of items: its segments (that of item i and worker w at i + w), the first segment of each worker, the workers of each item.
+struct Line {
+    int *header;            // units in all, units per worker
+    int *first;             // [workers]
+    int2 *item;             // first and last worker (first > last: no keys)
+    Segment *segments;      // [items + workers]
+};
+// The plan's ints.
 struct Plan {
-    int *header;
     GroupShape *shapes;     // [groups + 1], written by the host's part of the plan
     Group *groups;
     Query *query;
-    int2 *item;             // first and last CTA of an item (first > last: no keys)
-    int *first;             // first segment of a CTA
-    Segment *segments;      // [items + ctas], segment of item i and CTA c at i + c
+    Line shared, own;
 };
-
-}  // namespace cq_attn
-
-namespace cq_attn {
 
 // Everything a call has in hand besides its tensors.
 struct Call {
@@ -55,37 +62,45 @@ struct Call {
     Plan plan;
     float *o;               // partial outputs [rows][head_dim]
     float2 *ml;             // maximum (times scale and log2 e) and sum [rows]
-    int items_shared;
+    int shared_items;
 };
 
 inline int64_t align8(int64_t n) { return (n + 7) / 8 * 8; }
-inline int64_t items_own(const Shape &s) { return (int64_t)s.n_queries() * s.kv_heads; }
-inline int64_t part_rows(const Shape &s, int64_t shared) { return (shared + s.ctas) * s.row_tile + (items_own(s) + s.ctas) * s.per_kv(); }
-inline int64_t plan_ints(const Shape &s, int64_t shared) {
-    const int64_t items = shared + items_own(s);
-    return 16 + align8(3LL * (s.groups + 1)) + 4LL * s.groups + 4LL * s.n_queries() + 8 + align8(2 * items) + align8(s.ctas) + 8 * (items + s.ctas);
+inline int64_t part_rows(const Shape &s, int64_t shared) { return (shared + s.ctas) * s.row_tile + ((int64_t)s.own_items() + s.own_workers) * s.own_slot(); }
+inline Line line_of(int *&p, int *header, int64_t items, int64_t workers) {
+    Line l;
+    l.header = header;
+    l.first = p; p += align8(workers);
+    l.item = (int2 *)p; p += align8(2 * items);
+    l.segments = (Segment *)p; p += 8 * (items + workers);
+    return l;
 }
-inline Plan plan_of(int *p, const Shape &s, int64_t shared) {
-    const int64_t items = shared + items_own(s);
+inline Plan plan_of(int *base, const Shape &s, int64_t shared, int64_t *ints = nullptr) {
     Plan r;
-    r.header = p; p += 16;
+    int *p = base + 16;
     r.shapes = (GroupShape *)p; p += align8(3LL * (s.groups + 1));
-    r.groups = (Group *)p; p += 4LL * s.groups;
-    r.query = (Query *)p; p += 4LL * s.n_queries();
-    p += (8 - ((4LL * s.groups + 4LL * s.n_queries()) & 7)) & 7;
-    r.item = (int2 *)p; p += align8(2 * items);
-    r.first = p; p += align8(s.ctas);
-    r.segments = (Segment *)p;
+    r.groups = (Group *)p; p += align8(4LL * s.groups);
+    r.query = (Query *)p; p += 8LL * s.n_queries();
+    r.shared = line_of(p, base, shared, s.ctas);
+    r.own = line_of(p, base + 2, s.own_items(), s.own_workers);
+    if (ints) *ints = p - base;
     return r;
 }
-
-// First row of the partial results of segment (item, CTA).
-__host__ __device__ inline int64_t part_of(const Shape &s, int shared, int item, int cta) {
-    return item < shared ? (int64_t)(item + cta) * s.row_tile : (int64_t)(shared + s.ctas) * s.row_tile + (int64_t)(item - shared + cta) * s.per_kv();
+inline int64_t plan_ints(const Shape &s, int64_t shared) {
+    int64_t n;
+    (void)plan_of((int *)nullptr, s, shared, &n);
+    return n;
 }
 
-// One CTA's kernel for all segments, by element type (prefix_attn_simt.cu, prefix_attn_mma.cu).
+// First row of the partial results of segment i + w of a kind.
+__host__ __device__ inline int64_t part_shared(const Shape &s, int at) { return (int64_t)at * s.row_tile; }
+__host__ __device__ inline int64_t part_own(const Shape &s, int shared_items, int at) {
+    return (int64_t)(shared_items + s.ctas) * s.row_tile + (int64_t)at * s.own_slot();
+}
+
+// The kernels that make the segments' results (prefix_attn_simt.cu: f32; prefix_attn_mma.cu: f16 and bf16).
 void simt_launch(const Call &c, const cq_kv_cache &cache, int layer, const void *q, int64_t q_stride, float scale, cudaStream_t st);
 bool mma_launch(const Call &c, const cq_kv_cache &cache, int layer, const void *q, int64_t q_stride, float scale, cudaStream_t st);
+constexpr int kMmaWarps = 6;            // of a CTA of the latter: each is a worker of the own line
 
 }  // namespace cq_attn

@@ -80,14 +80,15 @@ __global__ void __launch_bounds__(kThreads) prefix_simt_kernel(const cq_kv_cache
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, per = call.sh.per_kv();
     cq_pdl_launch_dependents();
     cq_pdl_wait();
-    const int chunk = pl.header[1];
-    int left = min(pl.header[0] - (int)blockIdx.x * chunk, chunk);
-    if (left <= 0) return;
     const T *k_pool = reinterpret_cast<const T *>(cache.k), *v_pool = reinterpret_cast<const T *>(cache.v);
-    for (int at = pl.first[blockIdx.x]; left > 0; ++at) {
-        const Segment seg = pl.segments[at];
-        if (seg.tiles == 0) continue;
-        left -= seg.tiles;
+    for (int kind = 0; kind < 2; ++kind) {
+    const Line &line = kind ? pl.own : pl.shared;
+    const int chunk = line.header[1];
+    int left = min(line.header[0] - (int)blockIdx.x * chunk, chunk);
+    for (int at = left > 0 ? line.first[blockIdx.x] : 0; left > 0; ++at) {
+        const Segment seg = line.segments[at];
+        if (seg.units == 0) continue;
+        left -= seg.units;
         const int *table = s.tables + (size_t)seg.slot * s.max_pages;
         __syncthreads();
         for (int i = tid; i < kRows * (D / 4); i += kThreads) {
@@ -172,6 +173,7 @@ __global__ void __launch_bounds__(kThreads) prefix_simt_kernel(const cq_kv_cache
 #pragma unroll
                     for (int i = 0; i < V; ++i) call.o[(int64_t)(seg.part + r0 + r) * D + V * lane + i] = o[r][i] + mine[r * D + i];
         if (tid < seg.rows) call.ml[seg.part + tid] = make_float2(sm.m[tid], sm.l[tid]);
+    }
     }
 }
 

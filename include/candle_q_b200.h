@@ -455,7 +455,7 @@ int cq_kv_take_fault(const cq_kv_cache *cache, void *stream);
  * out[b, t] = softmax(scale q K^T) V over the first len_b - queries + 1 + t positions of slot b (a context without positions gives
  * zeros), query heads in groups of heads / kv_heads per KV head.  The batch is cut into `groups` runs of neighbouring sequences; the pages that all
  * sequences of a run have in common at their start are found on the device, by comparing the tables.
- *   cq_prefix_plan_shape  : fills row_tile, ctas, shared_items, n_ints, n_floats of a plan whose batch, queries, heads and groups are set, and `shapes`
+ *   cq_prefix_plan_shape  : fills ctas, shared_items, n_ints, n_floats of a plan whose batch, queries, heads and groups are set, and `shapes`
  *                           (host, 3 * (groups + 1) ints, or null).  group_sizes: host, sequences per group, null for one group or groups of one.  Host
  *                           only; 0 or, with the status set, 1.  The caller then gives the plan `ints` (device, n_ints) and `scratch` (device, n_floats),
  *                           32-byte aligned, and copies `shapes` to ints + 16.
@@ -467,7 +467,7 @@ int cq_kv_take_fault(const cq_kv_cache *cache, void *stream);
  * cache (cq_kv_take_fault) and reads nothing. */
 typedef struct cq_prefix_plan {
     int batch, queries, heads, groups;
-    int row_tile, ctas, shared_items;
+    int ctas, shared_items;
     int64_t n_ints, n_floats;
     int *ints;
     float *scratch;
