@@ -9,27 +9,29 @@ namespace {
 using namespace cq_attn;
 using cq_kv::State;
 
-constexpr int kThreads = 1024;
+constexpr int kThreads = 1024, kPlanCtas = 8;
+constexpr int kOwnLeast = 1;            // units of an own segment, at least
 
-__device__ __forceinline__ int scan_before(int v, int *sums, int &total) {
+// Sum of `v` over the threads before this one, two counts in one 64-bit word; `total` over all.
+__device__ __forceinline__ uint64_t scan_before(uint64_t v, uint64_t *sums, uint64_t &total) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    int x = v;
+    uint64_t x = v;
 #pragma unroll
     for (int m = 1; m < 32; m <<= 1) {
-        const int y = __shfl_up_sync(0xffffffffu, x, m);
+        const uint64_t y = __shfl_up_sync(0xffffffffu, x, m);
         if (lane >= m) x += y;
     }
     __syncthreads();
     if (lane == 31) sums[warp] = x;
     __syncthreads();
-    int w = sums[lane];
+    uint64_t w = sums[lane];
 #pragma unroll
     for (int m = 1; m < 32; m <<= 1) {
-        const int y = __shfl_up_sync(0xffffffffu, w, m);
+        const uint64_t y = __shfl_up_sync(0xffffffffu, w, m);
         if (lane >= m) w += y;
     }
     total = __shfl_sync(0xffffffffu, w, 31);
-    const int before = __shfl_sync(0xffffffffu, w, (warp + 31) & 31);
+    const uint64_t before = __shfl_sync(0xffffffffu, w, (warp + 31) & 31);
     return x - v + (warp ? before : 0);
 }
 // Index of the last entry of an ascending column that is not above `v`.
@@ -43,20 +45,24 @@ template <typename F> __device__ __forceinline__ int last_not_above(int n, int v
     return lo;
 }
 
-// One CTA.  The pages that a group shares are found by comparing the tables, so a plan cannot be wrong about them: the leading
+// One cluster.  The pages that a group shares are found by comparing the tables, so a plan cannot be wrong about them: the leading
 // entries that agree in all its sequences, as far as the shortest context among its queries fills pages.
-// Bound by latency: slots, lengths and tables are three reads that depend on one another, the rest works in shared memory.
+// Bound by latency - slots, lengths and tables are three reads that depend on one another, and a kernel of one CTA meets its instructions for
+// the first time as well - so the comparison and the workers' records are divided over kPlanCtas CTAs, and all else every CTA does for itself.
 __global__ void __launch_bounds__(kThreads) prefix_plan_kernel(const cq_kv_cache cache, const Call call, const int *__restrict__ slots) {
     extern __shared__ int dyn[];
-    __shared__ int sums[32], most;
+    __shared__ uint64_t sums[32];
+    __shared__ int most;
     const State s = cq_kv::state_of(cache);
     const Shape &sh = call.sh;
     const Plan &pl = call.plan;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int t = sh.queries, hkv = sh.kv_heads, cap = s.max_pages * s.page, nq = sh.n_queries(), per = sh.per_kv();
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, rank = (int)blockIdx.x, shift = 31 - __clz(s.page);
+    const int t = sh.queries, hkv = sh.kv_heads, cap = s.max_pages * s.page, nq = sh.n_queries();
     int *slot_of = dyn, *len_of = slot_of + sh.batch, *group_of = len_of + sh.batch;         // by sequence
     int *first_of = group_of + sh.batch, *count_of = first_of + sh.groups, *least_of = count_of + sh.groups;      // by group: of its sequences that
                                                                     // have a context for each query: the first, how many, pages that agree
+    int *shared_of = least_of + sh.groups, *group_start = shared_of + sh.groups;            // shared positions, first unit
+    int *start_of = group_start + sh.groups, *units_of = start_of + nq;                     // by query
     for (int g = tid; g < sh.groups; g += kThreads) { first_of[g] = INT32_MAX; count_of[g] = 0; least_of[g] = INT32_MAX; }
     if (tid == 0) most = 0;
     cq_pdl_launch_dependents();
@@ -65,7 +71,8 @@ __global__ void __launch_bounds__(kThreads) prefix_plan_kernel(const cq_kv_cache
     for (int b = tid; b < sh.batch; b += kThreads) {
         const int slot = slots[b];
         const bool there = slot >= 0 && slot < s.max_seqs;
-        const int len = there ? min(max(s.lens[slot], 0), cap) : -1, g = last_not_above(sh.groups, b * t, [&](int x) { return pl.shapes[x].query0; });
+        const int len = there ? min(max(s.lens[slot], 0), cap) : -1;
+        const int g = sh.groups == 1 ? 0 : last_not_above(sh.groups, b * t, [&](int x) { return pl.shapes[x].query0; });
         if (!there) atomicCAS(s.header, cq_kv::kOk, cq_kv::kBadSlot);
         slot_of[b] = slot;
         len_of[b] = len;
@@ -73,17 +80,18 @@ __global__ void __launch_bounds__(kThreads) prefix_plan_kernel(const cq_kv_cache
         if (len >= t) {
             atomicMin(&first_of[g], b);
             atomicAdd(&count_of[g], 1);
-            atomicMin(&least_of[g], (len - t + 1) / s.page);
-            atomicMax(&most, (len - t + 1) / s.page);
+            atomicMin(&least_of[g], (len - t + 1) >> shift);
+            atomicMax(&most, (len - t + 1) >> shift);
         }
     }
     __syncthreads();
     // a warp compares 128 entries of a sequence with those of its group's first one
-    const int blocks = (most + 127) / 128;
-    for (int u = warp; u < sh.batch * blocks; u += kThreads / 32) {
+    const int blocks = (most + 127) >> 7;
+#pragma unroll 1
+    for (int u = rank * (kThreads / 32) + warp; u < sh.batch * blocks; u += kPlanCtas * (kThreads / 32)) {
         const int b = u / blocks, j0 = u % blocks * 128 + lane, g = group_of[b];
-        if (len_of[b] < t || count_of[g] < 2) continue;         // the whole warp
-        const int n = (len_of[b] - t + 1) / s.page;
+        if (len_of[b] < t || count_of[g] < 2 || b == first_of[g]) continue;         // the whole warp
+        const int n = (len_of[b] - t + 1) >> shift;
         const int *mine = s.tables + (size_t)slot_of[b] * s.max_pages, *first = s.tables + (size_t)slot_of[first_of[g]] * s.max_pages;
         int p[4], f[4], bad = INT32_MAX;
 #pragma unroll
@@ -98,94 +106,100 @@ __global__ void __launch_bounds__(kThreads) prefix_plan_kernel(const cq_kv_cache
         bad = __reduce_min_sync(0xffffffffu, bad);
         if (lane == 0 && bad != INT32_MAX) atomicMin(&least_of[g], bad);
     }
-    __syncthreads();
-    // the shared line
-    int line = 0;
-    for (int g0 = 0; g0 < sh.groups; g0 += kThreads) {
-        const int g = g0 + tid;
-        Group gr{0, 0, 0, -1};
-        int n = 0, all;
-        if (g < sh.groups) {
-            if (count_of[g] >= 2 && least_of[g] > 0) {
-                gr.shared = least_of[g] * s.page;
-                gr.slot = slot_of[first_of[g]];
-                gr.units = (gr.shared + kKeyTile - 1) / kKeyTile;
-            }
-            n = gr.units * hkv * pl.shapes[g].row_tiles;
+    __syncwarp();
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    for (int g = tid; g < sh.groups; g += kThreads) {
+        int least = INT32_MAX;
+#pragma unroll
+        for (int r = 0; r < kPlanCtas; ++r) {
+            uint32_t at;
+            int v;
+            asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(cq_smem_u32(&least_of[g])), "r"(r));
+            asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
+            least = min(least, v);
         }
-        gr.start = line + scan_before(n, sums, all);
-        if (g < sh.groups) {
-            pl.groups[g] = gr;
-            least_of[g] = gr.shared;
-        }
-        line += all;
+        shared_of[g] = count_of[g] >= 2 ? least << shift : 0;
     }
+    __syncwarp();
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");         // the others' shared memory has been read
     __syncthreads();
-    const int chunk = max((line + sh.ctas - 1) / sh.ctas, 1), shared_line = line;
-    // the own line
-    const int tiles = sh.own_tiles();
-    line = 0;
-    for (int i0 = 0; i0 < nq; i0 += kThreads) {
+    // both lines at once: the units of group i, and of query i
+    uint64_t before = 0;
+    for (int i0 = 0; i0 < max(nq, sh.groups); i0 += kThreads) {
         const int i = i0 + tid;
-        Query q{};
-        int all;
+        int n_shared = 0, units = 0;
+        if (i < sh.groups) n_shared = ((shared_of[i] + kKeyTile - 1) / kKeyTile) * hkv * pl.shapes[i].row_tiles;
         if (i < nq) {
-            const int b = i / t, g = group_of[b], len = len_of[b], shared = len >= t ? least_of[g] : 0;
-            const GroupShape gs = pl.shapes[g];
-            q.len = len - t + 1 + i % t;
-            q.group = shared ? g : -1;
-            q.units = q.len > shared ? (q.len - shared + sh.own_step - 1) / sh.own_step : 0;
-            q.query0 = gs.query0; q.item0 = gs.item0; q.row_tiles = gs.row_tiles;
+            const int b = i / t, len = len_of[b], shared = len >= t ? shared_of[group_of[b]] : 0, n = len - t + 1 + i % t;
+            units = n > shared ? (n - shared + sh.own_step - 1) / sh.own_step : 0;
         }
-        q.start = line + scan_before(q.units * hkv * tiles, sums, all);
-        if (i < nq) pl.query[i] = q;
-        line += all;
-    }
-    const int own_chunk = max((line + sh.own_workers - 1) / sh.own_workers, 1);
-    if (tid == 0) {
-        pl.shared.header[0] = shared_line; pl.shared.header[1] = chunk;
-        pl.own.header[0] = line; pl.own.header[1] = own_chunk;
+        uint64_t all;
+        const uint64_t at = before + scan_before((uint64_t)n_shared << 32 | (unsigned)(units * hkv * sh.own_tiles()), sums, all);
+        if (i < sh.groups) group_start[i] = (int)(at >> 32);
+        if (i < nq) { start_of[i] = (int)(uint32_t)at; units_of[i] = units; }
+        before += all;
     }
     __syncthreads();
-    // segments of an item that starts at `start` of its line
-    auto write = [&](const Line &l, int workers, int chunk, int item, int start, int units, int step, Segment seg, int key0, int key1, int64_t part0, int part_step,
-                     int w_first, int w_step) {
-        const int w0 = start / chunk, w1 = units ? (start + units - 1) / chunk : w0;
-        if (w_first == 0) l.item[item] = units ? make_int2(w0, w1) : make_int2(1, 0);
-        for (int w = w0 + w_first; w <= w1; w += w_step) {
-            if (w >= workers) break;                    // an empty item at the very end of the line
-            const int a = max(start, w * chunk), b = min(start + units, (w + 1) * chunk);
-            seg.units = b - a;
-            seg.key0 = key0 + (a - start) * step;
-            seg.key1 = min(key1, key0 + (b - start) * step);
-            seg.part = (int)(part0 + (int64_t)(item + w) * part_step);
-            l.segments[item + w] = seg;
-            if (units && w * chunk >= start) l.first[w] = item + w;
-        }
-    };
-    for (int i = warp; i < call.shared_items; i += kThreads / 32) {
-        const int g = last_not_above(sh.groups, i, [&](int x) { return pl.shapes[x].item0; });
+    const int shared_line = (int)(before >> 32), own_line = (int)(uint32_t)before;
+    const int chunk = max((shared_line + sh.ctas - 1) / sh.ctas, 1), own_chunk = max((own_line + sh.own_workers - 1) / sh.own_workers, kOwnLeast);
+    if (rank == 0 && tid == 0) { pl.header[0] = shared_line; pl.header[1] = chunk; pl.header[2] = own_line; pl.header[3] = own_chunk; }
+    auto group_at = [&](int g) {
         const GroupShape gs = pl.shapes[g];
-        const Group gr = pl.groups[g];
-        const int local = i - gs.item0, row0 = gs.query0 * per + local % gs.row_tiles * sh.row_tile;
-        Segment seg{};
-        seg.row0 = row0;
-        seg.rows = min(sh.row_tile, pl.shapes[g + 1].query0 * per - row0);
-        seg.head = local / gs.row_tiles;
-        seg.slot = gr.slot;
-        write(pl.shared, sh.ctas, chunk, i, gr.start + local * gr.units, gr.units, kKeyTile, seg, 0, gr.shared, part_shared(sh, 0), sh.row_tile, lane, 32);
+        return Group{(shared_of[g] + kKeyTile - 1) / kKeyTile, shared_of[g], count_of[g] ? slot_of[first_of[g]] : -1, group_start[g], gs.query0, gs.rows, gs.item0, gs.row_tiles};
+    };
+    const int id = rank * kThreads + tid, all = kPlanCtas * kThreads;
+#pragma unroll 1
+    for (int i = id; i < sh.groups; i += all) pl.groups[i] = group_at(i);
+#pragma unroll 1
+    for (int i = id; i < nq; i += all) {
+        const int b = i / t, len = len_of[b];
+        Query q{};
+        q.len = len - t + 1 + i % t;
+        q.slot = slot_of[b];
+        q.units = units_of[i];
+        q.start = start_of[i];
+        if (len >= t && shared_of[group_of[b]]) {
+            const Group g = group_at(group_of[b]);
+            q.shared = g.shared;
+            q.group_start = g.start; q.group_units = g.units; q.query0 = g.query0; q.item0 = g.item0; q.row_tiles = g.row_tiles;
+        }
+        pl.query[i] = q;
     }
-    for (int i = tid; i < sh.own_items(); i += kThreads) {
-        const int tile = i % tiles, h = i / tiles % hkv, n = i / tiles / hkv;
-        const Query q = pl.query[n];
-        Segment seg{};
-        seg.row0 = n * per + tile * sh.own_rows;
-        seg.rows = min(sh.own_rows, per - tile * sh.own_rows);
-        seg.head = h;
-        seg.slot = slot_of[n / t];
-        write(pl.own, sh.own_workers, own_chunk, i, q.start + (h * tiles + tile) * q.units, q.units, sh.own_step, seg, q.group >= 0 ? least_of[q.group] : 0, q.len,
-              part_own(sh, call.shared_items, 0), sh.own_slot(), 0, 1);
+#pragma unroll 1
+    for (int w = id; w < sh.ctas + sh.own_workers; w += all) {
+        const bool own = w >= sh.ctas;
+        Start st{};
+        if (!own) {
+            const int u = w * chunk;
+            st.left = min(shared_line - u, chunk);
+            if (st.left > 0) {
+                // the last group that begins here or before; those without units begin where the next one does
+                st.index = last_not_above(sh.groups, u, [&](int x) { return group_start[x]; });
+                const Group g = group_at(st.index);
+                st.local = (u - g.start) / g.units;
+                st.unit = (u - g.start) % g.units;
+                const int c[8] = {g.units, g.shared, g.slot, g.start, g.query0, g.rows, g.item0, g.row_tiles};
+#pragma unroll
+                for (int i = 0; i < 8; ++i) st.copy[i] = c[i];
+            }
+        } else {
+            const int u = (w - sh.ctas) * own_chunk;
+            st.left = min(own_line - u, own_chunk);
+            if (st.left > 0) {
+                st.index = last_not_above(nq, u, [&](int x) { return start_of[x]; });
+                const int b = st.index / t, len = len_of[b], units = units_of[st.index];
+                st.local = (u - start_of[st.index]) / units;
+                st.unit = (u - start_of[st.index]) % units;
+                st.copy[0] = len - t + 1 + st.index % t;
+                st.copy[1] = slot_of[b];
+                st.copy[2] = len >= t ? shared_of[group_of[b]] : 0;
+                st.copy[3] = units;
+            }
+        }
+        (own ? pl.own - sh.ctas : pl.shared)[w] = st;
     }
+    __syncwarp();
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
 // One warp per row: lane x weighs segment x - those of the row's shared item, then those of its own one, in the order of their keys - and the
@@ -200,20 +214,23 @@ template <typename T, int D> __global__ void __launch_bounds__(256) prefix_join_
     if (row >= (int64_t)sh.n_queries() * sh.heads) return;
     const int n = (int)(row / sh.heads), hq = (int)(row % sh.heads), h = hq / per, in = hq % per;
     const Query q = pl.query[n];
+    const int chunk = pl.header[1], own_chunk = pl.header[3];
     constexpr int V = D / 32;
     float acc[V] = {}, m = -INFINITY, l = 0.0f;
     if (q.len > 0) {
+        // segments of an item: its units [start, start + units) of the line, cut at multiples of the chunk
         const int own_item = (n * sh.kv_heads + h) * sh.own_tiles() + in / sh.own_rows;
-        const int2 own = pl.own.item[own_item];
-        int2 shared = make_int2(1, 0);
+        const int own_start = q.start + (h * sh.own_tiles() + in / sh.own_rows) * q.units, own_w = own_start / own_chunk;
+        const int n_own = q.units ? (own_start + q.units - 1) / own_chunk - own_w + 1 : 0;
+        int n_shared = 0;
         int64_t shared0 = 0;
-        if (q.group >= 0) {
-            const int r = (n - q.query0) * per + in, item = q.item0 + h * q.row_tiles + r / sh.row_tile;
-            shared = pl.shared.item[item];
-            shared0 = part_shared(sh, item + shared.x) + r % sh.row_tile;
+        if (q.shared) {
+            const int r = (n - q.query0) * per + in, local = h * q.row_tiles + r / sh.row_tile, start = q.group_start + local * q.group_units, w = start / chunk;
+            n_shared = (start + q.group_units - 1) / chunk - w + 1;
+            shared0 = part_shared(sh, q.item0 + local + w) + r % sh.row_tile;
         }
-        const int n_shared = shared.y - shared.x + 1, n_all = n_shared + own.y - own.x + 1;
-        const int64_t own0 = part_own(sh, call.shared_items, own_item + own.x) + in % sh.own_rows;
+        const int n_all = n_shared + n_own;
+        const int64_t own0 = part_own(sh, call.shared_items, own_item + own_w) + in % sh.own_rows;
         for (int x0 = 0; x0 < n_all; x0 += 32) {
             const int x = x0 + lane, count = min(32, n_all - x0);
             const int part = (int)(x < n_shared ? shared0 + (int64_t)x * sh.row_tile : own0 + (int64_t)(x - n_shared) * sh.own_slot());
@@ -279,7 +296,8 @@ bool shape_ok(const cq_kv_cache *cache, const cq_prefix_plan *p, const char *who
         cq_set_status(status, msg);
         return false;
     }
-    s = Shape{p->batch, p->queries, p->heads, cache->kv_heads, p->groups, cache->head_dim, cache->elem, 0, p->ctas, 0, 0, 0};
+    s = Shape{p->batch, p->queries, p->heads, cache->kv_heads, p->groups, cache->head_dim, cache->elem, 0, p->ctas, 0, 0, 0, 0};
+    if (s.per_kv() > 1) s.rcp = (unsigned)(((1ull << 32) + s.per_kv() - 1) / s.per_kv());
     if (cache->elem == CQ_F32) { s.row_tile = s.own_rows = 32; s.own_step = 64; s.own_workers = s.ctas; }
     else { s.row_tile = 128; s.own_rows = 16; s.own_step = 16; s.own_workers = s.ctas * kMmaWarps; }
     return true;
@@ -288,15 +306,15 @@ Call call_of(const cq_prefix_plan *p, const Shape &s) {
     Call c;
     c.sh = s;
     c.shared_items = p->shared_items;
-    c.plan = plan_of(p->ints, s, p->shared_items);
+    c.plan = plan_of(p->ints, s);
     c.o = p->scratch;
     c.ml = reinterpret_cast<float2 *>(p->scratch + part_rows(s, p->shared_items) * s.head_dim);
     return c;
 }
 bool plan_ready(const cq_prefix_plan *p, const Shape &s, const char *who) {
     char msg[160];
-    if (!p->ints || !p->scratch || (((uintptr_t)p->ints | (uintptr_t)p->scratch) & 31) || p->ctas <= 0 || p->shared_items <= 0 ||
-        p->n_ints != plan_ints(s, p->shared_items) || p->n_floats != part_rows(s, p->shared_items) * (s.head_dim + 2)) {
+    if (!p->ints || !p->scratch || (((uintptr_t)p->ints | (uintptr_t)p->scratch) & 63) || p->ctas <= 0 || p->shared_items <= 0 ||
+        p->n_ints != plan_ints(s) || p->n_floats != part_rows(s, p->shared_items) * (s.head_dim + 2)) {
         std::snprintf(msg, sizeof msg, "%s: the plan is not one that cq_prefix_plan_shape has filled for this cache, or its memory is missing", who);
         cq_set_status(CQ_ERR_BAD_ARG, msg);
         return false;
@@ -316,14 +334,16 @@ extern "C" int cq_prefix_plan_shape(const cq_kv_cache *cache, cq_prefix_plan *pl
         const int n = group_sizes ? group_sizes[g] : plan->groups == 1 ? plan->batch : 1;
         if (n <= 0) { cq_set_status(CQ_ERR_BAD_ARG, "prefix_plan_shape: a group without sequences"); return 1; }
         const int64_t tiles = ((int64_t)n * s.queries * s.per_kv() + s.row_tile - 1) / s.row_tile;
-        if (shapes) { shapes[3 * g] = (int)(seqs * s.queries); shapes[3 * g + 1] = (int)items; shapes[3 * g + 2] = (int)tiles; }
+        if (shapes) {
+            int *to = shapes + 4 * g;
+            to[0] = (int)(seqs * s.queries); to[1] = n * s.queries * s.per_kv(); to[2] = (int)items; to[3] = (int)tiles;
+        }
         items += tiles * s.kv_heads;
         seqs += n;
     }
     if (seqs != plan->batch) { cq_set_status(CQ_ERR_BAD_ARG, "prefix_plan_shape: the groups' sizes do not add up to the batch"); return 1; }
-    if (shapes) { shapes[3 * plan->groups] = (int)(seqs * s.queries); shapes[3 * plan->groups + 1] = (int)items; shapes[3 * plan->groups + 2] = 0; }
     plan->shared_items = (int)items;
-    plan->n_ints = plan_ints(s, items);
+    plan->n_ints = plan_ints(s);
     plan->n_floats = part_rows(s, items) * (s.head_dim + 2);
     return 0;
 }
@@ -332,9 +352,9 @@ extern "C" void cq_prefix_plan_update(const cq_kv_cache *cache, const cq_prefix_
     Shape s;
     if (!shape_ok(cache, plan, "prefix_plan_update", s) || !plan_ready(plan, s, "prefix_plan_update")) return;
     if (!slots) { cq_set_status(CQ_ERR_BAD_ARG, "prefix_plan_update: null slots"); return; }
-    const size_t smem = 12 * ((size_t)s.batch + s.groups);
-    if (smem > 48 * 1024) cudaFuncSetAttribute(prefix_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    cq_launch_k(prefix_plan_kernel, dim3(1), dim3(kThreads), smem, (cudaStream_t)stream, *cache, call_of(plan, s), slots);
+    const size_t smem = 4 * (3 * (size_t)s.batch + 5 * (size_t)s.groups + 2 * (size_t)s.n_queries());
+    if (smem > 47 * 1024) cudaFuncSetAttribute(prefix_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    cq_launch_cluster_k(prefix_plan_kernel, dim3(kPlanCtas), dim3(kThreads), smem, (cudaStream_t)stream, kPlanCtas, *cache, call_of(plan, s), slots);
     cq_check_launch("prefix_plan_update");
 }
 

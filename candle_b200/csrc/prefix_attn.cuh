@@ -4,7 +4,7 @@
 // rows of consecutive sequences are consecutive.  Two kinds of items cover all (row, key) pairs:
 //   shared : up to `row_tile` rows of one group of sequences x one KV head x the keys of the pages that all of them share;
 //   own    : up to `own_rows` rows of one query x one KV head x the keys behind these pages.
-// An item is a number of units (128 keys of a shared item, `own_step` keys of an own one); the units of all items of a kind form a line, which
+// An item is a number of units (64 keys of a shared item, `own_step` keys of an own one); the units of all items of a kind form a line, which
 // its workers (CTAs for the shared items; CTAs or warps for the own ones) take in equal parts.  A part of an item that one worker takes
 // is a segment; it leaves (maximum, sum, unnormalised output) per row, and a second kernel joins a row's segments in the order of their keys:
 // m = max m_i,  l = sum 2^(m_i - m) l_i,  o = sum 2^(m_i - m) o_i / l.
@@ -13,9 +13,9 @@
 
 namespace cq_attn {
 
-constexpr int kKeyTile = 128;       // keys of a shared unit
+constexpr int kKeyTile = 64;        // keys of a shared unit
 
-struct Segment {            // 32 bytes
+struct Segment {
     int row0, rows;         // rows of the KV head
     int head;               // KV head
     int slot;               // whose table holds the pages
@@ -23,17 +23,23 @@ struct Segment {            // 32 bytes
     int part;               // first row of the partial results
     int units;
 };
-struct Query {              // 32 bytes
-    int len, group;         // context length; group with shared keys, or -1
-    int start, units;       // its first own unit on the line, units per item
-    int query0, item0, row_tiles, pad;          // of its group
+struct Group {              // 32 bytes
+    int units, shared, slot, start;             // units per item, shared positions, a slot whose table holds them, first unit on the line
+    int query0, rows, item0, row_tiles;         // from the sizes of the groups alone
 };
-struct Group { int start, units, shared, slot; };       // first unit, units per item, shared positions, a slot whose table holds them
-struct GroupShape { int query0, item0, row_tiles; };    // from the sizes of the groups alone
+struct Query {              // 64 bytes
+    int len, slot, shared, units;               // context length, slot, positions that its group shares (its own keys begin there), own units per item
+    int start, group_start, group_units, query0;
+    int item0, row_tiles, pad[6];
+};
+// Where a worker begins: the group (query), the item in it (head, then row tile), the unit in that, and how many units the worker has.
+struct Start { int index, local, unit, left, copy[8]; int pad[4]; };        // 64 bytes; copy: the Group, or the first half of the Query
+struct GroupShape { int query0, rows, item0, row_tiles; };
 
 struct Shape {
     int batch, queries, heads, kv_heads, groups, head_dim, elem;
     int row_tile, ctas, own_rows, own_step, own_workers;
+    unsigned rcp;           // ceil(2^32 / query heads per KV head); 0 for one
     __host__ __device__ int per_kv() const { return heads / kv_heads; }
     __host__ __device__ int n_queries() const { return batch * queries; }
     __host__ __device__ int own_tiles() const { return (per_kv() + own_rows - 1) / own_rows; }
@@ -41,19 +47,13 @@ struct Shape {
     __host__ __device__ int own_items() const { return n_queries() * kv_heads * own_tiles(); }          // query, then head, then row tile
 };
 
-// One kind of items: its segments (that of item i and worker w at i + w), the first segment of each worker, the workers of each item.
-struct Line {
-    int *header;            // units in all, units per worker
-    int *first;             // [workers]
-    int2 *item;             // first and last worker (first > last: no keys)
-    Segment *segments;      // [items + workers]
-};
 // The plan's ints.
 struct Plan {
-    GroupShape *shapes;     // [groups + 1], written by the host's part of the plan
+    int *header;            // units of the shared line, units per CTA; units of the own line, units per worker
+    GroupShape *shapes;     // [groups], written by the host's part of the plan
     Group *groups;
     Query *query;
-    Line shared, own;
+    Start *shared, *own;    // [ctas], [own_workers]
 };
 
 // Everything a call has in hand besides its tensors.
@@ -65,38 +65,100 @@ struct Call {
     int shared_items;
 };
 
-inline int64_t align8(int64_t n) { return (n + 7) / 8 * 8; }
 inline int64_t part_rows(const Shape &s, int64_t shared) { return (shared + s.ctas) * s.row_tile + ((int64_t)s.own_items() + s.own_workers) * s.own_slot(); }
-inline Line line_of(int *&p, int *header, int64_t items, int64_t workers) {
-    Line l;
-    l.header = header;
-    l.first = p; p += align8(workers);
-    l.item = (int2 *)p; p += align8(2 * items);
-    l.segments = (Segment *)p; p += 8 * (items + workers);
-    return l;
-}
-inline Plan plan_of(int *base, const Shape &s, int64_t shared, int64_t *ints = nullptr) {
+inline Plan plan_of(int *base, const Shape &s, int64_t *ints = nullptr) {
     Plan r;
     int *p = base + 16;
-    r.shapes = (GroupShape *)p; p += align8(3LL * (s.groups + 1));
-    r.groups = (Group *)p; p += align8(4LL * s.groups);
-    r.query = (Query *)p; p += 8LL * s.n_queries();
-    r.shared = line_of(p, base, shared, s.ctas);
-    r.own = line_of(p, base + 2, s.own_items(), s.own_workers);
+    r.header = base;
+    r.shapes = (GroupShape *)p; p += (4LL * s.groups + 15) / 16 * 16;
+    r.groups = (Group *)p; p += (8LL * s.groups + 15) / 16 * 16;
+    r.query = (Query *)p; p += 16LL * s.n_queries();
+    r.shared = (Start *)p; p += 16LL * s.ctas;
+    r.own = (Start *)p; p += 16LL * s.own_workers;
     if (ints) *ints = p - base;
     return r;
 }
-inline int64_t plan_ints(const Shape &s, int64_t shared) {
+inline int64_t plan_ints(const Shape &s) {
     int64_t n;
-    (void)plan_of((int *)nullptr, s, shared, &n);
+    (void)plan_of((int *)nullptr, s, &n);
     return n;
 }
 
-// First row of the partial results of segment i + w of a kind.
+// First row of the partial results of segment (item, worker) of a kind, at = item + worker: that sum is another one for every segment of a line.
 __host__ __device__ inline int64_t part_shared(const Shape &s, int at) { return (int64_t)at * s.row_tile; }
 __host__ __device__ inline int64_t part_own(const Shape &s, int shared_items, int at) {
     return (int64_t)(shared_items + s.ctas) * s.row_tile + (int64_t)at * s.own_slot();
 }
+
+// The segments of a worker, one after the other.
+struct SharedWalk {
+    int group, local, unit, left, cta;
+    Group g;
+    __device__ __forceinline__ SharedWalk(const Call &c, int cta) : cta(cta) {
+        const int4 *p = reinterpret_cast<const int4 *>(c.plan.shared + cta);
+        const int4 a = p[0], b = p[1], d = p[2];
+        group = a.x; local = a.y; unit = a.z; left = a.w;
+        g = Group{b.x, b.y, b.z, b.w, d.x, d.y, d.z, d.w};
+    }
+    __device__ __forceinline__ bool next(const Call &c, Segment &s) {
+        if (left <= 0) return false;
+        const Shape &sh = c.sh;
+        while (g.units == 0 || local == sh.kv_heads * g.row_tiles) {
+            const int4 *p = reinterpret_cast<const int4 *>(c.plan.groups + ++group);
+            const int4 b = p[0], d = p[1];
+            g = Group{b.x, b.y, b.z, b.w, d.x, d.y, d.z, d.w};
+            local = 0;
+        }
+        const int tile = local % g.row_tiles;
+        s.head = local / g.row_tiles;
+        s.row0 = g.query0 * sh.per_kv() + tile * sh.row_tile;
+        s.rows = min(sh.row_tile, g.rows - tile * sh.row_tile);
+        s.slot = g.slot;
+        s.units = min(left, g.units - unit);
+        s.key0 = unit * kKeyTile;
+        s.key1 = min(g.shared, (unit + s.units) * kKeyTile);
+        s.part = (int)part_shared(sh, g.item0 + local + cta);
+        left -= s.units;
+        unit += s.units;
+        if (unit == g.units) { unit = 0; ++local; }
+        return true;
+    }
+};
+struct OwnWalk {
+    int query, local, unit, left, worker;
+    int len, slot, shared, units;
+    __device__ __forceinline__ OwnWalk(const Call &c, int worker) : worker(worker) {
+        const int4 *p = reinterpret_cast<const int4 *>(c.plan.own + worker);
+        const int4 a = p[0], b = p[1];
+        query = a.x; local = a.y; unit = a.z; left = a.w;
+        len = b.x; slot = b.y; shared = b.z; units = b.w;
+    }
+    __device__ __forceinline__ bool next(const Call &c, Segment &s) {
+        if (left <= 0) return false;
+        const Shape &sh = c.sh;
+        const int tiles = sh.own_tiles(), per = sh.per_kv();
+        while (units == 0 || local == sh.kv_heads * tiles) {
+            const int4 b = *reinterpret_cast<const int4 *>(c.plan.query + ++query);
+            len = b.x; slot = b.y; shared = b.z; units = b.w;
+            local = 0;
+        }
+        const int tile = tiles == 1 ? 0 : local % tiles;
+        s.head = tiles == 1 ? local : local / tiles;
+        s.row0 = query * per + tile * sh.own_rows;
+        s.rows = min(sh.own_rows, per - tile * sh.own_rows);
+        s.slot = slot;
+        s.units = min(left, units - unit);
+        s.key0 = shared + unit * sh.own_step;
+        s.key1 = min(len, s.key0 + s.units * sh.own_step);
+        s.part = (int)part_own(sh, c.shared_items, query * sh.kv_heads * tiles + local + worker);
+        left -= s.units;
+        unit += s.units;
+        if (unit == units) { unit = 0; ++local; }
+        return true;
+    }
+};
+// n / per for the rows of a call, by a multiplication: exact for n < 2^22, per <= 32, with rcp = ceil(2^32 / per)
+__device__ __forceinline__ int div_per(int n, const Shape &s) { return s.rcp ? (int)__umulhi((unsigned)n, s.rcp) : n; }
 
 // The kernels that make the segments' results (prefix_attn_simt.cu: f32; prefix_attn_mma.cu: f16 and bf16).
 void simt_launch(const Call &c, const cq_kv_cache &cache, int layer, const void *q, int64_t q_stride, float scale, cudaStream_t st);

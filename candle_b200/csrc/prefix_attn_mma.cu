@@ -1,9 +1,9 @@
 // Segments of the shared-prefix attention (prefix_attn.cuh) on the tensor cores: f16 and bf16 caches.
 //
-// Shared items (many rows, keys mostly from L2): tiles of 128 rows x 128 keys by tcgen05.  S = Q K^T goes to tensor memory; thread r of the softmax
+// Shared items (many rows, keys mostly from L2): tiles of 128 rows x 64 keys by tcgen05.  S = Q K^T goes to tensor memory; thread r of the softmax
 // warps owns row r, reads it there, and writes the weights 2^(s c - m), c = scale log2 e, back over it in 16 bits as the first operand of O += P V.
-// Warps: 0-3 softmax (TMEM lanes 32 w ..), 4 copies, 5 MMA.  Within a CTA the products and the softmax of a tile follow one another (the
-// weights lie where the scores were: 256 columns a CTA); two CTAs per SM fill each other's gaps.
+// Warps: 0-3 softmax (TMEM lanes 32 w ..), 4 copies, 5 MMA.  256 columns a CTA: the scores of two tiles, so that one tile's softmax has the products
+// of its neighbours beside it, and the outputs.  Two CTAs per SM.
 //
 // Own items (as many rows as a KV head has query heads, keys from HBM): a warp is a worker of its own, 16 rows x 16 keys a step by mma.sync, with two
 // steps of keys and values on their way.  Through the first form an item of four rows costs the waits of a whole tile chain - QK,
@@ -26,16 +26,17 @@ namespace {
 using namespace cq_attn;
 using namespace cq_prompt;
 
-constexpr int kThreads = 32 * kMmaWarps, kStages = 2, kCols = 256, kHalfBytes = 128 * 128;       // a half: 128 rows of 64 elements
-constexpr int kS = 0, kO = 128;                                                          // columns of scores / weights and of outputs
+constexpr int kThreads = 32 * kMmaWarps, kStages = 2, kCols = 256, kHalfBytes = 128 * 128;       // 128 rows of 64 elements
+constexpr int kS = 0, kO = 128;                                      // columns of scores / weights (two tiles) and of outputs
 
-struct Bars { uint64_t q, k, v, s, p, o; };      // operands there (q, k, v), scores there (and Q, K free), weights there, outputs there (and V free)
+// operands there (q, k, v), scores there (and K free), weights there, outputs there (and V, weights free)
+struct Bars { uint64_t q, k[2], v[2], s[2], p[2], o[2]; };
 
 constexpr int kStep = 16;                // keys of a step of an own item
 template <int D> struct Step { uint8_t k[D / 64][kStep * 128], v[D / 64][kStep * 128]; };
 template <int D> struct Tiles {
     union {
-        struct { uint8_t q[D / 64][kHalfBytes], k[D / 64][kHalfBytes], v[D / 64][kHalfBytes]; };
+        struct { uint8_t q[D / 64][kHalfBytes], k[2][D / 64][kKeyTile * 128], v[2][D / 64][kKeyTile * 128]; };
         Step<D> step[kMmaWarps][kStages];
     };
     Bars bar;
@@ -64,13 +65,10 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&v)[16
                  ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]),
                  "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]) : "memory");
 }
-__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&v)[32]) {
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
-        "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};"
-        ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]),
-        "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]),
-        "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31]) : "memory");
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&v)[16]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]),
+                   "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]) : "r"(taddr) : "memory");
 }
 __device__ __forceinline__ float ex2(float x) {
     float r;
@@ -92,58 +90,55 @@ template <bool BF16> __device__ __forceinline__ uint32_t pack(float a, float b, 
 }
 
 // The CTA's share of the shared line.  False: a wait gave up.
+// The scores of two tiles have room, so QK of the next tile and PV of the one before run beside a tile's softmax; a barrier per buffer, since
+// no waiter may fall two phases behind.
 template <int D, bool BF16>
 __device__ bool shared_part(Tiles<D> &sm, const cq_kv_cache &cache, const cq_kv::State &st, const Call &call, const CUtensorMap &k_map, const CUtensorMap &v_map,
                             const uint8_t *__restrict__ q, int64_t q_stride, float c, uint32_t tmem) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, page = st.page;
-    constexpr uint32_t kIdescQK = (1u << 4) | (BF16 ? (1u << 7) | (1u << 10) : 0u) | (128u >> 3) << 17 | (128u >> 4) << 24;
+    constexpr uint32_t kIdescQK = (1u << 4) | (BF16 ? (1u << 7) | (1u << 10) : 0u) | ((uint32_t)kKeyTile >> 3) << 17 | (128u >> 4) << 24;
     constexpr uint32_t kIdescPV = (1u << 4) | (BF16 ? (1u << 7) | (1u << 10) : 0u) | (1u << 16) | ((uint32_t)D >> 3) << 17 | (128u >> 4) << 24;
     volatile int *abort_flag = &sm.abort;
-    const Line &line = call.plan.shared;
-    const int chunk = line.header[1];
-    int left = min(line.header[0] - (int)blockIdx.x * chunk, chunk);
-    int at = left > 0 ? line.first[blockIdx.x] : 0;
+    SharedWalk walk(call, blockIdx.x);
+    Segment seg;
     bool ok = true;
+    unsigned tile = 0;              // buffer tile & 1, phase tile / 2
     if (warp < 4) {
         const int per = call.sh.per_kv(), row = warp * 32 + lane;
         const uint32_t mine = tmem + ((uint32_t)(warp * 32) << 16);
-        unsigned tile = 0;              // parity of the barriers
-        for (; ok && left > 0; ++at) {
-            const Segment seg = line.segments[at];
-            if (seg.units == 0) continue;
-            left -= seg.units;
+        while (ok && walk.next(call, seg)) {
             // Q: all rows of the segment by the four warps; rows behind them keep what was there, and nobody reads their results
             const uint8_t *src = q + (int64_t)seg.head * per * D * 2;
             for (int i = tid; i < seg.rows * (D / 8); i += 128) {
-                const int r = i / (D / 8), x = i % (D / 8), n = seg.row0 + r;
-                const uint4 w = *reinterpret_cast<const uint4 *>(src + ((int64_t)(n / per) * q_stride + (int64_t)(n % per) * D + x * 8) * 2);
-                *reinterpret_cast<uint4 *>(&sm.q[x >> 3][r * 128 + ((x & 7) ^ (r & 7)) * 16]) = w;
+                const int r = i / (D / 8), x = i % (D / 8), n = div_per(seg.row0 + r, call.sh), in = seg.row0 + r - n * per;
+                cq_cp_async16(&sm.q[x >> 3][r * 128 + ((x & 7) ^ (r & 7)) * 16], src + ((int64_t)n * q_stride + (int64_t)in * D + x * 8) * 2);
             }
+            cq_cp_async_commit();
+            cq_cp_async_wait<0>();
             fence_proxy_async_smem();
             arrive_warp(&sm.bar.q, lane);
             const bool active = warp * 32 < seg.rows;
             float m = -INFINITY, l = 0.0f;
             for (int j = 0; j < seg.units; ++j, ++tile) {
-                const int n = seg.key1 - seg.key0 - j * kKeyTile;          // keys of this tile, if fewer than 128
-                if (!(ok = wait_warp(&sm.bar.s, tile & 1, abort_flag))) break;
+                const int n = seg.key1 - seg.key0 - j * kKeyTile;          // keys of this tile, if fewer than kKeyTile
+                const unsigned b = tile & 1, phase = tile >> 1 & 1;
+                const uint32_t sp = mine + kS + b * kKeyTile;
+                if (!(ok = wait_warp(&sm.bar.s[b], phase, abort_flag))) break;
                 tc_fence_after();
                 if (active) {
-                    uint32_t s[32];
-                    float mx = -INFINITY;
+                    uint32_t s[2][32];
+                    tmem_ld32(sp, s[0]);
+                    tmem_ld32(sp + 32, s[1]);
+                    tmem_ld_wait();
+                    if (n < kKeyTile) {
 #pragma unroll
-                    for (int x = 0; x < 4; ++x) {
-                        tmem_ld32(mine + kS + 32 * x, s);
-                        tmem_ld_wait();
-                        if (n >= 32 * (x + 1)) {
-#pragma unroll
-                            for (int i = 0; i < 32; ++i) mx = fmaxf(mx, __uint_as_float(s[i]));
-                        } else {
-#pragma unroll
-                            for (int i = 0; i < 32; ++i)
-                                if (32 * x + i < n) mx = fmaxf(mx, __uint_as_float(s[i]));
-                        }
+                        for (int i = 0; i < kKeyTile; ++i)
+                            if (i >= n) s[i >> 5][i & 31] = 0xff800000u;        // -inf
                     }
-                    mx *= c;
+                    float mx = -INFINITY, my = -INFINITY;
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) { mx = fmaxf(mx, __uint_as_float(s[0][i])); my = fmaxf(my, __uint_as_float(s[1][i])); }
+                    mx = fmaxf(mx, my) * c;
                     if (j == 0) m = mx;
                     else {
                         const bool up = mx > m + 8.0f;          // from -inf as well
@@ -151,53 +146,45 @@ __device__ bool shared_part(Tiles<D> &sm, const cq_kv_cache &cache, const cq_kv:
                             const float f = up ? ex2(m - mx) : 1.0f;
                             if (up) m = mx;
                             l *= f;
+                            if (!(ok = wait_warp(&sm.bar.o[b ^ 1], (tile - 1) >> 1 & 1, abort_flag))) break;        // the outputs so far
+                            tc_fence_after();
 #pragma unroll
-                            for (int x = 0; x < D / 32; ++x) {
-                                tmem_ld32(mine + kO + 32 * x, s);
+                            for (int x = 0; x < D / 16; ++x) {
+                                uint32_t o[16];
+                                tmem_ld16(mine + kO + 16 * x, o);
                                 tmem_ld_wait();
 #pragma unroll
-                                for (int i = 0; i < 32; ++i) s[i] = __float_as_uint(__uint_as_float(s[i]) * f);
-                                tmem_st32(mine + kO + 32 * x, s);
+                                for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+                                tmem_st16(mine + kO + 16 * x, o);
                             }
                         }
                     }
                     const float base = m == -INFINITY ? 0.0f : m;
                     float sum0 = 0.0f, sum1 = 0.0f;
 #pragma unroll
-                    for (int x = 0; x < 4; ++x) {
-                        tmem_ld32(mine + kS + 32 * x, s);
-                        tmem_ld_wait();
+                    for (int x = 0; x < 2; ++x) {
                         uint32_t w[16];
-                        if (n >= 32 * (x + 1)) {
 #pragma unroll
-                            for (int i = 0; i < 16; ++i)
-                                w[i] = pack<BF16>(ex2(__fmaf_rn(__uint_as_float(s[2 * i]), c, -base)), ex2(__fmaf_rn(__uint_as_float(s[2 * i + 1]), c, -base)),
-                                                  i & 1 ? sum1 : sum0);
-                        } else {
-#pragma unroll
-                            for (int i = 0; i < 16; ++i) {
-                                const float a = 32 * x + 2 * i < n ? ex2(__fmaf_rn(__uint_as_float(s[2 * i]), c, -base)) : 0.0f;
-                                const float b = 32 * x + 2 * i + 1 < n ? ex2(__fmaf_rn(__uint_as_float(s[2 * i + 1]), c, -base)) : 0.0f;
-                                w[i] = pack<BF16>(a, b, i & 1 ? sum1 : sum0);
-                            }
-                        }
-                        tmem_st16(mine + kS + 16 * x, w);       // over scores that this thread has read
+                        for (int i = 0; i < 16; ++i)
+                            w[i] = pack<BF16>(ex2(__fmaf_rn(__uint_as_float(s[x][2 * i]), c, -base)), ex2(__fmaf_rn(__uint_as_float(s[x][2 * i + 1]), c, -base)),
+                                              i & 1 ? sum1 : sum0);
+                        tmem_st16(sp + 16 * x, w);              // over the scores
                     }
                     l += sum0 + sum1;
                     tmem_st_wait();
                     tc_fence_before();
                 }
                 if (n < kKeyTile) {
-                    if (!(ok = wait_warp(&sm.bar.v, tile & 1, abort_flag))) break;
+                    if (!(ok = wait_warp(&sm.bar.v[b], phase, abort_flag))) break;
                     for (int i = tid; i < (kKeyTile - n) * (D / 8); i += 128) {
                         const int r = n + i / (D / 8), x = i % (D / 8);
-                        *reinterpret_cast<uint4 *>(&sm.v[x >> 3][r * 128 + (x & 7) * 16]) = make_uint4(0, 0, 0, 0);
+                        *reinterpret_cast<uint4 *>(&sm.v[b][x >> 3][r * 128 + (x & 7) * 16]) = make_uint4(0, 0, 0, 0);
                     }
                     fence_proxy_async_smem();
                 }
-                arrive_warp(&sm.bar.p, lane);
+                arrive_warp(&sm.bar.p[b], lane);
             }
-            if (!ok || !(ok = wait_warp(&sm.bar.o, (tile - 1) & 1, abort_flag))) break;
+            if (!ok || !(ok = wait_warp(&sm.bar.o[(tile - 1) & 1], (tile - 1) >> 1 & 1, abort_flag))) break;
             tc_fence_after();
             if (active) {
                 float *to = call.o + (int64_t)(seg.part + row) * D;
@@ -216,80 +203,85 @@ __device__ bool shared_part(Tiles<D> &sm, const cq_kv_cache &cache, const cq_kv:
             }
         }
     } else if (warp == 4) {
-        unsigned tile = 0, k_sent = 0, v_sent = 0;
-        for (; ok && left > 0; ++at) {
-            const Segment seg = line.segments[at];
-            if (seg.units == 0) continue;
-            left -= seg.units;
+        const int shift = 31 - __clz(page), box = min(page, kKeyTile);
+        while (ok && walk.next(call, seg)) {
             const int *table = st.tables + (size_t)seg.slot * st.max_pages;
+            int base = INT32_MIN / 2, ids = -1;             // page numbers base .. base + 31 of the table, one a lane
             for (int j = 0; j < seg.units; ++j, ++tile) {
-                const int key = seg.key0 + j * kKeyTile + lane * page;           // a lane takes a page
-                int id = -1;
-                if (lane * page < kKeyTile && key < seg.key1) {
-                    id = table[key / page];
-                    if (id < 0 || id >= st.pages) { id = -1; atomicCAS(st.header, cq_kv::kOk, cq_kv::kBadPage); }
+                const unsigned b = tile & 1, before = (tile >> 1 & 1) ^ 1;
+                const int key = seg.key0 + j * kKeyTile, p0 = key >> shift, mine = key + lane * box;
+                if (((key + kKeyTile - 1) >> shift) - base >= 32) {
+                    base = p0;
+                    ids = (p0 + lane) << shift < seg.key1 ? table[p0 + lane] : -1;
                 }
-                const unsigned bytes = (unsigned)__popc(__ballot_sync(0xffffffffu, id >= 0)) * page * D * 2;
-                const int y = (id * cache.kv_heads + seg.head) * page;
-                if (tile > 0 && !(ok = wait_warp(&sm.bar.s, (tile - 1) & 1, abort_flag))) break;
-                if (lane == 0) cq_mbar_expect_tx(&sm.bar.k, bytes);
+                int id = __shfl_sync(0xffffffffu, ids, ((mine >> shift) - base) & 31);           // a lane takes a box
+                if (lane * box >= kKeyTile || mine >= seg.key1) id = -1;
+                else if (id < 0 || id >= st.pages) { id = -1; atomicCAS(st.header, cq_kv::kOk, cq_kv::kBadPage); }
+                const unsigned bytes = (unsigned)__popc(__ballot_sync(0xffffffffu, id >= 0)) * box * D * 2;
+                const int y = ((id * cache.kv_heads + seg.head) << shift) + (mine & (page - 1));
+                if (tile >= 2 && !(ok = wait_warp(&sm.bar.s[b], before, abort_flag))) break;
+                if (lane == 0) cq_mbar_expect_tx(&sm.bar.k[b], bytes);
                 __syncwarp();
                 if (id >= 0)
 #pragma unroll
-                    for (int h = 0; h < D / 64; ++h) cq_tmap::load_2d(&sm.k[h][lane * page * 128], &k_map, 64 * h, y, &sm.bar.k);
-                ++k_sent;
-                if (tile > 0 && !(ok = wait_warp(&sm.bar.o, (tile - 1) & 1, abort_flag))) break;
-                if (lane == 0) cq_mbar_expect_tx(&sm.bar.v, bytes);
+                    for (int h = 0; h < D / 64; ++h) cq_tmap::load_2d(&sm.k[b][h][lane * box * 128], &k_map, 64 * h, y, &sm.bar.k[b]);
+                if (tile >= 2 && !(ok = wait_warp(&sm.bar.o[b], before, abort_flag))) break;
+                if (lane == 0) cq_mbar_expect_tx(&sm.bar.v[b], bytes);
                 __syncwarp();
                 if (id >= 0)
 #pragma unroll
-                    for (int h = 0; h < D / 64; ++h) cq_tmap::load_2d(&sm.v[h][lane * page * 128], &v_map, 64 * h, y, &sm.bar.v);
-                ++v_sent;
+                    for (int h = 0; h < D / 64; ++h) cq_tmap::load_2d(&sm.v[b][h][lane * box * 128], &v_map, 64 * h, y, &sm.bar.v[b]);
             }
         }
-        if (!ok) {                      // leaving early: not before what is on its way has come
-            if (k_sent) (void)cq_mbar_wait_bounded(&sm.bar.k, (k_sent - 1) & 1);
-            if (v_sent) (void)cq_mbar_wait_bounded(&sm.bar.v, (v_sent - 1) & 1);
-        }
+        if (!ok)                        // leaving early: not before what is on its way has come (a copy that was never sent costs the wait's bound)
+            for (unsigned b = 0; b < 2; ++b)
+                if (tile >= b) {
+                    const unsigned last = (tile - b) >> 1 & 1;          // phase of the newest copy that may be out
+                    (void)(cq_mbar_wait_bounded(&sm.bar.k[b], last ^ 1) && cq_mbar_wait_bounded(&sm.bar.k[b], last));
+                    (void)(cq_mbar_wait_bounded(&sm.bar.v[b], last ^ 1) && cq_mbar_wait_bounded(&sm.bar.v[b], last));
+                }
     } else {
-        unsigned tile = 0, segment = 0, s_sent = 0, o_sent = 0;
-        const uint32_t qa = uniform(cq_smem_u32(&sm.q[0][0]) >> 4), ka = uniform(cq_smem_u32(&sm.k[0][0]) >> 4), va = uniform(cq_smem_u32(&sm.v[0][0]) >> 4);
+        unsigned segment = 0, qk = 0;           // tiles whose first product is under way
+        const uint32_t qa = uniform(cq_smem_u32(&sm.q[0][0]) >> 4), ka = uniform(cq_smem_u32(&sm.k[0][0][0]) >> 4), va = uniform(cq_smem_u32(&sm.v[0][0][0]) >> 4);
         const uint32_t t0 = uniform(tmem);
-        for (; ok && left > 0; ++at) {
-            const int tiles = (int)uniform((uint32_t)line.segments[at].units);
-            if (tiles == 0) continue;
-            left -= tiles;
-            if (!(ok = wait_warp(&sm.bar.q, segment++ & 1, abort_flag))) break;
-            for (int j = 0; j < tiles; ++j, ++tile) {
-                if (!(ok = wait_warp(&sm.bar.k, tile & 1, abort_flag))) break;
-                if (tile > 0 && !(ok = wait_warp(&sm.bar.o, (tile - 1) & 1, abort_flag))) break;      // the weights before have been read
+        constexpr uint32_t kHalfK = kKeyTile * 128 >> 4, kBuf = D / 64 * kHalfK;
+        auto scores = [&]() {                   // S = Q K^T of tile qk
+            const unsigned b = qk & 1, phase = qk >> 1 & 1;
+            if (!wait_warp(&sm.bar.k[b], phase, abort_flag)) return false;
+            if (qk >= 2 && !wait_warp(&sm.bar.o[b], phase ^ 1, abort_flag)) return false;          // the weights there have been read
+            tc_fence_after();
+            if (elect_one()) {
+#pragma unroll
+                for (int x = 0; x < D / 16; ++x)
+                    mma_ss(t0 + kS + b * kKeyTile, qa + (x >> 2) * (kHalfBytes >> 4) + (x & 3) * 2, ka + b * kBuf + (x >> 2) * kHalfK + (x & 3) * 2, kIdescQK, x > 0);
+                tc_commit(&sm.bar.s[b]);
+            }
+            __syncwarp();
+            ++qk;
+            return true;
+        };
+        while (ok && walk.next(call, seg)) {
+            const int units = (int)uniform((uint32_t)seg.units);
+            if (!(ok = wait_warp(&sm.bar.q, segment++ & 1, abort_flag) && scores())) break;
+            for (int j = 0; j < units; ++j, ++tile) {
+                const unsigned b = tile & 1, phase = tile >> 1 & 1;
+                if (j + 1 < units && !(ok = scores())) break;
+                if (!(ok = wait_warp(&sm.bar.v[b], phase, abort_flag)) || !(ok = wait_warp(&sm.bar.p[b], phase, abort_flag))) break;
                 tc_fence_after();
                 if (elect_one()) {
 #pragma unroll
-                    for (int x = 0; x < D / 16; ++x) {
-                        const uint32_t off = (x >> 2) * (kHalfBytes >> 4) + (x & 3) * 2;
-                        mma_ss(t0 + kS, qa + off, ka + off, kIdescQK, x > 0);
-                    }
-                    tc_commit(&sm.bar.s);
+                    for (int x = 0; x < kKeyTile / 16; ++x)
+                        mma_ts(t0 + kO, t0 + kS + b * kKeyTile + 8 * x, (va + b * kBuf + x * (2048 >> 4)) | kHalfK << 16, kIdescPV, j > 0 || x > 0);
+                    tc_commit(&sm.bar.o[b]);
                 }
                 __syncwarp();
-                ++s_sent;
-                if (!(ok = wait_warp(&sm.bar.v, tile & 1, abort_flag)) || !(ok = wait_warp(&sm.bar.p, tile & 1, abort_flag))) break;
-                tc_fence_after();
-                if (elect_one()) {
-#pragma unroll
-                    for (int x = 0; x < 8; ++x)
-                        mma_ts(t0 + kO, t0 + kS + 8 * x, (va + x * (2048 >> 4)) | (uint32_t)(kHalfBytes >> 4) << 16, kIdescPV, j > 0 || x > 0);
-                    tc_commit(&sm.bar.o);
-                }
-                __syncwarp();
-                ++o_sent;
             }
         }
-        if (!ok) {                      // nor before the products have ended
-            if (s_sent) (void)cq_mbar_wait_bounded(&sm.bar.s, (s_sent - 1) & 1);
-            if (o_sent) (void)cq_mbar_wait_bounded(&sm.bar.o, (o_sent - 1) & 1);
-        }
+        if (!ok)                        // nor before the products have ended
+            for (unsigned b = 0; b < 2; ++b) {
+                if (qk > b) (void)cq_mbar_wait_bounded(&sm.bar.s[b], (qk - 1 - b) >> 1 & 1);
+                if (tile > b) (void)cq_mbar_wait_bounded(&sm.bar.o[b], (tile - 1 - b) >> 1 & 1);
+            }
     }
     return ok;
 }
@@ -312,27 +304,29 @@ template <bool BF16> __device__ __forceinline__ void mma16816(float (&d)[4], con
 
 // The copies of a warp's steps, ahead of their use and across its segments.
 template <int D> struct Loader {
+    OwnWalk walk;
     Segment seg;
-    int at, step, left;             // segment, step in it, steps of this worker not yet sent
-    int base, ids;                  // page numbers base .. base + 31 of the segment's table, one a lane
-    __device__ __forceinline__ void send(Step<D> &to, uint64_t *bar, const Line &line, const cq_kv::State &st, int kv_heads, const CUtensorMap &k_map, const CUtensorMap &v_map,
+    int step, sent;                 // step in the segment, steps sent
+    int base, ids, shift;           // page numbers base .. base + 31 of the segment's table, one a lane
+    __device__ __forceinline__ Loader(const Call &call, int worker, int page_shift) : walk(call, worker), step(0), sent(0), shift(page_shift) { seg.units = 0; }
+    __device__ __forceinline__ void send(Step<D> &to, uint64_t *bar, const Call &call, const cq_kv::State &st, int kv_heads, const CUtensorMap &k_map, const CUtensorMap &v_map,
                                          int lane) {
-        while (step == seg.units) {
-            seg = line.segments[++at];
+        if (step == seg.units) {
+            if (!walk.next(call, seg)) return;
             step = 0;
             base = INT32_MIN / 2;
         }
-        const int key = seg.key0 + kStep * step, j = key / st.page;
+        const int key = seg.key0 + kStep * step, j = key >> shift;
         if (j - base >= 32) {
             base = j;
-            ids = (j + lane) * st.page < seg.key1 ? st.tables[(size_t)seg.slot * st.max_pages + j + lane] : -1;
+            ids = (j + lane) << shift < seg.key1 ? st.tables[(size_t)seg.slot * st.max_pages + j + lane] : -1;
         }
         const int id = __shfl_sync(0xffffffffu, ids, j - base);
         const bool there = id >= 0 && id < st.pages;
         if (lane == 0) {
             cq_mbar_expect_tx(bar, there ? (unsigned)sizeof(Step<D>) : 0u);
             if (there) {
-                const int y = (id * kv_heads + seg.head) * st.page + key % st.page;
+                const int y = ((id * kv_heads + seg.head) << shift) + (key & (st.page - 1));
 #pragma unroll
                 for (int h = 0; h < D / 64; ++h) {
                     cq_tmap::load_2d(to.k[h], &k_map, 64 * h, y, bar);
@@ -341,7 +335,7 @@ template <int D> struct Loader {
             } else atomicCAS(st.header, cq_kv::kOk, cq_kv::kBadPage);
         }
         ++step;
-        --left;
+        ++sent;
     }
 };
 
@@ -350,17 +344,15 @@ template <int D, bool BF16>
 __device__ bool own_part(Tiles<D> &sm, const cq_kv_cache &cache, const cq_kv::State &st, const Call &call, const CUtensorMap &k_map, const CUtensorMap &v_map,
                          const uint8_t *__restrict__ q, int64_t q_stride, float c) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, x2 = (lane & 3) * 2, per = call.sh.per_kv();
-    const Line &line = call.plan.own;
-    const int worker = blockIdx.x * kMmaWarps + warp, chunk = line.header[1], units = min(line.header[0] - worker * chunk, chunk);
-    if (units <= 0) return true;
+    const int worker = blockIdx.x * kMmaWarps + warp;
     Step<D> *steps = sm.step[warp];
     uint64_t *bars = sm.step_bar[warp];
-    int at = line.first[worker] - 1;
-    Loader<D> load;
-    load.at = at; load.step = 0; load.left = units; load.seg.units = 0;
+    Loader<D> load(call, worker, 31 - __clz(st.page));
+    OwnWalk walk = load.walk;
+    const int units = walk.left;
+    if (units <= 0) return true;
 #pragma unroll
-    for (int i = 0; i < kStages; ++i)
-        if (load.left > 0) load.send(steps[i], &bars[i], line, st, cache.kv_heads, k_map, v_map, lane);
+    for (int i = 0; i < kStages; ++i) load.send(steps[i], &bars[i], call, st, cache.kv_heads, k_map, v_map, lane);
     Segment seg;
     seg.units = 0;
     int step = 0;
@@ -370,10 +362,10 @@ __device__ bool own_part(Tiles<D> &sm, const cq_kv_cache &cache, const cq_kv::St
     for (int u = 0; u < units; ++u) {
         const int stage = u % kStages;
         if (step == seg.units) {
-            do seg = line.segments[++at];
-            while (seg.units == 0);
+            walk.next(call, seg);
             step = 0;
-            const uint8_t *src = q + ((int64_t)(seg.row0 / per) * q_stride + (int64_t)(seg.head * per + seg.row0 % per) * D) * 2;
+            const int query = div_per(seg.row0, call.sh);
+            const uint8_t *src = q + ((int64_t)query * q_stride + (int64_t)(seg.head * per + seg.row0 - query * per) * D) * 2;
 #pragma unroll
             for (int x = 0; x < D / 16; ++x)
 #pragma unroll
@@ -449,7 +441,7 @@ __device__ bool own_part(Tiles<D> &sm, const cq_kv_cache &cache, const cq_kv::St
             mma16816<BF16>(o[2 * x + 1], p, b[2], b[3]);
         }
         __syncwarp();
-        if (load.left > 0) load.send(steps[stage], &bars[stage], line, st, cache.kv_heads, k_map, v_map, lane);
+        load.send(steps[stage], &bars[stage], call, st, cache.kv_heads, k_map, v_map, lane);
         if (++step == seg.units) {
             l0 += __shfl_xor_sync(0xffffffffu, l0, 1);
             l1 += __shfl_xor_sync(0xffffffffu, l1, 1);
@@ -469,7 +461,7 @@ __device__ bool own_part(Tiles<D> &sm, const cq_kv_cache &cache, const cq_kv::St
     }
     if (!ok)                            // leaving early: not before what is on its way has come
         for (int i = 0; i < kStages; ++i) {
-            const int sent = (units - load.left - i + kStages - 1) / kStages;       // copies into this stage
+            const int sent = (load.sent - i + kStages - 1) / kStages;       // copies into this stage
             if (sent > 0) (void)cq_mbar_wait_bounded(&bars[i], (sent - 1) & 1);
         }
     return ok;
@@ -485,8 +477,11 @@ __global__ void __launch_bounds__(kThreads, 2) prefix_mma_kernel(const cq_kv_cac
     const cq_kv::State st = cq_kv::state_of(cache);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     if (tid == 0) {
-        cq_mbar_init(&sm.bar.q, 4); cq_mbar_init(&sm.bar.k, 1); cq_mbar_init(&sm.bar.v, 1);
-        cq_mbar_init(&sm.bar.s, 1); cq_mbar_init(&sm.bar.p, 4); cq_mbar_init(&sm.bar.o, 1);
+        cq_mbar_init(&sm.bar.q, 4);
+        for (int i = 0; i < 2; ++i) {
+            cq_mbar_init(&sm.bar.k[i], 1); cq_mbar_init(&sm.bar.v[i], 1);
+            cq_mbar_init(&sm.bar.s[i], 1); cq_mbar_init(&sm.bar.p[i], 4); cq_mbar_init(&sm.bar.o[i], 1);
+        }
         for (int i = 0; i < kMmaWarps * kStages; ++i) cq_mbar_init(&sm.step_bar[0][i], 1);
         sm.abort = 0;
         cq_fence_mbar_init();
@@ -552,8 +547,9 @@ void launch(const Call &c, const cq_kv_cache &cache, const CUtensorMap (&m)[4], 
 bool cq_attn::mma_launch(const Call &c, const cq_kv_cache &cache, int layer, const void *q, int64_t q_stride, float scale, cudaStream_t st) {
     const int64_t rows = (int64_t)cache.pages * cache.kv_heads * cache.page_size, offset = rows * layer * cache.head_dim * 2;
     const uint8_t *k = (const uint8_t *)cache.k + offset, *v = (const uint8_t *)cache.v + offset;
+    const int box = cache.page_size < kKeyTile ? cache.page_size : kKeyTile;
     CUtensorMap m[4];
-    if (!pool_map(k, rows, cache.head_dim, cache.page_size, m[0]) || !pool_map(v, rows, cache.head_dim, cache.page_size, m[1]) ||
+    if (!pool_map(k, rows, cache.head_dim, box, m[0]) || !pool_map(v, rows, cache.head_dim, box, m[1]) ||
         !pool_map(k, rows, cache.head_dim, kStep, m[2]) || !pool_map(v, rows, cache.head_dim, kStep, m[3])) {
         cq_set_status(CQ_ERR_CUDA, "prefix_attention: cuTensorMapEncodeTiled is not available or refused the pool");
         return false;

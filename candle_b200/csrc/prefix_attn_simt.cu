@@ -76,19 +76,14 @@ __global__ void __launch_bounds__(kThreads) prefix_simt_kernel(const cq_kv_cache
     extern __shared__ __align__(16) uint8_t raw[];
     Smem<D> &sm = *reinterpret_cast<Smem<D> *>(raw);
     const cq_kv::State s = cq_kv::state_of(cache);
-    const Plan &pl = call.plan;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, per = call.sh.per_kv();
     cq_pdl_launch_dependents();
     cq_pdl_wait();
     const T *k_pool = reinterpret_cast<const T *>(cache.k), *v_pool = reinterpret_cast<const T *>(cache.v);
-    for (int kind = 0; kind < 2; ++kind) {
-    const Line &line = kind ? pl.own : pl.shared;
-    const int chunk = line.header[1];
-    int left = min(line.header[0] - (int)blockIdx.x * chunk, chunk);
-    for (int at = left > 0 ? line.first[blockIdx.x] : 0; left > 0; ++at) {
-        const Segment seg = line.segments[at];
-        if (seg.units == 0) continue;
-        left -= seg.units;
+    SharedWalk shared(call, blockIdx.x);
+    OwnWalk own(call, blockIdx.x);
+    Segment seg;
+    while (shared.next(call, seg) || own.next(call, seg)) {
         const int *table = s.tables + (size_t)seg.slot * s.max_pages;
         __syncthreads();
         for (int i = tid; i < kRows * (D / 4); i += kThreads) {
@@ -173,7 +168,6 @@ __global__ void __launch_bounds__(kThreads) prefix_simt_kernel(const cq_kv_cache
 #pragma unroll
                     for (int i = 0; i < V; ++i) call.o[(int64_t)(seg.part + r0 + r) * D + V * lane + i] = o[r][i] + mine[r * D + i];
         if (tid < seg.rows) call.ml[seg.part + tid] = make_float2(sm.m[tid], sm.l[tid]);
-    }
     }
 }
 

@@ -212,7 +212,7 @@ class AttentionPlan:
         self._c = capi.PrefixPlan(batch=batch, queries=queries, heads=heads, groups=len(groups))
         self._p = C.byref(self._c)
         sizes = np.array(groups, dtype=np.int32)
-        shapes = np.zeros(3 * (len(groups) + 1), dtype=np.int32)
+        shapes = np.zeros(4 * len(groups), dtype=np.int32)
         with capi.on_device(cache.device):
             if capi.lib().cq_prefix_plan_shape(cache._p, self._p, sizes.ctypes.data, shapes.ctypes.data):
                 capi.check("attention_plan")

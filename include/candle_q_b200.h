@@ -456,9 +456,9 @@ int cq_kv_take_fault(const cq_kv_cache *cache, void *stream);
  * zeros), query heads in groups of heads / kv_heads per KV head.  The batch is cut into `groups` runs of neighbouring sequences; the pages that all
  * sequences of a run have in common at their start are found on the device, by comparing the tables.
  *   cq_prefix_plan_shape  : fills ctas, shared_items, n_ints, n_floats of a plan whose batch, queries, heads and groups are set, and `shapes`
- *                           (host, 3 * (groups + 1) ints, or null).  group_sizes: host, sequences per group, null for one group or groups of one.  Host
+ *                           (host, 4 * groups ints, or null).  group_sizes: host, sequences per group, null for one group or groups of one.  Host
  *                           only; 0 or, with the status set, 1.  The caller then gives the plan `ints` (device, n_ints) and `scratch` (device, n_floats),
- *                           32-byte aligned, and copies `shapes` to ints + 16.
+ *                           64-byte aligned, and copies `shapes` to ints + 16.
  *   cq_prefix_plan_update : the plan for the slots' lengths and tables as they are when it runs; once a step, for all layers.
  *   cq_prefix_attention   : one layer.  q: batch * queries rows of q_stride elements of the cache's type, heads side by side, 16-byte aligned;
  *                           out: [batch, queries, heads, head_dim] of that type.  Scores, sums and the join in f32; 16-bit types: the weights are
