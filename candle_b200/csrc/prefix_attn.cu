@@ -9,7 +9,7 @@ namespace {
 using namespace cq_attn;
 using cq_kv::State;
 
-constexpr int kThreads = 1024, kPlanCtas = 8;
+constexpr int kThreads = 256, kPlanCtas = 8;
 constexpr int kOwnLeast = 1;            // units of an own segment, at least
 
 // Sum of `v` over the threads before this one, two counts in one 64-bit word; `total` over all.
@@ -24,15 +24,14 @@ __device__ __forceinline__ uint64_t scan_before(uint64_t v, uint64_t *sums, uint
     __syncthreads();
     if (lane == 31) sums[warp] = x;
     __syncthreads();
-    uint64_t w = sums[lane];
+    uint64_t before = 0;
+    total = 0;
 #pragma unroll
-    for (int m = 1; m < 32; m <<= 1) {
-        const uint64_t y = __shfl_up_sync(0xffffffffu, w, m);
-        if (lane >= m) w += y;
+    for (int w = 0; w < kThreads / 32; ++w) {
+        if (w == warp) before = total;
+        total += sums[w];
     }
-    total = __shfl_sync(0xffffffffu, w, 31);
-    const uint64_t before = __shfl_sync(0xffffffffu, w, (warp + 31) & 31);
-    return x - v + (warp ? before : 0);
+    return before + x - v;
 }
 // Index of the last entry of an ascending column that is not above `v`.
 template <typename F> __device__ __forceinline__ int last_not_above(int n, int v, F column) {
@@ -45,13 +44,17 @@ template <typename F> __device__ __forceinline__ int last_not_above(int n, int v
     return lo;
 }
 
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+
 // One cluster.  The pages that a group shares are found by comparing the tables, so a plan cannot be wrong about them: the leading
 // entries that agree in all its sequences, as far as the shortest context among its queries fills pages.
-// Bound by latency - slots, lengths and tables are three reads that depend on one another, and a kernel of one CTA meets its instructions for
-// the first time as well - so the comparison and the workers' records are divided over kPlanCtas CTAs, and all else every CTA does for itself.
+// Bound by latency: slots, lengths and tables are three reads that depend on one another, and a warp by itself takes some five clocks an instruction.
+// So the comparison and the records are divided over the CTAs, everything else each does for itself, and divisions are kept out of the way (one CTA of 1024 threads
+// took 16 - 33 us for 64 - 128 sequences).
 __global__ void __launch_bounds__(kThreads) prefix_plan_kernel(const cq_kv_cache cache, const Call call, const int *__restrict__ slots) {
     extern __shared__ int dyn[];
-    __shared__ uint64_t sums[32];
+    __shared__ uint64_t sums[kThreads / 32];
     __shared__ int most;
     const State s = cq_kv::state_of(cache);
     const Shape &sh = call.sh;
@@ -61,10 +64,11 @@ __global__ void __launch_bounds__(kThreads) prefix_plan_kernel(const cq_kv_cache
     int *slot_of = dyn, *len_of = slot_of + sh.batch, *group_of = len_of + sh.batch;         // by sequence
     int *first_of = group_of + sh.batch, *count_of = first_of + sh.groups, *least_of = count_of + sh.groups;      // by group: of its sequences that
                                                                     // have a context for each query: the first, how many, pages that agree
-    int *shared_of = least_of + sh.groups, *group_start = shared_of + sh.groups;            // shared positions, first unit
-    int *start_of = group_start + sh.groups, *units_of = start_of + nq;                     // by query
+    int *group_start = least_of + sh.groups, *start_of = group_start + sh.groups, *units_of = start_of + nq;      // first units; by query
     for (int g = tid; g < sh.groups; g += kThreads) { first_of[g] = INT32_MAX; count_of[g] = 0; least_of[g] = INT32_MAX; }
     if (tid == 0) most = 0;
+    __syncwarp();
+    cluster_arrive();                       // the others may write this CTA's least_of
     cq_pdl_launch_dependents();
     cq_pdl_wait();
     __syncthreads();
@@ -85,56 +89,48 @@ __global__ void __launch_bounds__(kThreads) prefix_plan_kernel(const cq_kv_cache
         }
     }
     __syncthreads();
+    cluster_wait();
     // a warp compares 128 entries of a sequence with those of its group's first one
-    const int blocks = (most + 127) >> 7;
+    for (int j0 = 0; j0 < most; j0 += 128)
 #pragma unroll 1
-    for (int u = rank * (kThreads / 32) + warp; u < sh.batch * blocks; u += kPlanCtas * (kThreads / 32)) {
-        const int b = u / blocks, j0 = u % blocks * 128 + lane, g = group_of[b];
-        if (len_of[b] < t || count_of[g] < 2 || b == first_of[g]) continue;         // the whole warp
-        const int n = (len_of[b] - t + 1) >> shift;
-        const int *mine = s.tables + (size_t)slot_of[b] * s.max_pages, *first = s.tables + (size_t)slot_of[first_of[g]] * s.max_pages;
-        int p[4], f[4], bad = INT32_MAX;
+        for (int b = rank * (kThreads / 32) + warp; b < sh.batch; b += kPlanCtas * (kThreads / 32)) {
+            const int g = group_of[b], n = (len_of[b] - t + 1) >> shift, from = first_of[g];
+            if (len_of[b] < t || b == from || j0 >= n) continue;        // the whole warp
+            const int *mine = s.tables + (size_t)slot_of[b] * s.max_pages + j0 + lane, *first = s.tables + (size_t)slot_of[from] * s.max_pages + j0 + lane;
+            int p[4], f[4], bad = INT32_MAX;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const bool in = j0 + 32 * i < n;
-            p[i] = in ? mine[j0 + 32 * i] : 0;
-            f[i] = in ? first[j0 + 32 * i] : 0;
+            for (int i = 0; i < 4; ++i) {
+                const bool in = j0 + 32 * i + lane < n;
+                p[i] = in ? mine[32 * i] : 0;
+                f[i] = in ? first[32 * i] : 0;
+            }
+#pragma unroll
+            for (int i = 3; i >= 0; --i)
+                if (p[i] != f[i] || (unsigned)p[i] >= (unsigned)s.pages) bad = j0 + 32 * i + lane;
+            bad = __reduce_min_sync(0xffffffffu, bad);
+            if (bad != INT32_MAX && lane < kPlanCtas) {
+                uint32_t at;
+                asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(cq_smem_u32(&least_of[g])), "r"(lane));
+                asm volatile("red.relaxed.cluster.shared::cluster.min.s32 [%0], %1;" ::"r"(at), "r"(bad) : "memory");
+            }
         }
-#pragma unroll
-        for (int i = 3; i >= 0; --i)
-            if (p[i] != f[i] || p[i] < 0 || p[i] >= s.pages) bad = j0 + 32 * i;
-        bad = __reduce_min_sync(0xffffffffu, bad);
-        if (lane == 0 && bad != INT32_MAX) atomicMin(&least_of[g], bad);
-    }
     __syncwarp();
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-    for (int g = tid; g < sh.groups; g += kThreads) {
-        int least = INT32_MAX;
-#pragma unroll
-        for (int r = 0; r < kPlanCtas; ++r) {
-            uint32_t at;
-            int v;
-            asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(cq_smem_u32(&least_of[g])), "r"(r));
-            asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
-            least = min(least, v);
-        }
-        shared_of[g] = count_of[g] >= 2 ? least << shift : 0;
-    }
-    __syncwarp();
-    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");         // the others' shared memory has been read
-    __syncthreads();
+    cluster_arrive();
+    cluster_wait();
+    auto shared_of = [&](int g) { return count_of[g] >= 2 ? least_of[g] << shift : 0; };       // positions
     // both lines at once: the units of group i, and of query i
     uint64_t before = 0;
+#pragma unroll 1
     for (int i0 = 0; i0 < max(nq, sh.groups); i0 += kThreads) {
         const int i = i0 + tid;
         int n_shared = 0, units = 0;
-        if (i < sh.groups) n_shared = ((shared_of[i] + kKeyTile - 1) / kKeyTile) * hkv * pl.shapes[i].row_tiles;
+        if (i < sh.groups) n_shared = ((shared_of(i) + kKeyTile - 1) / kKeyTile) * hkv * pl.shapes[i].row_tiles;
         if (i < nq) {
-            const int b = i / t, len = len_of[b], shared = len >= t ? shared_of[group_of[b]] : 0, n = len - t + 1 + i % t;
-            units = n > shared ? (n - shared + sh.own_step - 1) / sh.own_step : 0;
+            const int b = t == 1 ? i : i / t, len = len_of[b], shared = len >= t ? shared_of(group_of[b]) : 0, n = len - t + 1 + (i - b * t);
+            units = n > shared ? (n - shared + (1 << sh.own_shift) - 1) >> sh.own_shift : 0;
         }
         uint64_t all;
-        const uint64_t at = before + scan_before((uint64_t)n_shared << 32 | (unsigned)(units * hkv * sh.own_tiles()), sums, all);
+        const uint64_t at = before + scan_before((uint64_t)n_shared << 32 | (unsigned)(units * hkv * sh.own_tiles), sums, all);
         if (i < sh.groups) group_start[i] = (int)(at >> 32);
         if (i < nq) { start_of[i] = (int)(uint32_t)at; units_of[i] = units; }
         before += all;
@@ -142,64 +138,63 @@ __global__ void __launch_bounds__(kThreads) prefix_plan_kernel(const cq_kv_cache
     __syncthreads();
     const int shared_line = (int)(before >> 32), own_line = (int)(uint32_t)before;
     const int chunk = max((shared_line + sh.ctas - 1) / sh.ctas, 1), own_chunk = max((own_line + sh.own_workers - 1) / sh.own_workers, kOwnLeast);
-    if (rank == 0 && tid == 0) { pl.header[0] = shared_line; pl.header[1] = chunk; pl.header[2] = own_line; pl.header[3] = own_chunk; }
     auto group_at = [&](int g) {
         const GroupShape gs = pl.shapes[g];
-        return Group{(shared_of[g] + kKeyTile - 1) / kKeyTile, shared_of[g], count_of[g] ? slot_of[first_of[g]] : -1, group_start[g], gs.query0, gs.rows, gs.item0, gs.row_tiles};
+        const int shared = shared_of(g);
+        return Group{(shared + kKeyTile - 1) / kKeyTile, shared, count_of[g] ? slot_of[first_of[g]] : -1, group_start[g], gs.query0, gs.rows, gs.item0, gs.row_tiles};
     };
-    const int id = rank * kThreads + tid, all = kPlanCtas * kThreads;
+    // records, dealt out one a CTA: of the workers, the queries, the groups
+    const int workers = sh.ctas + sh.own_workers;
 #pragma unroll 1
-    for (int i = id; i < sh.groups; i += all) pl.groups[i] = group_at(i);
-#pragma unroll 1
-    for (int i = id; i < nq; i += all) {
-        const int b = i / t, len = len_of[b];
-        Query q{};
-        q.len = len - t + 1 + i % t;
-        q.slot = slot_of[b];
-        q.units = units_of[i];
-        q.start = start_of[i];
-        if (len >= t && shared_of[group_of[b]]) {
-            const Group g = group_at(group_of[b]);
-            q.shared = g.shared;
-            q.group_start = g.start; q.group_units = g.units; q.query0 = g.query0; q.item0 = g.item0; q.row_tiles = g.row_tiles;
-        }
-        pl.query[i] = q;
-    }
-#pragma unroll 1
-    for (int w = id; w < sh.ctas + sh.own_workers; w += all) {
-        const bool own = w >= sh.ctas;
-        Start st{};
-        if (!own) {
-            const int u = w * chunk;
-            st.left = min(shared_line - u, chunk);
+    for (int i = tid * kPlanCtas + rank; i < workers + nq + sh.groups; i += kPlanCtas * kThreads) {
+        if (i < workers) {
+            const bool own = i >= sh.ctas;
+            const int w = own ? i - sh.ctas : i, u = w * (own ? own_chunk : chunk);
+            Start st{};
+            st.left = own ? min(own_line - u, own_chunk) : min(shared_line - u, chunk);
             if (st.left > 0) {
-                // the last group that begins here or before; those without units begin where the next one does
-                st.index = last_not_above(sh.groups, u, [&](int x) { return group_start[x]; });
-                const Group g = group_at(st.index);
-                st.local = (u - g.start) / g.units;
-                st.unit = (u - g.start) % g.units;
-                const int c[8] = {g.units, g.shared, g.slot, g.start, g.query0, g.rows, g.item0, g.row_tiles};
-#pragma unroll
-                for (int i = 0; i < 8; ++i) st.copy[i] = c[i];
+                // the last group (query) that begins here or before; those without units begin where the next one does
+                const int *starts = own ? start_of : group_start;
+                const int x = last_not_above(own ? nq : sh.groups, u, [&](int y) { return starts[y]; });
+                int units, tiles;
+                st.index = x;
+                if (own) {
+                    const int b = t == 1 ? x : x / t, len = len_of[b];
+                    units = units_of[x];
+                    tiles = sh.own_tiles;
+                    st.copy[0] = len - t + 1 + (x - b * t);
+                    st.copy[1] = slot_of[b];
+                    st.copy[2] = len >= t ? shared_of(group_of[b]) : 0;
+                    st.copy[3] = units;
+                } else {
+                    const Group g = group_at(x);
+                    units = g.units;
+                    tiles = g.row_tiles;
+                    st.copy[0] = g.units; st.copy[1] = g.shared; st.copy[2] = g.slot; st.copy[3] = g.start;
+                    st.copy[4] = g.query0; st.copy[5] = g.rows; st.copy[6] = g.item0; st.copy[7] = g.row_tiles;
+                }
+                const int local = (u - starts[x]) / units;
+                st.unit = u - starts[x] - local * units;
+                st.head = tiles == 1 ? local : local / tiles;
+                st.tile = local - st.head * tiles;
             }
-        } else {
-            const int u = (w - sh.ctas) * own_chunk;
-            st.left = min(own_line - u, own_chunk);
-            if (st.left > 0) {
-                st.index = last_not_above(nq, u, [&](int x) { return start_of[x]; });
-                const int b = st.index / t, len = len_of[b], units = units_of[st.index];
-                st.local = (u - start_of[st.index]) / units;
-                st.unit = (u - start_of[st.index]) % units;
-                st.copy[0] = len - t + 1 + st.index % t;
-                st.copy[1] = slot_of[b];
-                st.copy[2] = len >= t ? shared_of[group_of[b]] : 0;
-                st.copy[3] = units;
+            (own ? pl.own : pl.shared)[w] = st;
+        } else if (i < workers + nq) {
+            const int x = i - workers, b = t == 1 ? x : x / t, len = len_of[b];
+            Query q{};
+            q.len = len - t + 1 + (x - b * t);
+            q.slot = slot_of[b];
+            q.units = units_of[x];
+            q.start = start_of[x];
+            if (len >= t && shared_of(group_of[b])) {
+                const Group g = group_at(group_of[b]);
+                q.shared = g.shared;
+                q.group_start = g.start; q.group_units = g.units; q.query0 = g.query0; q.item0 = g.item0; q.row_tiles = g.row_tiles;
             }
-        }
-        (own ? pl.own - sh.ctas : pl.shared)[w] = st;
+            pl.query[x] = q;
+        } else pl.groups[i - workers - nq] = group_at(i - workers - nq);
     }
-    __syncwarp();
-    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    if (rank == 0 && tid == 0) { pl.header[0] = shared_line; pl.header[1] = chunk; pl.header[2] = own_line; pl.header[3] = own_chunk; }
 }
 
 // One warp per row: lane x weighs segment x - those of the row's shared item, then those of its own one, in the order of their keys - and the
@@ -209,18 +204,18 @@ template <typename T, int D> __global__ void __launch_bounds__(256) prefix_join_
     const Plan &pl = call.plan;
     cq_pdl_launch_dependents();
     cq_pdl_wait();
-    const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-    const int lane = threadIdx.x & 31, per = sh.per_kv();
-    if (row >= (int64_t)sh.n_queries() * sh.heads) return;
-    const int n = (int)(row / sh.heads), hq = (int)(row % sh.heads), h = hq / per, in = hq % per;
+    const int lane = threadIdx.x & 31, per = sh.per_kv, n = blockIdx.y, hq = blockIdx.x * 8 + (threadIdx.x >> 5);
+    if (hq >= sh.heads) return;
+    const int h = div_per(hq, sh), in = hq - h * per, tile = in / sh.own_rows;          // own_rows: 16 or 32
+    const int64_t row = (int64_t)n * sh.heads + hq;
     const Query q = pl.query[n];
     const int chunk = pl.header[1], own_chunk = pl.header[3];
     constexpr int V = D / 32;
     float acc[V] = {}, m = -INFINITY, l = 0.0f;
     if (q.len > 0) {
         // segments of an item: its units [start, start + units) of the line, cut at multiples of the chunk
-        const int own_item = (n * sh.kv_heads + h) * sh.own_tiles() + in / sh.own_rows;
-        const int own_start = q.start + (h * sh.own_tiles() + in / sh.own_rows) * q.units, own_w = own_start / own_chunk;
+        const int local = h * sh.own_tiles + tile, own_item = n * sh.kv_heads * sh.own_tiles + local;
+        const int own_start = q.start + local * q.units, own_w = own_start / own_chunk;
         const int n_own = q.units ? (own_start + q.units - 1) / own_chunk - own_w + 1 : 0;
         int n_shared = 0;
         int64_t shared0 = 0;
@@ -230,7 +225,7 @@ template <typename T, int D> __global__ void __launch_bounds__(256) prefix_join_
             shared0 = part_shared(sh, q.item0 + local + w) + r % sh.row_tile;
         }
         const int n_all = n_shared + n_own;
-        const int64_t own0 = part_own(sh, call.shared_items, own_item + own_w) + in % sh.own_rows;
+        const int64_t own0 = part_own(sh, call.shared_items, own_item + own_w) + in - tile * sh.own_rows;
         for (int x0 = 0; x0 < n_all; x0 += 32) {
             const int x = x0 + lane, count = min(32, n_all - x0);
             const int part = (int)(x < n_shared ? shared0 + (int64_t)x * sh.row_tile : own0 + (int64_t)(x - n_shared) * sh.own_slot());
@@ -270,7 +265,7 @@ template <typename T, int D> __global__ void __launch_bounds__(256) prefix_join_
 }
 
 template <int D> void join_launch(const Call &c, void *out, cudaStream_t st) {
-    const dim3 grid((unsigned)(((int64_t)c.sh.n_queries() * c.sh.heads + 7) / 8));
+    const dim3 grid((unsigned)((c.sh.heads + 7) / 8), (unsigned)c.sh.n_queries());
     if (c.sh.elem == CQ_F32) cq_launch_k(prefix_join_kernel<float, D>, grid, dim3(256), 0, st, c, (float *)out);
     else if (c.sh.elem == CQ_F16) cq_launch_k(prefix_join_kernel<__half, D>, grid, dim3(256), 0, st, c, (__half *)out);
     else cq_launch_k(prefix_join_kernel<__nv_bfloat16, D>, grid, dim3(256), 0, st, c, (__nv_bfloat16 *)out);
@@ -296,10 +291,12 @@ bool shape_ok(const cq_kv_cache *cache, const cq_prefix_plan *p, const char *who
         cq_set_status(status, msg);
         return false;
     }
-    s = Shape{p->batch, p->queries, p->heads, cache->kv_heads, p->groups, cache->head_dim, cache->elem, 0, p->ctas, 0, 0, 0, 0};
-    if (s.per_kv() > 1) s.rcp = (unsigned)(((1ull << 32) + s.per_kv() - 1) / s.per_kv());
-    if (cache->elem == CQ_F32) { s.row_tile = s.own_rows = 32; s.own_step = 64; s.own_workers = s.ctas; }
-    else { s.row_tile = 128; s.own_rows = 16; s.own_step = 16; s.own_workers = s.ctas * kMmaWarps; }
+    s = Shape{p->batch, p->queries, p->heads, cache->kv_heads, p->groups, cache->head_dim, cache->elem, p->heads / cache->kv_heads};
+    s.ctas = p->ctas;
+    if (cache->elem == CQ_F32) { s.row_tile = s.own_rows = 32; s.own_shift = 6; s.own_workers = s.ctas; }
+    else { s.row_tile = 128; s.own_rows = 16; s.own_shift = 4; s.own_workers = s.ctas * kMmaWarps; }
+    s.own_tiles = (s.per_kv + s.own_rows - 1) / s.own_rows;
+    if (s.per_kv > 1) s.rcp = (unsigned)(((1ull << 32) + s.per_kv - 1) / s.per_kv);
     return true;
 }
 Call call_of(const cq_prefix_plan *p, const Shape &s) {
@@ -333,10 +330,10 @@ extern "C" int cq_prefix_plan_shape(const cq_kv_cache *cache, cq_prefix_plan *pl
     for (int g = 0; g < plan->groups; ++g) {
         const int n = group_sizes ? group_sizes[g] : plan->groups == 1 ? plan->batch : 1;
         if (n <= 0) { cq_set_status(CQ_ERR_BAD_ARG, "prefix_plan_shape: a group without sequences"); return 1; }
-        const int64_t tiles = ((int64_t)n * s.queries * s.per_kv() + s.row_tile - 1) / s.row_tile;
+        const int64_t tiles = ((int64_t)n * s.queries * s.per_kv + s.row_tile - 1) / s.row_tile;
         if (shapes) {
             int *to = shapes + 4 * g;
-            to[0] = (int)(seqs * s.queries); to[1] = n * s.queries * s.per_kv(); to[2] = (int)items; to[3] = (int)tiles;
+            to[0] = (int)(seqs * s.queries); to[1] = n * s.queries * s.per_kv; to[2] = (int)items; to[3] = (int)tiles;
         }
         items += tiles * s.kv_heads;
         seqs += n;
@@ -352,7 +349,7 @@ extern "C" void cq_prefix_plan_update(const cq_kv_cache *cache, const cq_prefix_
     Shape s;
     if (!shape_ok(cache, plan, "prefix_plan_update", s) || !plan_ready(plan, s, "prefix_plan_update")) return;
     if (!slots) { cq_set_status(CQ_ERR_BAD_ARG, "prefix_plan_update: null slots"); return; }
-    const size_t smem = 4 * (3 * (size_t)s.batch + 5 * (size_t)s.groups + 2 * (size_t)s.n_queries());
+    const size_t smem = 4 * (3 * (size_t)s.batch + 4 * (size_t)s.groups + 2 * (size_t)s.n_queries());
     if (smem > 47 * 1024) cudaFuncSetAttribute(prefix_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     cq_launch_cluster_k(prefix_plan_kernel, dim3(kPlanCtas), dim3(kThreads), smem, (cudaStream_t)stream, kPlanCtas, *cache, call_of(plan, s), slots);
     cq_check_launch("prefix_plan_update");

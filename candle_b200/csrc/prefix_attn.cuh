@@ -4,7 +4,7 @@
 // rows of consecutive sequences are consecutive.  Two kinds of items cover all (row, key) pairs:
 //   shared : up to `row_tile` rows of one group of sequences x one KV head x the keys of the pages that all of them share;
 //   own    : up to `own_rows` rows of one query x one KV head x the keys behind these pages.
-// An item is a number of units (64 keys of a shared item, `own_step` keys of an own one); the units of all items of a kind form a line, which
+// An item is a number of units (64 keys of a shared item, 2^own_shift keys of an own one); the units of all items of a kind form a line, which
 // its workers (CTAs for the shared items; CTAs or warps for the own ones) take in equal parts.  A part of an item that one worker takes
 // is a segment; it leaves (maximum, sum, unnormalised output) per row, and a second kernel joins a row's segments in the order of their keys:
 // m = max m_i,  l = sum 2^(m_i - m) l_i,  o = sum 2^(m_i - m) o_i / l.
@@ -32,19 +32,18 @@ struct Query {              // 64 bytes
     int start, group_start, group_units, query0;
     int item0, row_tiles, pad[6];
 };
-// Where a worker begins: the group (query), the item in it (head, then row tile), the unit in that, and how many units the worker has.
-struct Start { int index, local, unit, left, copy[8]; int pad[4]; };        // 64 bytes; copy: the Group, or the first half of the Query
+// Where a worker begins: the group (query), head and row tile of its first item, the unit in that, and how many units the worker has.
+struct Start { int index, head, tile, unit, left, pad[3], copy[8]; };       // 64 bytes; copy: the Group, or the first half of the Query
 struct GroupShape { int query0, rows, item0, row_tiles; };
 
 struct Shape {
-    int batch, queries, heads, kv_heads, groups, head_dim, elem;
-    int row_tile, ctas, own_rows, own_step, own_workers;
+    int batch, queries, heads, kv_heads, groups, head_dim, elem, per_kv;
+    int row_tile, ctas, own_rows, own_shift, own_workers;       // 2^own_shift keys an own unit
+    int own_tiles;          // row tiles of a KV head's query heads
     unsigned rcp;           // ceil(2^32 / query heads per KV head); 0 for one
-    __host__ __device__ int per_kv() const { return heads / kv_heads; }
     __host__ __device__ int n_queries() const { return batch * queries; }
-    __host__ __device__ int own_tiles() const { return (per_kv() + own_rows - 1) / own_rows; }
-    __host__ __device__ int own_slot() const { return per_kv() < own_rows ? per_kv() : own_rows; }      // rows of a partial result
-    __host__ __device__ int own_items() const { return n_queries() * kv_heads * own_tiles(); }          // query, then head, then row tile
+    __host__ __device__ int own_slot() const { return per_kv < own_rows ? per_kv : own_rows; }      // rows of a partial result
+    __host__ __device__ int own_items() const { return n_queries() * kv_heads * own_tiles; }        // query, then head, then row tile
 };
 
 // The plan's ints.
@@ -92,68 +91,73 @@ __host__ __device__ inline int64_t part_own(const Shape &s, int shared_items, in
 
 // The segments of a worker, one after the other.
 struct SharedWalk {
-    int group, local, unit, left, cta;
+    int group, head, tile, unit, left, cta;
     Group g;
+    __device__ __forceinline__ void take(const int4 &b, const int4 &d) { g = Group{b.x, b.y, b.z, b.w, d.x, d.y, d.z, d.w}; }
     __device__ __forceinline__ SharedWalk(const Call &c, int cta) : cta(cta) {
         const int4 *p = reinterpret_cast<const int4 *>(c.plan.shared + cta);
-        const int4 a = p[0], b = p[1], d = p[2];
-        group = a.x; local = a.y; unit = a.z; left = a.w;
-        g = Group{b.x, b.y, b.z, b.w, d.x, d.y, d.z, d.w};
+        const int4 a = p[0];
+        left = p[1].x;
+        group = a.x; head = a.y; tile = a.z; unit = a.w;
+        take(p[2], p[3]);
     }
     __device__ __forceinline__ bool next(const Call &c, Segment &s) {
         if (left <= 0) return false;
         const Shape &sh = c.sh;
-        while (g.units == 0 || local == sh.kv_heads * g.row_tiles) {
+        while (g.units == 0 || head == sh.kv_heads) {
             const int4 *p = reinterpret_cast<const int4 *>(c.plan.groups + ++group);
-            const int4 b = p[0], d = p[1];
-            g = Group{b.x, b.y, b.z, b.w, d.x, d.y, d.z, d.w};
-            local = 0;
+            take(p[0], p[1]);
+            head = 0;
         }
-        const int tile = local % g.row_tiles;
-        s.head = local / g.row_tiles;
-        s.row0 = g.query0 * sh.per_kv() + tile * sh.row_tile;
+        s.head = head;
+        s.row0 = g.query0 * sh.per_kv + tile * sh.row_tile;
         s.rows = min(sh.row_tile, g.rows - tile * sh.row_tile);
         s.slot = g.slot;
         s.units = min(left, g.units - unit);
         s.key0 = unit * kKeyTile;
         s.key1 = min(g.shared, (unit + s.units) * kKeyTile);
-        s.part = (int)part_shared(sh, g.item0 + local + cta);
+        s.part = (int)part_shared(sh, g.item0 + head * g.row_tiles + tile + cta);
         left -= s.units;
         unit += s.units;
-        if (unit == g.units) { unit = 0; ++local; }
+        if (unit == g.units) {
+            unit = 0;
+            if (++tile == g.row_tiles) { tile = 0; ++head; }
+        }
         return true;
     }
 };
 struct OwnWalk {
-    int query, local, unit, left, worker;
+    int query, head, tile, unit, left, worker;
     int len, slot, shared, units;
     __device__ __forceinline__ OwnWalk(const Call &c, int worker) : worker(worker) {
         const int4 *p = reinterpret_cast<const int4 *>(c.plan.own + worker);
-        const int4 a = p[0], b = p[1];
-        query = a.x; local = a.y; unit = a.z; left = a.w;
+        const int4 a = p[0], b = p[2];
+        left = p[1].x;
+        query = a.x; head = a.y; tile = a.z; unit = a.w;
         len = b.x; slot = b.y; shared = b.z; units = b.w;
     }
     __device__ __forceinline__ bool next(const Call &c, Segment &s) {
         if (left <= 0) return false;
         const Shape &sh = c.sh;
-        const int tiles = sh.own_tiles(), per = sh.per_kv();
-        while (units == 0 || local == sh.kv_heads * tiles) {
+        while (units == 0 || head == sh.kv_heads) {
             const int4 b = *reinterpret_cast<const int4 *>(c.plan.query + ++query);
             len = b.x; slot = b.y; shared = b.z; units = b.w;
-            local = 0;
+            head = 0;
         }
-        const int tile = tiles == 1 ? 0 : local % tiles;
-        s.head = tiles == 1 ? local : local / tiles;
-        s.row0 = query * per + tile * sh.own_rows;
-        s.rows = min(sh.own_rows, per - tile * sh.own_rows);
+        s.head = head;
+        s.row0 = query * sh.per_kv + tile * sh.own_rows;
+        s.rows = min(sh.own_rows, sh.per_kv - tile * sh.own_rows);
         s.slot = slot;
         s.units = min(left, units - unit);
-        s.key0 = shared + unit * sh.own_step;
-        s.key1 = min(len, s.key0 + s.units * sh.own_step);
-        s.part = (int)part_own(sh, c.shared_items, query * sh.kv_heads * tiles + local + worker);
+        s.key0 = shared + (unit << sh.own_shift);
+        s.key1 = min(len, s.key0 + (s.units << sh.own_shift));
+        s.part = (int)part_own(sh, c.shared_items, (query * sh.kv_heads + head) * sh.own_tiles + tile + worker);
         left -= s.units;
         unit += s.units;
-        if (unit == units) { unit = 0; ++local; }
+        if (unit == units) {
+            unit = 0;
+            if (++tile == sh.own_tiles) { tile = 0; ++head; }
+        }
         return true;
     }
 };

@@ -104,7 +104,7 @@ __device__ bool shared_part(Tiles<D> &sm, const cq_kv_cache &cache, const cq_kv:
     bool ok = true;
     unsigned tile = 0;              // buffer tile & 1, phase tile / 2
     if (warp < 4) {
-        const int per = call.sh.per_kv(), row = warp * 32 + lane;
+        const int per = call.sh.per_kv, row = warp * 32 + lane;
         const uint32_t mine = tmem + ((uint32_t)(warp * 32) << 16);
         while (ok && walk.next(call, seg)) {
             // Q: all rows of the segment by the four warps; rows behind them keep what was there, and nobody reads their results
@@ -343,7 +343,7 @@ template <int D> struct Loader {
 template <int D, bool BF16>
 __device__ bool own_part(Tiles<D> &sm, const cq_kv_cache &cache, const cq_kv::State &st, const Call &call, const CUtensorMap &k_map, const CUtensorMap &v_map,
                          const uint8_t *__restrict__ q, int64_t q_stride, float c) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, x2 = (lane & 3) * 2, per = call.sh.per_kv();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, x2 = (lane & 3) * 2, per = call.sh.per_kv;
     const int worker = blockIdx.x * kMmaWarps + warp;
     Step<D> *steps = sm.step[warp];
     uint64_t *bars = sm.step_bar[warp];

@@ -76,7 +76,7 @@ __global__ void __launch_bounds__(kThreads) prefix_simt_kernel(const cq_kv_cache
     extern __shared__ __align__(16) uint8_t raw[];
     Smem<D> &sm = *reinterpret_cast<Smem<D> *>(raw);
     const cq_kv::State s = cq_kv::state_of(cache);
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, per = call.sh.per_kv();
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, per = call.sh.per_kv;
     cq_pdl_launch_dependents();
     cq_pdl_wait();
     const T *k_pool = reinterpret_cast<const T *>(cache.k), *v_pool = reinterpret_cast<const T *>(cache.v);
