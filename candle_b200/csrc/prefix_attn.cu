@@ -294,7 +294,7 @@ bool shape_ok(const cq_kv_cache *cache, const cq_prefix_plan *p, const char *who
     s = Shape{p->batch, p->queries, p->heads, cache->kv_heads, p->groups, cache->head_dim, cache->elem, p->heads / cache->kv_heads};
     s.ctas = p->ctas;
     if (cache->elem == CQ_F32) { s.row_tile = s.own_rows = 32; s.own_shift = 6; s.own_workers = s.ctas; }
-    else { s.row_tile = 128; s.own_rows = 16; s.own_shift = 4; s.own_workers = s.ctas * kMmaWarps; }
+    else { s.row_tile = 256; s.own_rows = 16; s.own_shift = 4; s.own_workers = s.ctas * kMmaWarps; }
     s.own_tiles = (s.per_kv + s.own_rows - 1) / s.own_rows;
     if (s.per_kv > 1) s.rcp = (unsigned)(((1ull << 32) + s.per_kv - 1) / s.per_kv);
     return true;
@@ -324,7 +324,7 @@ bool plan_ready(const cq_prefix_plan *p, const Shape &s, const char *who) {
 extern "C" int cq_prefix_plan_shape(const cq_kv_cache *cache, cq_prefix_plan *plan, const int *group_sizes, int *shapes) {
     Shape s;
     if (!shape_ok(cache, plan, "prefix_plan_shape", s)) return 1;
-    s.ctas = plan->ctas = 2 * cq_sm_count();
+    s.ctas = plan->ctas = (s.elem == CQ_F32 ? 2 : 1) * cq_sm_count();
     s.own_workers = s.elem == CQ_F32 ? s.ctas : s.ctas * kMmaWarps;
     int64_t items = 0, seqs = 0;
     for (int g = 0; g < plan->groups; ++g) {

@@ -167,6 +167,6 @@ __device__ __forceinline__ int div_per(int n, const Shape &s) { return s.rcp ? (
 // The kernels that make the segments' results (prefix_attn_simt.cu: f32; prefix_attn_mma.cu: f16 and bf16).
 void simt_launch(const Call &c, const cq_kv_cache &cache, int layer, const void *q, int64_t q_stride, float scale, cudaStream_t st);
 bool mma_launch(const Call &c, const cq_kv_cache &cache, int layer, const void *q, int64_t q_stride, float scale, cudaStream_t st);
-constexpr int kMmaWarps = 6;            // of a CTA of the latter: each is a worker of the own line
+constexpr int kMmaWarps = 4;            // warps of a CTA of the latter that are workers of the own line
 
 }  // namespace cq_attn

@@ -1,23 +1,19 @@
 // Segments of the shared-prefix attention (prefix_attn.cuh) on the tensor cores: f16 and bf16 caches.
 //
-// Shared items (many rows, keys mostly from L2): tiles of 128 rows x 64 keys by tcgen05.  S = Q K^T goes to tensor memory; thread r of the softmax
-// warps owns row r, reads it there, and writes the weights 2^(s c - m), c = scale log2 e, back over it in 16 bits as the first operand of O += P V.
-// Warps: 0-3 softmax (TMEM lanes 32 w ..), 4 copies, 5 MMA.  256 columns a CTA: the scores of two tiles, so that one tile's softmax has the products
-// of its neighbours beside it, and the outputs.  Two CTAs per SM.
+// Shared items (many rows, keys mostly from L2): tiles of 2 x 128 rows x 64 keys by tcgen05.  S = Q K^T goes to tensor memory; thread r of a
+// half's softmax warps owns row r, reads it there, and writes the weights 2^(s c - m), c = scale log2 e, back over it in 16 bits as the first operand of
+// O += P V.  512 columns: for each half the scores of two tiles, so that one tile's softmax has the products of its neighbours beside it, and the outputs.
 //
-// Own items (as many rows as a KV head has query heads, keys from HBM): a warp is a worker of its own, 16 rows x 16 keys a step by mma.sync, with two
-// steps of keys and values on their way.  Through the first form an item of four rows costs the waits of a whole tile chain - QK,
-// softmax, PV, some 10,000 clocks for 64 KB - where HBM gives an SM 64 KB in 2,850; here twelve warps of an SM have 190 KB in flight and
-// nothing to wait for but that.
+// Own items (as many rows as a KV head has query heads, keys from HBM): a warp is a worker of its own, 16 rows x 16 keys a step by mma.sync, with its
+// next steps of keys and values on their way.  Through the first form an item of four rows costs the waits of a whole tile chain - QK, softmax, PV, some
+// 10,000 clocks for 64 KB - where HBM gives an SM 64 KB in 2,850.  These warps run beside the others all the time, so that HBM and tensor cores are both in use.
 //
 // In both m is the row's maximum so far, kept until a score passes it by 2^8 (weights up to 256 are as good as any, the sum has the same
 // factor), so that outputs are scaled in the first tiles only.  The sum adds the weights as rounded: rounding moves weight between keys but
-// not the total.  Keys and values come by tiled TMA copies of 64 dims and a page (own items: 16 rows) at a time, 128-byte swizzle: K as it is
+// not the total.  Keys and values of shared items come by tiled TMA copies of 64 dims and a page at a time, 128-byte swizzle: K as it is
 // for the first product, V for the second with its rows as the K dimension.  Rows of a tile behind the last key hold whatever the page or the tile
 // before left there: their scores are masked, their values set to zero before the second product, since 0 x NaN is not 0.
 #include <cuda.h>
-
-#include <mutex>
 
 #include "prefix_attn.cuh"
 #include "prompt_f16.cuh"
@@ -26,21 +22,22 @@ namespace {
 using namespace cq_attn;
 using namespace cq_prompt;
 
-constexpr int kThreads = 32 * kMmaWarps, kStages = 2, kCols = 256, kHalfBytes = 128 * 128;       // 128 rows of 64 elements
-constexpr int kS = 0, kO = 128;                                      // columns of scores / weights (two tiles) and of outputs
+// Warps: 0-3 and 4-7 softmax of a row tile's halves, 8 copies, 9 products, 12-15 own items.
+constexpr int kThreads = 512, kCopyWarp = 8, kMmaWarp = 9, kOwnWarp = 12;
+constexpr int kKvStages = 3, kCols = 512;
+constexpr int kHalfBytes = 128 * 128;                        // 128 rows of 64 elements
+constexpr int kGroup = 256, kO = 128;                        // columns of a half; in it the scores / weights of two tiles and the outputs
+constexpr int kStep = 16;                                    // keys of a step of an own item
+// registers a thread by warpgroup: 128 * (144 + 144 + 64 + 160) is what the block was launched with, 512 * 128
+constexpr int kRegsSoft = 144, kRegsMisc = 64, kRegsOwn = 160;
 
-// operands there (q, k, v), scores there (and K free), weights there, outputs there (and V, weights free)
-struct Bars { uint64_t q, k[2], v[2], s[2], p[2], o[2]; };
-
-constexpr int kStep = 16;                // keys of a step of an own item
 template <int D> struct Step { uint8_t k[D / 64][kStep * 128], v[D / 64][kStep * 128]; };
 template <int D> struct Tiles {
-    union {
-        struct { uint8_t q[D / 64][kHalfBytes], k[2][D / 64][kKeyTile * 128], v[2][D / 64][kKeyTile * 128]; };
-        Step<D> step[kMmaWarps][kStages];
-    };
-    Bars bar;
-    uint64_t step_bar[kMmaWarps][kStages];
+    static constexpr int kStages = D == 64 ? 4 : 2;          // steps of an own warp: 64 KB for four of them
+    uint8_t q[2][D / 64][kHalfBytes], k[kKvStages][D / 64][kKeyTile * 128], v[kKvStages][D / 64][kKeyTile * 128];
+    Step<D> step[kMmaWarps][kStages];
+    // operands there; K, V free; by half and buffer: scores there, weights there, weights read and outputs there
+    uint64_t q_bar[2], k_bar[kKvStages], v_bar[kKvStages], k_free[kKvStages], v_free[kKvStages], s_bar[2][2], p_bar[2][2], o_bar[2][2];
     uint32_t tmem;
     int abort;
 };
@@ -89,200 +86,255 @@ template <bool BF16> __device__ __forceinline__ uint32_t pack(float a, float b, 
     return w;
 }
 
-// The CTA's share of the shared line.  False: a wait gave up.
-// The scores of two tiles have room, so QK of the next tile and PV of the one before run beside a tile's softmax; a barrier per buffer, since
-// no waiter may fall two phases behind.
+__device__ __forceinline__ void load_3d(uint32_t smem, const void *map, int x, int y, int z, uint32_t bar) {
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(smem), "l"(map), "r"(x), "r"(y), "r"(z),
+                 "r"(bar) : "memory");
+}
+__device__ __forceinline__ void expect_tx(uint32_t bar, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+
+// ---- shared items ----
+// Buffers are used in turn: use n of one of N goes to n % N, and waits for the phase that use n - N has completed.  Every barrier belongs to one buffer, so no
+// waiter can fall two phases behind.
+
+// Softmax of one half of the row tiles.  False: a wait gave up.
 template <int D, bool BF16>
-__device__ bool shared_part(Tiles<D> &sm, const cq_kv_cache &cache, const cq_kv::State &st, const Call &call, const CUtensorMap &k_map, const CUtensorMap &v_map,
-                            const uint8_t *__restrict__ q, int64_t q_stride, float c, uint32_t tmem) {
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, page = st.page;
-    constexpr uint32_t kIdescQK = (1u << 4) | (BF16 ? (1u << 7) | (1u << 10) : 0u) | ((uint32_t)kKeyTile >> 3) << 17 | (128u >> 4) << 24;
-    constexpr uint32_t kIdescPV = (1u << 4) | (BF16 ? (1u << 7) | (1u << 10) : 0u) | (1u << 16) | ((uint32_t)D >> 3) << 17 | (128u >> 4) << 24;
+__device__ bool softmax_part(Tiles<D> &sm, const Call &call, const CUtensorMap &o_map, const uint8_t *__restrict__ q, int64_t q_stride, float c, int half) {
+    const int tid = threadIdx.x & 127, lane = tid & 31, warp = tid >> 5, row = tid, per = call.sh.per_kv;
+    const uint32_t mine = sm.tmem + ((uint32_t)(warp * 32) << 16) + half * kGroup;
     volatile int *abort_flag = &sm.abort;
     SharedWalk walk(call, blockIdx.x);
     Segment seg;
-    bool ok = true;
-    unsigned tile = 0;              // buffer tile & 1, phase tile / 2
-    if (warp < 4) {
-        const int per = call.sh.per_kv, row = warp * 32 + lane;
-        const uint32_t mine = tmem + ((uint32_t)(warp * 32) << 16);
-        while (ok && walk.next(call, seg)) {
-            // Q: all rows of the segment by the four warps; rows behind them keep what was there, and nobody reads their results
-            const uint8_t *src = q + (int64_t)seg.head * per * D * 2;
-            for (int i = tid; i < seg.rows * (D / 8); i += 128) {
-                const int r = i / (D / 8), x = i % (D / 8), n = div_per(seg.row0 + r, call.sh), in = seg.row0 + r - n * per;
-                cq_cp_async16(&sm.q[x >> 3][r * 128 + ((x & 7) ^ (r & 7)) * 16], src + ((int64_t)n * q_stride + (int64_t)in * D + x * 8) * 2);
-            }
-            cq_cp_async_commit();
-            cq_cp_async_wait<0>();
-            fence_proxy_async_smem();
-            arrive_warp(&sm.bar.q, lane);
-            const bool active = warp * 32 < seg.rows;
-            float m = -INFINITY, l = 0.0f;
-            for (int j = 0; j < seg.units; ++j, ++tile) {
-                const int n = seg.key1 - seg.key0 - j * kKeyTile;          // keys of this tile, if fewer than kKeyTile
-                const unsigned b = tile & 1, phase = tile >> 1 & 1;
-                const uint32_t sp = mine + kS + b * kKeyTile;
-                if (!(ok = wait_warp(&sm.bar.s[b], phase, abort_flag))) break;
-                tc_fence_after();
-                if (active) {
-                    uint32_t s[2][32];
-                    tmem_ld32(sp, s[0]);
-                    tmem_ld32(sp + 32, s[1]);
-                    tmem_ld_wait();
-                    if (n < kKeyTile) {
-#pragma unroll
-                        for (int i = 0; i < kKeyTile; ++i)
-                            if (i >= n) s[i >> 5][i & 31] = 0xff800000u;        // -inf
-                    }
-                    float mx = -INFINITY, my = -INFINITY;
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) { mx = fmaxf(mx, __uint_as_float(s[0][i])); my = fmaxf(my, __uint_as_float(s[1][i])); }
-                    mx = fmaxf(mx, my) * c;
-                    if (j == 0) m = mx;
-                    else {
-                        const bool up = mx > m + 8.0f;          // from -inf as well
-                        if (__any_sync(0xffffffffu, up)) {
-                            const float f = up ? ex2(m - mx) : 1.0f;
-                            if (up) m = mx;
-                            l *= f;
-                            if (!(ok = wait_warp(&sm.bar.o[b ^ 1], (tile - 1) >> 1 & 1, abort_flag))) break;        // the outputs so far
-                            tc_fence_after();
-#pragma unroll
-                            for (int x = 0; x < D / 16; ++x) {
-                                uint32_t o[16];
-                                tmem_ld16(mine + kO + 16 * x, o);
-                                tmem_ld_wait();
-#pragma unroll
-                                for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-                                tmem_st16(mine + kO + 16 * x, o);
-                            }
-                        }
-                    }
-                    const float base = m == -INFINITY ? 0.0f : m;
-                    float sum0 = 0.0f, sum1 = 0.0f;
-#pragma unroll
-                    for (int x = 0; x < 2; ++x) {
-                        uint32_t w[16];
-#pragma unroll
-                        for (int i = 0; i < 16; ++i)
-                            w[i] = pack<BF16>(ex2(__fmaf_rn(__uint_as_float(s[x][2 * i]), c, -base)), ex2(__fmaf_rn(__uint_as_float(s[x][2 * i + 1]), c, -base)),
-                                              i & 1 ? sum1 : sum0);
-                        tmem_st16(sp + 16 * x, w);              // over the scores
-                    }
-                    l += sum0 + sum1;
-                    tmem_st_wait();
-                    tc_fence_before();
-                }
-                if (n < kKeyTile) {
-                    if (!(ok = wait_warp(&sm.bar.v[b], phase, abort_flag))) break;
-                    for (int i = tid; i < (kKeyTile - n) * (D / 8); i += 128) {
-                        const int r = n + i / (D / 8), x = i % (D / 8);
-                        *reinterpret_cast<uint4 *>(&sm.v[b][x >> 3][r * 128 + (x & 7) * 16]) = make_uint4(0, 0, 0, 0);
-                    }
-                    fence_proxy_async_smem();
-                }
-                arrive_warp(&sm.bar.p[b], lane);
-            }
-            if (!ok || !(ok = wait_warp(&sm.bar.o[(tile - 1) & 1], (tile - 1) >> 1 & 1, abort_flag))) break;
+    unsigned tile = 0;                      // of this half
+    while (walk.next(call, seg)) {
+        const int rows = min(seg.rows - half * 128, 128), row0 = seg.row0 + half * 128;
+        if (rows <= 0) continue;
+        // Q: rows behind the last keep what was there, and nobody reads their results
+        const uint8_t *src = q + (int64_t)seg.head * per * D * 2;
+        for (int i = tid; i < rows * (D / 8); i += 128) {
+            const int r = i / (D / 8), x = i % (D / 8), n = div_per(row0 + r, call.sh), in = row0 + r - n * per;
+            cq_cp_async16(&sm.q[half][x >> 3][r * 128 + ((x & 7) ^ (r & 7)) * 16], src + ((int64_t)n * q_stride + (int64_t)in * D + x * 8) * 2);
+        }
+        cq_cp_async_commit();
+        cq_cp_async_wait<0>();
+        fence_proxy_async_smem();
+        arrive_warp(&sm.q_bar[half], lane);
+        const bool active = warp * 32 < rows;
+        float m = -INFINITY, l = 0.0f;
+        for (int j = 0; j < seg.units; ++j, ++tile) {
+            const int n = seg.key1 - seg.key0 - j * kKeyTile;          // keys of this tile, if fewer than kKeyTile
+            const unsigned b = tile & 1, phase = tile >> 1 & 1;
+            const uint32_t sp = mine + b * kKeyTile;
+            if (!wait_warp(&sm.s_bar[half][b], phase, abort_flag)) return false;
             tc_fence_after();
             if (active) {
-                float *to = call.o + (int64_t)(seg.part + row) * D;
+                uint32_t s[2][32];
+                tmem_ld32(sp, s[0]);
+                tmem_ld32(sp + 32, s[1]);
+                tmem_ld_wait();
+                if (n < kKeyTile) {
 #pragma unroll
-                for (int x = 0; x < D / 32; ++x) {
-                    uint32_t s[32];
-                    tmem_ld32(mine + kO + 32 * x, s);
-                    tmem_ld_wait();
-                    if (row < seg.rows)
-#pragma unroll
-                        for (int i = 0; i < 8; ++i)
-                            *reinterpret_cast<uint4 *>(to + 32 * x + 4 * i) = make_uint4(s[4 * i], s[4 * i + 1], s[4 * i + 2], s[4 * i + 3]);
+                    for (int i = 0; i < kKeyTile; ++i)
+                        if (i >= n) s[i >> 5][i & 31] = 0xff800000u;        // -inf
                 }
-                if (row < seg.rows) call.ml[seg.part + row] = make_float2(m, l);
+                float mx = -INFINITY, my = -INFINITY;
+#pragma unroll
+                for (int i = 0; i < 32; ++i) { mx = fmaxf(mx, __uint_as_float(s[0][i])); my = fmaxf(my, __uint_as_float(s[1][i])); }
+                mx = fmaxf(mx, my) * c;
+                if (j == 0) m = mx;
+                else {
+                    const bool up = mx > m + 8.0f;          // from -inf as well
+                    if (__any_sync(0xffffffffu, up)) {
+                        const float f = up ? ex2(m - mx) : 1.0f;
+                        if (up) m = mx;
+                        l *= f;
+                        if (!wait_warp(&sm.o_bar[half][b ^ 1], (tile - 1) >> 1 & 1, abort_flag)) return false;        // the outputs so far
+                        tc_fence_after();
+#pragma unroll
+                        for (int x = 0; x < D / 16; ++x) {
+                            uint32_t o[16];
+                            tmem_ld16(mine + kO + 16 * x, o);
+                            tmem_ld_wait();
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+                            tmem_st16(mine + kO + 16 * x, o);
+                        }
+                    }
+                }
+                const float base = m == -INFINITY ? 0.0f : m;
+                float sum0 = 0.0f, sum1 = 0.0f;
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                    uint32_t w[8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        w[i] = pack<BF16>(ex2(__fmaf_rn(__uint_as_float(s[x >> 1][16 * (x & 1) + 2 * i]), c, -base)),
+                                          ex2(__fmaf_rn(__uint_as_float(s[x >> 1][16 * (x & 1) + 2 * i + 1]), c, -base)), i & 1 ? sum1 : sum0);
+                    tmem_st8(sp + 8 * x, w);                // over the scores
+                }
+                l += sum0 + sum1;
+                tmem_st_wait();
                 tc_fence_before();
             }
-        }
-    } else if (warp == 4) {
-        const int shift = 31 - __clz(page), box = min(page, kKeyTile);
-        while (ok && walk.next(call, seg)) {
-            const int *table = st.tables + (size_t)seg.slot * st.max_pages;
-            int base = INT32_MIN / 2, ids = -1;             // page numbers base .. base + 31 of the table, one a lane
-            for (int j = 0; j < seg.units; ++j, ++tile) {
-                const unsigned b = tile & 1, before = (tile >> 1 & 1) ^ 1;
-                const int key = seg.key0 + j * kKeyTile, p0 = key >> shift, mine = key + lane * box;
-                if (((key + kKeyTile - 1) >> shift) - base >= 32) {
-                    base = p0;
-                    ids = (p0 + lane) << shift < seg.key1 ? table[p0 + lane] : -1;
+            if (n < kKeyTile && half == 0) {                // before either half's product: the second follows the first
+                const unsigned stage = tile % kKvStages;    // the first half has a part in every tile
+                if (!wait_warp(&sm.v_bar[stage], tile / kKvStages & 1, abort_flag)) return false;
+                for (int i = tid; i < (kKeyTile - n) * (D / 8); i += 128) {
+                    const int r = n + i / (D / 8), x = i % (D / 8);
+                    *reinterpret_cast<uint4 *>(&sm.v[stage][x >> 3][r * 128 + (x & 7) * 16]) = make_uint4(0, 0, 0, 0);
                 }
-                int id = __shfl_sync(0xffffffffu, ids, ((mine >> shift) - base) & 31);           // a lane takes a box
-                if (lane * box >= kKeyTile || mine >= seg.key1) id = -1;
-                else if (id < 0 || id >= st.pages) { id = -1; atomicCAS(st.header, cq_kv::kOk, cq_kv::kBadPage); }
-                const unsigned bytes = (unsigned)__popc(__ballot_sync(0xffffffffu, id >= 0)) * box * D * 2;
-                const int y = ((id * cache.kv_heads + seg.head) << shift) + (mine & (page - 1));
-                if (tile >= 2 && !(ok = wait_warp(&sm.bar.s[b], before, abort_flag))) break;
-                if (lane == 0) cq_mbar_expect_tx(&sm.bar.k[b], bytes);
-                __syncwarp();
-                if (id >= 0)
-#pragma unroll
-                    for (int h = 0; h < D / 64; ++h) cq_tmap::load_2d(&sm.k[b][h][lane * box * 128], &k_map, 64 * h, y, &sm.bar.k[b]);
-                if (tile >= 2 && !(ok = wait_warp(&sm.bar.o[b], before, abort_flag))) break;
-                if (lane == 0) cq_mbar_expect_tx(&sm.bar.v[b], bytes);
-                __syncwarp();
-                if (id >= 0)
-#pragma unroll
-                    for (int h = 0; h < D / 64; ++h) cq_tmap::load_2d(&sm.v[b][h][lane * box * 128], &v_map, 64 * h, y, &sm.bar.v[b]);
+                fence_proxy_async_smem();
             }
+            arrive_warp(&sm.p_bar[half][b], lane);
         }
-        if (!ok)                        // leaving early: not before what is on its way has come (a copy that was never sent costs the wait's bound)
-            for (unsigned b = 0; b < 2; ++b)
-                if (tile >= b) {
-                    const unsigned last = (tile - b) >> 1 & 1;          // phase of the newest copy that may be out
-                    (void)(cq_mbar_wait_bounded(&sm.bar.k[b], last ^ 1) && cq_mbar_wait_bounded(&sm.bar.k[b], last));
-                    (void)(cq_mbar_wait_bounded(&sm.bar.v[b], last ^ 1) && cq_mbar_wait_bounded(&sm.bar.v[b], last));
+        if (!wait_warp(&sm.o_bar[half][(tile - 1) & 1], (tile - 1) >> 1 & 1, abort_flag)) return false;
+        tc_fence_after();
+        if (active) {
+            // The outputs go out as 32 x 32 boxes of 128-byte rows, one warp's each, from where Q was.  (Stored by their threads, a row each, they
+            // took the load / store unit 8,000 clocks, and the own warps' fragments with them.)
+            const int part = seg.part + half * 128 + warp * 32;
+#pragma unroll
+            for (int x = 0; x < D / 32; ++x) {
+                uint32_t o[32];
+                tmem_ld32(mine + kO + 32 * x, o);
+                tmem_ld_wait();
+                uint8_t *box = &sm.q[half][x % (D / 64)][warp * 4096];
+                if (x == D / 64) {
+                    if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+                    __syncwarp();
                 }
-    } else {
-        unsigned segment = 0, qk = 0;           // tiles whose first product is under way
-        const uint32_t qa = uniform(cq_smem_u32(&sm.q[0][0]) >> 4), ka = uniform(cq_smem_u32(&sm.k[0][0][0]) >> 4), va = uniform(cq_smem_u32(&sm.v[0][0][0]) >> 4);
-        const uint32_t t0 = uniform(tmem);
-        constexpr uint32_t kHalfK = kKeyTile * 128 >> 4, kBuf = D / 64 * kHalfK;
-        auto scores = [&]() {                   // S = Q K^T of tile qk
-            const unsigned b = qk & 1, phase = qk >> 1 & 1;
-            if (!wait_warp(&sm.bar.k[b], phase, abort_flag)) return false;
-            if (qk >= 2 && !wait_warp(&sm.bar.o[b], phase ^ 1, abort_flag)) return false;          // the weights there have been read
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    *reinterpret_cast<uint4 *>(box + lane * 128 + (i ^ (lane & 7)) * 16) = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0)
+                    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];\n\tcp.async.bulk.commit_group;"
+                                 ::"l"(&o_map), "r"(32 * x), "r"(part), "r"(cq_smem_u32(box)) : "memory");
+            }
+            if (row < rows) call.ml[part + lane] = make_float2(m, l);
+            tc_fence_before();
+        }
+        if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+        asm volatile("bar.sync %0, 128;" ::"r"(1 + half) : "memory");           // before the next Q
+    }
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+    return true;
+}
+
+template <int D>
+__device__ bool copy_part(Tiles<D> &sm, const cq_kv_cache &cache, const cq_kv::State &st, const Call &call, const CUtensorMap &k_map, const CUtensorMap &v_map) {
+    const int lane = threadIdx.x & 31, page = st.page, shift = 31 - __clz(page), box = min(page, kKeyTile), boxes = page < kKeyTile ? D / 64 : 1;
+    volatile int *abort_flag = &sm.abort;
+    SharedWalk walk(call, blockIdx.x);
+    Segment seg;
+    unsigned tile = 0, stage = 0, phase = 1;        // phase: of the use before
+    bool ok = true;
+    while (ok && walk.next(call, seg)) {
+        const int *table = st.tables + (size_t)seg.slot * st.max_pages;
+        int base = INT32_MIN / 2, ids = -1;             // page numbers base .. base + 31 of the table, one a lane
+        for (int j = 0; j < seg.units; ++j, ++tile) {
+            const int key = seg.key0 + j * kKeyTile, mine = key + lane * box;
+            if (((key + kKeyTile - 1) >> shift) - base >= 32) {
+                base = key >> shift;
+                ids = (base + lane) << shift < seg.key1 ? table[base + lane] : -1;
+            }
+            int id = __shfl_sync(0xffffffffu, ids, ((mine >> shift) - base) & 31);           // a lane takes a box
+            if (lane * box >= kKeyTile || mine >= seg.key1) id = -1;
+            else if (id < 0 || id >= st.pages) { id = -1; atomicCAS(st.header, cq_kv::kOk, cq_kv::kBadPage); }
+            const unsigned bytes = (unsigned)__popc(__ballot_sync(0xffffffffu, id >= 0)) * box * D * 2;
+            const int y = ((id * cache.kv_heads + seg.head) << shift) + (mine & (page - 1));
+            if (tile >= kKvStages && !(ok = wait_warp(&sm.k_free[stage], phase, abort_flag))) break;
+            if (lane == 0) expect_tx(cq_smem_u32(&sm.k_bar[stage]), bytes);
+            __syncwarp();
+            if (id >= 0)
+                for (int h = 0; h < boxes; ++h) load_3d(cq_smem_u32(&sm.k[stage][h][lane * box * 128]), &k_map, 0, y, h, cq_smem_u32(&sm.k_bar[stage]));
+            if (tile >= kKvStages && !(ok = wait_warp(&sm.v_free[stage], phase, abort_flag))) break;
+            if (lane == 0) expect_tx(cq_smem_u32(&sm.v_bar[stage]), bytes);
+            __syncwarp();
+            if (id >= 0)
+                for (int h = 0; h < boxes; ++h) load_3d(cq_smem_u32(&sm.v[stage][h][lane * box * 128]), &v_map, 0, y, h, cq_smem_u32(&sm.v_bar[stage]));
+            if (++stage == kKvStages) { stage = 0; phase ^= 1; }
+        }
+    }
+    if (!ok)                        // leaving early: not before what is on its way has come (a copy that was never sent costs the wait's bound)
+        for (unsigned b = 0; b < kKvStages; ++b)
+            if (tile >= b) {
+                const unsigned last = (tile - b) / kKvStages & 1;          // phase of the newest copy that may be out
+                (void)(cq_mbar_wait_bounded(&sm.k_bar[b], last ^ 1) && cq_mbar_wait_bounded(&sm.k_bar[b], last));
+                (void)(cq_mbar_wait_bounded(&sm.v_bar[b], last ^ 1) && cq_mbar_wait_bounded(&sm.v_bar[b], last));
+            }
+    return ok;
+}
+
+template <int D, bool BF16> __device__ bool mma_part(Tiles<D> &sm, const Call &call) {
+    constexpr uint32_t kTypes = BF16 ? (1u << 7) | (1u << 10) : 0u;
+    constexpr uint32_t kIdescQK = (1u << 4) | kTypes | ((uint32_t)kKeyTile >> 3) << 17 | (128u >> 4) << 24;
+    constexpr uint32_t kIdescPV = (1u << 4) | kTypes | (1u << 16) | ((uint32_t)D >> 3) << 17 | (128u >> 4) << 24;
+    constexpr uint32_t kHalfK = kKeyTile * 128 >> 4, kBuf = D / 64 * kHalfK, kQ = D / 64 * (kHalfBytes >> 4);
+    const uint32_t qa = uniform(cq_smem_u32(&sm.q[0][0][0]) >> 4), ka = uniform(cq_smem_u32(&sm.k[0][0][0]) >> 4), va = uniform(cq_smem_u32(&sm.v[0][0][0]) >> 4);
+    const uint32_t t0 = uniform(sm.tmem);
+    volatile int *abort_flag = &sm.abort;
+    SharedWalk walk(call, blockIdx.x);
+    Segment seg;
+    unsigned segments[2] = {0, 0}, qk[2] = {0, 0}, pv[2] = {0, 0};          // by half: segments, products under way
+    unsigned k_stage = 0, k_phase = 0, v_stage = 0, v_phase = 0;
+    auto scores = [&](int halves) {             // S = Q K^T of the next tile
+        if (!wait_warp(&sm.k_bar[k_stage], k_phase, abort_flag)) return false;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            if (h >= halves) break;
+            const unsigned b = qk[h] & 1;
+            if (qk[h] >= 2 && !wait_warp(&sm.o_bar[h][b], (qk[h] >> 1 & 1) ^ 1, abort_flag)) return false;          // the weights there have been read
             tc_fence_after();
             if (elect_one()) {
 #pragma unroll
                 for (int x = 0; x < D / 16; ++x)
-                    mma_ss(t0 + kS + b * kKeyTile, qa + (x >> 2) * (kHalfBytes >> 4) + (x & 3) * 2, ka + b * kBuf + (x >> 2) * kHalfK + (x & 3) * 2, kIdescQK, x > 0);
-                tc_commit(&sm.bar.s[b]);
+                    mma_ss(t0 + h * kGroup + b * kKeyTile, qa + h * kQ + (x >> 2) * (kHalfBytes >> 4) + (x & 3) * 2, ka + k_stage * kBuf + (x >> 2) * kHalfK + (x & 3) * 2,
+                           kIdescQK, x > 0);
+                tc_commit(&sm.s_bar[h][b]);
+                if (h == halves - 1) tc_commit(&sm.k_free[k_stage]);
             }
             __syncwarp();
-            ++qk;
-            return true;
-        };
-        while (ok && walk.next(call, seg)) {
-            const int units = (int)uniform((uint32_t)seg.units);
-            if (!(ok = wait_warp(&sm.bar.q, segment++ & 1, abort_flag) && scores())) break;
-            for (int j = 0; j < units; ++j, ++tile) {
-                const unsigned b = tile & 1, phase = tile >> 1 & 1;
-                if (j + 1 < units && !(ok = scores())) break;
-                if (!(ok = wait_warp(&sm.bar.v[b], phase, abort_flag)) || !(ok = wait_warp(&sm.bar.p[b], phase, abort_flag))) break;
+            ++qk[h];
+        }
+        if (++k_stage == kKvStages) { k_stage = 0; k_phase ^= 1; }
+        return true;
+    };
+    bool ok = true;
+    while (ok && walk.next(call, seg)) {
+        const int units = (int)uniform((uint32_t)seg.units), halves = uniform((uint32_t)seg.rows) > 128 ? 2 : 1;
+        for (int h = 0; h < halves && ok; ++h) ok = wait_warp(&sm.q_bar[h], segments[h]++ & 1, abort_flag);
+        if (!ok || !(ok = scores(halves))) break;
+        for (int j = 0; ok && j < units; ++j) {
+            if (j + 1 < units && !(ok = scores(halves))) break;
+            if (!(ok = wait_warp(&sm.v_bar[v_stage], v_phase, abort_flag))) break;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                if (h >= halves) break;
+                const unsigned b = pv[h] & 1;
+                if (!(ok = wait_warp(&sm.p_bar[h][b], pv[h] >> 1 & 1, abort_flag))) break;
                 tc_fence_after();
                 if (elect_one()) {
 #pragma unroll
                     for (int x = 0; x < kKeyTile / 16; ++x)
-                        mma_ts(t0 + kO, t0 + kS + b * kKeyTile + 8 * x, (va + b * kBuf + x * (2048 >> 4)) | kHalfK << 16, kIdescPV, j > 0 || x > 0);
-                    tc_commit(&sm.bar.o[b]);
+                        mma_ts(t0 + h * kGroup + kO, t0 + h * kGroup + b * kKeyTile + 8 * x, (va + v_stage * kBuf + x * (2048 >> 4)) | kHalfK << 16, kIdescPV, j > 0 || x > 0);
+                    tc_commit(&sm.o_bar[h][b]);
+                    if (h == halves - 1) tc_commit(&sm.v_free[v_stage]);
                 }
                 __syncwarp();
+                ++pv[h];
             }
+            if (++v_stage == kKvStages) { v_stage = 0; v_phase ^= 1; }
         }
-        if (!ok)                        // nor before the products have ended
-            for (unsigned b = 0; b < 2; ++b) {
-                if (qk > b) (void)cq_mbar_wait_bounded(&sm.bar.s[b], (qk - 1 - b) >> 1 & 1);
-                if (tile > b) (void)cq_mbar_wait_bounded(&sm.bar.o[b], (tile - 1 - b) >> 1 & 1);
-            }
     }
+    if (!ok)                        // nor before the products have ended
+        for (int h = 0; h < 2; ++h)
+            for (unsigned b = 0; b < 2; ++b) {
+                if (qk[h] > b) (void)cq_mbar_wait_bounded(&sm.s_bar[h][b], (qk[h] - 1 - b) >> 1 & 1);
+                if (pv[h] > b) (void)cq_mbar_wait_bounded(&sm.o_bar[h][b], (pv[h] - 1 - b) >> 1 & 1);
+            }
     return ok;
 }
 
@@ -302,65 +354,81 @@ template <bool BF16> __device__ __forceinline__ void mma16816(float (&d)[4], con
                      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// The copies of a warp's steps, ahead of their use and across its segments.
+// The copies of a warp's steps, ahead of their use and across its segments.  Sixteen rows of a page are one block of memory, which the lanes copy 16 bytes
+// at a time; rows behind the last key come as zeros.  (By TMA a step cost its warp 500 clocks of issue against some 100.)
 template <int D> struct Loader {
     OwnWalk walk;
     Segment seg;
-    int step, sent;                 // step in the segment, steps sent
+    int step;                       // in the segment
     int base, ids, shift;           // page numbers base .. base + 31 of the segment's table, one a lane
-    __device__ __forceinline__ Loader(const Call &call, int worker, int page_shift) : walk(call, worker), step(0), sent(0), shift(page_shift) { seg.units = 0; }
-    __device__ __forceinline__ void send(Step<D> &to, uint64_t *bar, const Call &call, const cq_kv::State &st, int kv_heads, const CUtensorMap &k_map, const CUtensorMap &v_map,
-                                         int lane) {
-        if (step == seg.units) {
-            if (!walk.next(call, seg)) return;
+    const uint8_t *k, *v;           // the layer, at this lane's 16 bytes
+    uint32_t off[D / 32];           // of this lane's pieces in shared memory, by piece modulo D / 32
+    __device__ __forceinline__ Loader(const Call &call, int worker, int page_shift, const void *kp, const void *vp, int lane)
+        : walk(call, worker), step(0), shift(page_shift), k((const uint8_t *)kp + lane * 16), v((const uint8_t *)vp + lane * 16) {
+        seg.units = 0;
+        constexpr int kUnits = D / 8, kRows = 32 / kUnits;              // 16-byte units of a row, rows of a piece
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) {
+            const int row = lane / kUnits + i * kRows, x = lane % kUnits;
+            off[i] = (x >> 3) * (kStep * 128) + row * 128 + ((x & 7) ^ (row & 7)) * 16;
+        }
+    }
+    __device__ __forceinline__ void send(uint32_t to, const Call &call, const cq_kv::State &st, int kv_heads, int lane) {
+        constexpr int kPieces = D / 16, kPeriod = D / 32, kRows = 256 / D;      // pieces of 512 bytes; after kPeriod of them (8 rows) the pattern repeats
+        if (step == seg.units && walk.next(call, seg)) {
             step = 0;
             base = INT32_MIN / 2;
         }
-        const int key = seg.key0 + kStep * step, j = key >> shift;
-        if (j - base >= 32) {
-            base = j;
-            ids = (j + lane) << shift < seg.key1 ? st.tables[(size_t)seg.slot * st.max_pages + j + lane] : -1;
-        }
-        const int id = __shfl_sync(0xffffffffu, ids, j - base);
-        const bool there = id >= 0 && id < st.pages;
-        if (lane == 0) {
-            cq_mbar_expect_tx(bar, there ? (unsigned)sizeof(Step<D>) : 0u);
-            if (there) {
-                const int y = ((id * kv_heads + seg.head) << shift) + (key & (st.page - 1));
+        if (step < seg.units) {
+            const int key = seg.key0 + kStep * step, j = key >> shift;
+            if (j - base >= 32) {
+                base = j;
+                ids = (j + lane) << shift < seg.key1 ? st.tables[(size_t)seg.slot * st.max_pages + j + lane] : -1;
+            }
+            int id = __shfl_sync(0xffffffffu, ids, j - base), n = seg.key1 - key;
+            if ((unsigned)id >= (unsigned)st.pages) {
+                if (lane == 0) atomicCAS(st.header, cq_kv::kOk, cq_kv::kBadPage);
+                id = n = 0;
+            }
+            const int64_t at = (int64_t)(((id * kv_heads + seg.head) << shift) + (key & (st.page - 1))) * (D * 2);
+            const uint8_t *ks = k + at, *vs = v + at;
+            const uint32_t vt = to + (uint32_t)sizeof(Step<D>) / 2;
 #pragma unroll
-                for (int h = 0; h < D / 64; ++h) {
-                    cq_tmap::load_2d(to.k[h], &k_map, 64 * h, y, bar);
-                    cq_tmap::load_2d(to.v[h], &v_map, 64 * h, y, bar);
-                }
-            } else atomicCAS(st.header, cq_kv::kOk, cq_kv::kBadPage);
+            for (int i = 0; i < kPieces; ++i) {
+                const uint32_t o = off[i % kPeriod] + i / kPeriod * 1024;
+                const int bytes = lane / (D / 8) + i * kRows < n ? 16 : 0;
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + o), "l"(ks + i * 512), "r"(bytes) : "memory");
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(vt + o), "l"(vs + i * 512), "r"(bytes) : "memory");
+            }
+            ++step;
         }
-        ++step;
-        ++sent;
+        cq_cp_async_commit();           // one group a step, an empty one behind the last
     }
 };
 
 // The warp's share of the own line.  Fragments as mma.sync m16n8k16 has them: a lane holds rows lane / 4 and lane / 4 + 8.
 template <int D, bool BF16>
-__device__ bool own_part(Tiles<D> &sm, const cq_kv_cache &cache, const cq_kv::State &st, const Call &call, const CUtensorMap &k_map, const CUtensorMap &v_map,
-                         const uint8_t *__restrict__ q, int64_t q_stride, float c) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, x2 = (lane & 3) * 2, per = call.sh.per_kv;
+__device__ void own_part(Tiles<D> &sm, const cq_kv_cache &cache, const cq_kv::State &st, const Call &call, const uint8_t *__restrict__ k_layer,
+                         const uint8_t *__restrict__ v_layer, const uint8_t *__restrict__ q, int64_t q_stride, float c) {
+    constexpr int kStages = Tiles<D>::kStages;
+    const int lane = threadIdx.x & 31, warp = (threadIdx.x >> 5) - kOwnWarp, g = lane >> 2, x2 = (lane & 3) * 2, per = call.sh.per_kv;
     const int worker = blockIdx.x * kMmaWarps + warp;
-    Step<D> *steps = sm.step[warp];
-    uint64_t *bars = sm.step_bar[warp];
-    Loader<D> load(call, worker, 31 - __clz(st.page));
+    const uint32_t steps_at = uniform(cq_smem_u32(sm.step[warp]));
+    Loader<D> load(call, worker, 31 - __clz(st.page), k_layer, v_layer, lane);
     OwnWalk walk = load.walk;
     const int units = walk.left;
-    if (units <= 0) return true;
-#pragma unroll
-    for (int i = 0; i < kStages; ++i) load.send(steps[i], &bars[i], call, st, cache.kv_heads, k_map, v_map, lane);
+    if (units <= 0) return;
+    auto send = [&](int i) { load.send(steps_at + i * (uint32_t)sizeof(Step<D>), call, st, cache.kv_heads, lane); };
+#pragma unroll 1
+    for (int i = 0; i < kStages; ++i) send(i);
     Segment seg;
     seg.units = 0;
     int step = 0;
-    bool ok = true;
     uint32_t qa[D / 16][4];
     float o[D / 8][4], m0 = 0.0f, m1 = 0.0f, l0 = 0.0f, l1 = 0.0f;
+    int stage = 0;
+#pragma unroll 1
     for (int u = 0; u < units; ++u) {
-        const int stage = u % kStages;
         if (step == seg.units) {
             walk.next(call, seg);
             step = 0;
@@ -381,8 +449,9 @@ __device__ bool own_part(Tiles<D> &sm, const cq_kv_cache &cache, const cq_kv::St
         }
         const int n = seg.key1 - seg.key0 - kStep * step;        // keys of this step, if fewer than 16
         const bool upper = seg.rows > 8;
-        if (!(ok = wait_warp(&bars[stage], (u / kStages) & 1, &sm.abort))) break;
-        const uint32_t kb = cq_smem_u32(steps[stage].k), vb = cq_smem_u32(steps[stage].v);
+        cq_cp_async_wait<kStages - 1>();
+        __syncwarp();
+        const uint32_t kb = steps_at + stage * (uint32_t)sizeof(Step<D>), vb = kb + (uint32_t)sizeof(Step<D>) / 2;
         float s[2][4] = {};
 #pragma unroll
         for (int x = 0; x < D / 32; ++x)
@@ -400,12 +469,6 @@ __device__ bool own_part(Tiles<D> &sm, const cq_kv_cache &cache, const cq_kv::St
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
                     if (8 * t + x2 + (i & 1) >= n) s[t][i] = -INFINITY;
-            for (int i = lane; i < (kStep - n) * (D / 8); i += 32) {
-                const int r = n + i / (D / 8), x = i % (D / 8);
-                *reinterpret_cast<uint4 *>(&steps[stage].v[x >> 3][r * 128 + (x & 7) * 16]) = make_uint4(0, 0, 0, 0);
-            }
-            fence_proxy_async_smem();
-            __syncwarp();
         }
         float mx0 = fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[1][0], s[1][1])), mx1 = fmaxf(fmaxf(s[0][2], s[0][3]), fmaxf(s[1][2], s[1][3]));
         mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, 1));
@@ -441,7 +504,8 @@ __device__ bool own_part(Tiles<D> &sm, const cq_kv_cache &cache, const cq_kv::St
             mma16816<BF16>(o[2 * x + 1], p, b[2], b[3]);
         }
         __syncwarp();
-        load.send(steps[stage], &bars[stage], call, st, cache.kv_heads, k_map, v_map, lane);
+        send(stage);
+        if (++stage == kStages) stage = 0;
         if (++step == seg.units) {
             l0 += __shfl_xor_sync(0xffffffffu, l0, 1);
             l1 += __shfl_xor_sync(0xffffffffu, l1, 1);
@@ -459,34 +523,29 @@ __device__ bool own_part(Tiles<D> &sm, const cq_kv_cache &cache, const cq_kv::St
             }
         }
     }
-    if (!ok)                            // leaving early: not before what is on its way has come
-        for (int i = 0; i < kStages; ++i) {
-            const int sent = (load.sent - i + kStages - 1) / kStages;       // copies into this stage
-            if (sent > 0) (void)cq_mbar_wait_bounded(&bars[i], (sent - 1) & 1);
-        }
-    return ok;
 }
 
-// The first half of the CTAs begins with shared items, the second with own ones, so that the tensor cores and HBM are both in use.
 template <int D, bool BF16>
-__global__ void __launch_bounds__(kThreads, 2) prefix_mma_kernel(const cq_kv_cache cache, const Call call, const __grid_constant__ CUtensorMap k_map,
-                                                                 const __grid_constant__ CUtensorMap v_map, const __grid_constant__ CUtensorMap k_step,
-                                                                 const __grid_constant__ CUtensorMap v_step, const uint8_t *__restrict__ q, int64_t q_stride, float c) {
+__global__ void __launch_bounds__(kThreads, 1) prefix_mma_kernel(const cq_kv_cache cache, const Call call, const __grid_constant__ CUtensorMap k_map,
+                                                                 const __grid_constant__ CUtensorMap v_map, const __grid_constant__ CUtensorMap o_map,
+                                                                 const uint8_t *__restrict__ k_layer, const uint8_t *__restrict__ v_layer,
+                                                                 const uint8_t *__restrict__ q, int64_t q_stride, float c) {
     extern __shared__ uint8_t raw[];
     Tiles<D> &sm = *reinterpret_cast<Tiles<D> *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
     const cq_kv::State st = cq_kv::state_of(cache);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     if (tid == 0) {
-        cq_mbar_init(&sm.bar.q, 4);
         for (int i = 0; i < 2; ++i) {
-            cq_mbar_init(&sm.bar.k[i], 1); cq_mbar_init(&sm.bar.v[i], 1);
-            cq_mbar_init(&sm.bar.s[i], 1); cq_mbar_init(&sm.bar.p[i], 4); cq_mbar_init(&sm.bar.o[i], 1);
+            cq_mbar_init(&sm.q_bar[i], 4);
+            for (int b = 0; b < 2; ++b) { cq_mbar_init(&sm.s_bar[i][b], 1); cq_mbar_init(&sm.p_bar[i][b], 4); cq_mbar_init(&sm.o_bar[i][b], 1); }
         }
-        for (int i = 0; i < kMmaWarps * kStages; ++i) cq_mbar_init(&sm.step_bar[0][i], 1);
+        for (int i = 0; i < kKvStages; ++i) {
+            cq_mbar_init(&sm.k_bar[i], 1); cq_mbar_init(&sm.v_bar[i], 1); cq_mbar_init(&sm.k_free[i], 1); cq_mbar_init(&sm.v_free[i], 1);
+        }
         sm.abort = 0;
         cq_fence_mbar_init();
     }
-    if (warp == 5) {
+    if (warp == kMmaWarp) {
         tmem_alloc(&sm.tmem, kCols);
         tmem_relinquish();
         tc_fence_before();
@@ -494,51 +553,61 @@ __global__ void __launch_bounds__(kThreads, 2) prefix_mma_kernel(const cq_kv_cac
     cq_pdl_launch_dependents();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = sm.tmem;
     cq_pdl_wait();
-    const bool own_first = blockIdx.x >= gridDim.x / 2;
     bool ok = true;
-    if (own_first) {
-        ok = own_part<D, BF16>(sm, cache, st, call, k_step, v_step, q, q_stride, c);
-        __syncthreads();
+    if (warp < kCopyWarp) {
+        regs_up<kRegsSoft>();
+        ok = softmax_part<D, BF16>(sm, call, o_map, q, q_stride, c, warp >> 2);
     }
-    if (!sm.abort) ok = shared_part<D, BF16>(sm, cache, st, call, k_map, v_map, q, q_stride, c, tmem) && ok;
-    if (!own_first) {
-        __syncthreads();
-        if (!sm.abort) ok = own_part<D, BF16>(sm, cache, st, call, k_step, v_step, q, q_stride, c) && ok;
+    else if (warp < kOwnWarp) {
+        regs_down<kRegsMisc>();
+        if (warp == kCopyWarp) ok = copy_part<D>(sm, cache, st, call, k_map, v_map);
+        else if (warp == kMmaWarp) ok = mma_part<D, BF16>(sm, call);
+    } else {
+        regs_up<kRegsOwn>();
+        own_part<D, BF16>(sm, cache, st, call, k_layer, v_layer, q, q_stride, c);
     }
     if (!ok && lane == 0) atomicCAS(st.header, cq_kv::kOk, cq_kv::kTimeout);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    if (warp == 5) tmem_dealloc(tmem, kCols);
+    if (warp == kMmaWarp) tmem_dealloc(sm.tmem, kCols);
 }
 
-// One layer of a pool as rows of D elements; box: rows of one page x 64 elements, 128-byte swizzle.
-bool pool_map(const void *base, int64_t rows, int d, int box_rows, CUtensorMap &out) {
+bool encode(CUtensorMap &out, CUtensorMapDataType type, int rank, const void *base, const cuuint64_t *dims, const cuuint64_t *strides, const cuuint32_t *box) {
     using Encode = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *, const cuuint32_t *,
                                 const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-    static const Encode encode = [] {
-        void *fn = nullptr;
+    static const Encode fn = [] {
+        void *f = nullptr;
         cudaDriverEntryPointQueryResult res;
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &res) != cudaSuccess || res != cudaDriverEntryPointSuccess) {
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &res) != cudaSuccess || res != cudaDriverEntryPointSuccess) {
             (void)cudaGetLastError();
-            fn = nullptr;
+            f = nullptr;
         }
-        return (Encode)fn;
+        return (Encode)f;
     }();
-    if (!encode) return false;
-    const cuuint64_t dims[2] = {(cuuint64_t)d, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)d * 2};
-    const cuuint32_t box[2] = {64, (cuuint32_t)box_rows}, one[2] = {1, 1};
-    return encode(&out, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, const_cast<void *>(base), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+    const cuuint32_t one[3] = {1, 1, 1};
+    return fn && fn(&out, type, rank, const_cast<void *>(base), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                    CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+// One layer of a pool as [D / 64][rows][64]; box: `boxes` blocks of 64 dims of some rows of a page.
+bool pool_map(const void *base, int64_t rows, int d, int box_rows, int boxes, CUtensorMap &out) {
+    const cuuint64_t dims[3] = {64, (cuuint64_t)rows, (cuuint64_t)d / 64}, strides[2] = {(cuuint64_t)d * 2, 128};
+    const cuuint32_t box[3] = {64, (cuuint32_t)box_rows, (cuuint32_t)boxes};
+    return encode(out, CU_TENSOR_MAP_DATA_TYPE_UINT16, 3, base, dims, strides, box);
+}
+// The partial outputs of shared items as [rows][D] f32; box: 32 x 32.
+bool part_map(const Call &c, CUtensorMap &out) {
+    const cuuint64_t dims[2] = {(cuuint64_t)c.sh.head_dim, (cuuint64_t)(c.shared_items + c.sh.ctas) * c.sh.row_tile}, strides[1] = {(cuuint64_t)c.sh.head_dim * 4};
+    const cuuint32_t box[2] = {32, 32};
+    return encode(out, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 2, c.o, dims, strides, box);
 }
 
 template <int D, bool BF16>
-void launch(const Call &c, const cq_kv_cache &cache, const CUtensorMap (&m)[4], const void *q, int64_t q_stride, float scale, cudaStream_t st) {
+void launch(const Call &c, const cq_kv_cache &cache, const CUtensorMap (&m)[3], const uint8_t *k, const uint8_t *v, const void *q, int64_t q_stride, float scale, cudaStream_t st) {
     constexpr int smem = (int)sizeof(Tiles<D>) + 1024;
     cudaFuncSetAttribute(prefix_mma_kernel<D, BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    cq_launch_k(prefix_mma_kernel<D, BF16>, dim3(c.sh.ctas), dim3(kThreads), smem, st, cache, c, m[0], m[1], m[2], m[3], (const uint8_t *)q, q_stride,
+    cq_launch_k(prefix_mma_kernel<D, BF16>, dim3(c.sh.ctas), dim3(kThreads), smem, st, cache, c, m[0], m[1], m[2], k, v, (const uint8_t *)q, q_stride,
                 (float)(scale * 1.4426950408889634));
 }
 
@@ -547,15 +616,14 @@ void launch(const Call &c, const cq_kv_cache &cache, const CUtensorMap (&m)[4], 
 bool cq_attn::mma_launch(const Call &c, const cq_kv_cache &cache, int layer, const void *q, int64_t q_stride, float scale, cudaStream_t st) {
     const int64_t rows = (int64_t)cache.pages * cache.kv_heads * cache.page_size, offset = rows * layer * cache.head_dim * 2;
     const uint8_t *k = (const uint8_t *)cache.k + offset, *v = (const uint8_t *)cache.v + offset;
-    const int box = cache.page_size < kKeyTile ? cache.page_size : kKeyTile;
-    CUtensorMap m[4];
-    if (!pool_map(k, rows, cache.head_dim, box, m[0]) || !pool_map(v, rows, cache.head_dim, box, m[1]) ||
-        !pool_map(k, rows, cache.head_dim, kStep, m[2]) || !pool_map(v, rows, cache.head_dim, kStep, m[3])) {
+    const int d = cache.head_dim, box = cache.page_size < kKeyTile ? cache.page_size : kKeyTile, boxes = cache.page_size < kKeyTile ? 1 : d / 64;
+    CUtensorMap m[3];
+    if (!pool_map(k, rows, d, box, boxes, m[0]) || !pool_map(v, rows, d, box, boxes, m[1]) || !part_map(c, m[2])) {
         cq_set_status(CQ_ERR_CUDA, "prefix_attention: cuTensorMapEncodeTiled is not available or refused the pool");
         return false;
     }
     const bool bf16 = c.sh.elem == CQ_BF16;
-    if (c.sh.head_dim == 128) bf16 ? launch<128, true>(c, cache, m, q, q_stride, scale, st) : launch<128, false>(c, cache, m, q, q_stride, scale, st);
-    else bf16 ? launch<64, true>(c, cache, m, q, q_stride, scale, st) : launch<64, false>(c, cache, m, q, q_stride, scale, st);
+    if (c.sh.head_dim == 128) bf16 ? launch<128, true>(c, cache, m, k, v, q, q_stride, scale, st) : launch<128, false>(c, cache, m, k, v, q, q_stride, scale, st);
+    else bf16 ? launch<64, true>(c, cache, m, k, v, q, q_stride, scale, st) : launch<64, false>(c, cache, m, k, v, q, q_stride, scale, st);
     return true;
 }
