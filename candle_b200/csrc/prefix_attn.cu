@@ -206,7 +206,7 @@ template <typename T, int D> __global__ void __launch_bounds__(256) prefix_join_
     cq_pdl_wait();
     const int lane = threadIdx.x & 31, per = sh.per_kv, n = blockIdx.y, hq = blockIdx.x * 8 + (threadIdx.x >> 5);
     if (hq >= sh.heads) return;
-    const int h = div_per(hq, sh), in = hq - h * per, tile = in / sh.own_rows;          // own_rows: 16 or 32
+    const int h = div_per(hq, sh), in = hq - h * per, tile = in / sh.own_rows;          // own_rows: 8 or 32
     const int64_t row = (int64_t)n * sh.heads + hq;
     const Query q = pl.query[n];
     const int chunk = pl.header[1], own_chunk = pl.header[3];
@@ -294,7 +294,7 @@ bool shape_ok(const cq_kv_cache *cache, const cq_prefix_plan *p, const char *who
     s = Shape{p->batch, p->queries, p->heads, cache->kv_heads, p->groups, cache->head_dim, cache->elem, p->heads / cache->kv_heads};
     s.ctas = p->ctas;
     if (cache->elem == CQ_F32) { s.row_tile = s.own_rows = 32; s.own_shift = 6; s.own_workers = s.ctas; }
-    else { s.row_tile = 256; s.own_rows = 16; s.own_shift = 4; s.own_workers = s.ctas * kMmaWarps; }
+    else { s.row_tile = 256; s.own_rows = 8; s.own_shift = 4; s.own_workers = s.ctas * kMmaWarps; }
     s.own_tiles = (s.per_kv + s.own_rows - 1) / s.own_rows;
     if (s.per_kv > 1) s.rcp = (unsigned)(((1ull << 32) + s.per_kv - 1) / s.per_kv);
     return true;

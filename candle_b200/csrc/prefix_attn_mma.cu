@@ -406,7 +406,30 @@ template <int D> struct Loader {
     }
 };
 
-// The warp's share of the own line.  Fragments as mma.sync m16n8k16 has them: a lane holds rows lane / 4 and lane / 4 + 8.
+// 8 x 8 of 16 bits, a lane holding two of row lane / 4, to the same of its transpose
+__device__ __forceinline__ uint32_t transpose8(uint32_t v) {
+    uint32_t r;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    return r;
+}
+template <bool BF16> __device__ __forceinline__ uint32_t pack(float a, float b, float &sum_a, float &sum_b) {
+    uint32_t w;
+    if constexpr (BF16) {
+        asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(b), "f"(a));
+        sum_a += __uint_as_float(w << 16);
+        sum_b += __uint_as_float(w & 0xffff0000u);
+    } else {
+        asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(b), "f"(a));
+        const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w));
+        sum_a += f.x;
+        sum_b += f.y;
+    }
+    return w;
+}
+
+// The warp's share of the own line: S^T = K Q^T (16 keys x 8 rows), O^T += V^T P^T (dims x 8 rows) by mma.sync m16n8k16.  With rows as the narrow side eight of them
+// cost half the products and half the registers that they would cost as half of a 16-row side.  A lane holds rows 2 (lane % 4) and the next, keys (dims)
+// lane / 4 and + 8; the weights change sides by a transposition.
 template <int D, bool BF16>
 __device__ void own_part(Tiles<D> &sm, const cq_kv_cache &cache, const cq_kv::State &st, const Call &call, const uint8_t *__restrict__ k_layer,
                          const uint8_t *__restrict__ v_layer, const uint8_t *__restrict__ q, int64_t q_stride, float c) {
@@ -421,11 +444,13 @@ __device__ void own_part(Tiles<D> &sm, const cq_kv_cache &cache, const cq_kv::St
     auto send = [&](int i) { load.send(steps_at + i * (uint32_t)sizeof(Step<D>), call, st, cache.kv_heads, lane); };
 #pragma unroll 1
     for (int i = 0; i < kStages; ++i) send(i);
+    // this lane's row address in the fragments' 8 x 8 blocks: of K by key and half of a 16-dim step, of V by key and half of a 16-dim tile
+    const int k_key = (lane >> 3 & 1) * 8 + (lane & 7), k_half = lane >> 4, v_key = (lane >> 4) * 8 + (lane & 7), v_half = lane >> 3 & 1;
     Segment seg;
     seg.units = 0;
     int step = 0;
-    uint32_t qa[D / 16][4];
-    float o[D / 8][4], m0 = 0.0f, m1 = 0.0f, l0 = 0.0f, l1 = 0.0f;
+    uint32_t qb[D / 16][2];
+    float o[D / 16][4], m0 = 0.0f, m1 = 0.0f, l0 = 0.0f, l1 = 0.0f;
     int stage = 0;
 #pragma unroll 1
     for (int u = 0; u < units; ++u) {
@@ -433,51 +458,44 @@ __device__ void own_part(Tiles<D> &sm, const cq_kv_cache &cache, const cq_kv::St
             walk.next(call, seg);
             step = 0;
             const int query = div_per(seg.row0, call.sh);
-            const uint8_t *src = q + ((int64_t)query * q_stride + (int64_t)(seg.head * per + seg.row0 - query * per) * D) * 2;
+            const uint8_t *src = q + ((int64_t)query * q_stride + (int64_t)(seg.head * per + seg.row0 - query * per + g) * D + x2) * 2;
 #pragma unroll
             for (int x = 0; x < D / 16; ++x)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int r = g + (i & 1) * 8;
-                    qa[x][i] = r < seg.rows ? *reinterpret_cast<const uint32_t *>(src + ((int64_t)r * D + 16 * x + (i >> 1) * 8 + x2) * 2) : 0u;
-                }
+                for (int i = 0; i < 2; ++i) qb[x][i] = g < seg.rows ? *reinterpret_cast<const uint32_t *>(src + (16 * x + 8 * i) * 2) : 0u;
 #pragma unroll
-            for (int x = 0; x < D / 8; ++x)
+            for (int x = 0; x < D / 16; ++x)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) o[x][i] = 0.0f;
             l0 = l1 = 0.0f;
         }
         const int n = seg.key1 - seg.key0 - kStep * step;        // keys of this step, if fewer than 16
-        const bool upper = seg.rows > 8;
         cq_cp_async_wait<kStages - 1>();
         __syncwarp();
         const uint32_t kb = steps_at + stage * (uint32_t)sizeof(Step<D>), vb = kb + (uint32_t)sizeof(Step<D>) / 2;
         float s[2][4] = {};
 #pragma unroll
-        for (int x = 0; x < D / 32; ++x)
-#pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                const int key = 8 * t + (lane & 7), unit = 4 * x + (lane >> 3);
-                uint32_t b[4];
-                ldsm(b, kb + (unit >> 3) * (kStep * 128) + key * 128 + ((unit & 7) ^ (key & 7)) * 16);
-                mma16816<BF16>(s[t], qa[2 * x], b[0], b[1]);
-                mma16816<BF16>(s[t], qa[2 * x + 1], b[2], b[3]);
-            }
-        if (n < kStep) {
-#pragma unroll
-            for (int t = 0; t < 2; ++t)
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (8 * t + x2 + (i & 1) >= n) s[t][i] = -INFINITY;
+        for (int x = 0; x < D / 16; ++x) {
+            const int unit = 2 * x + k_half;
+            uint32_t a[4];
+            ldsm(a, kb + (unit >> 3) * (kStep * 128) + k_key * 128 + ((unit & 7) ^ (k_key & 7)) * 16);
+            mma16816<BF16>(s[x & 1], a, qb[x][0], qb[x][1]);
         }
-        float mx0 = fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[1][0], s[1][1])), mx1 = fmaxf(fmaxf(s[0][2], s[0][3]), fmaxf(s[1][2], s[1][3]));
-        mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, 1));
-        mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, 1));
-        mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, 2)) * c;
-        mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, 2)) * c;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[0][i] += s[1][i];
+        if (g >= n) s[0][0] = s[0][1] = -INFINITY;
+        if (g + 8 >= n) s[0][2] = s[0][3] = -INFINITY;
+        float mx0 = fmaxf(s[0][0], s[0][2]), mx1 = fmaxf(s[0][1], s[0][3]);
+#pragma unroll
+        for (int x = 4; x <= 16; x <<= 1) {
+            mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, x));
+            mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, x));
+        }
+        mx0 *= c;
+        mx1 *= c;
         if (step == 0) { m0 = mx0; m1 = mx1; }
         else {
-            const bool up0 = mx0 > m0 + 8.0f, up1 = upper && mx1 > m1 + 8.0f;
+            const bool up0 = mx0 > m0 + 8.0f, up1 = mx1 > m1 + 8.0f;
             if (__any_sync(0xffffffffu, up0 || up1)) {
                 const float f0 = up0 ? ex2(m0 - mx0) : 1.0f, f1 = up1 ? ex2(m1 - mx1) : 1.0f;
                 if (up0) m0 = mx0;
@@ -485,41 +503,37 @@ __device__ void own_part(Tiles<D> &sm, const cq_kv_cache &cache, const cq_kv::St
                 l0 *= f0;
                 l1 *= f1;
 #pragma unroll
-                for (int x = 0; x < D / 8; ++x) { o[x][0] *= f0; o[x][1] *= f0; o[x][2] *= f1; o[x][3] *= f1; }
+                for (int x = 0; x < D / 16; ++x) { o[x][0] *= f0; o[x][1] *= f1; o[x][2] *= f0; o[x][3] *= f1; }
             }
         }
         const float b0 = m0 == -INFINITY ? 0.0f : m0, b1 = m1 == -INFINITY ? 0.0f : m1;
-        uint32_t p[4];
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-            p[2 * t] = pack<BF16>(ex2(__fmaf_rn(s[t][0], c, -b0)), ex2(__fmaf_rn(s[t][1], c, -b0)), l0);
-            p[2 * t + 1] = upper ? pack<BF16>(ex2(__fmaf_rn(s[t][2], c, -b1)), ex2(__fmaf_rn(s[t][3], c, -b1)), l1) : 0u;
-        }
+        const uint32_t p0 = transpose8(pack<BF16>(ex2(__fmaf_rn(s[0][0], c, -b0)), ex2(__fmaf_rn(s[0][1], c, -b1)), l0, l1));
+        const uint32_t p1 = transpose8(pack<BF16>(ex2(__fmaf_rn(s[0][2], c, -b0)), ex2(__fmaf_rn(s[0][3], c, -b1)), l0, l1));
 #pragma unroll
         for (int x = 0; x < D / 16; ++x) {
-            const int key = lane & 15, unit = 2 * x + (lane >> 4);
-            uint32_t b[4];
-            ldsm_t(b, vb + (unit >> 3) * (kStep * 128) + key * 128 + ((unit & 7) ^ (key & 7)) * 16);
-            mma16816<BF16>(o[2 * x], p, b[0], b[1]);
-            mma16816<BF16>(o[2 * x + 1], p, b[2], b[3]);
+            const int unit = 2 * x + v_half;
+            uint32_t a[4];
+            ldsm_t(a, vb + (unit >> 3) * (kStep * 128) + v_key * 128 + ((unit & 7) ^ (v_key & 7)) * 16);
+            mma16816<BF16>(o[x], a, p0, p1);
         }
         __syncwarp();
         send(stage);
         if (++stage == kStages) stage = 0;
         if (++step == seg.units) {
-            l0 += __shfl_xor_sync(0xffffffffu, l0, 1);
-            l1 += __shfl_xor_sync(0xffffffffu, l1, 1);
-            l0 += __shfl_xor_sync(0xffffffffu, l0, 2);
-            l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
-            float *to = call.o + ((int64_t)seg.part + g) * D + x2;
 #pragma unroll
-            for (int x = 0; x < D / 8; ++x) {
-                if (g < seg.rows) *reinterpret_cast<float2 *>(to + 8 * x) = make_float2(o[x][0], o[x][1]);
-                if (g + 8 < seg.rows) *reinterpret_cast<float2 *>(to + 8 * D + 8 * x) = make_float2(o[x][2], o[x][3]);
+            for (int x = 4; x <= 16; x <<= 1) {
+                l0 += __shfl_xor_sync(0xffffffffu, l0, x);
+                l1 += __shfl_xor_sync(0xffffffffu, l1, x);
             }
-            if (x2 == 0) {
-                if (g < seg.rows) call.ml[seg.part + g] = make_float2(m0, l0);
-                if (g + 8 < seg.rows) call.ml[seg.part + g + 8] = make_float2(m1, l1);
+            float *to = call.o + ((int64_t)seg.part + x2) * D + g;
+#pragma unroll
+            for (int x = 0; x < D / 16; ++x) {
+                if (x2 < seg.rows) { to[16 * x] = o[x][0]; to[16 * x + 8] = o[x][2]; }
+                if (x2 + 1 < seg.rows) { to[D + 16 * x] = o[x][1]; to[D + 16 * x + 8] = o[x][3]; }
+            }
+            if (g == 0) {
+                if (x2 < seg.rows) call.ml[seg.part + x2] = make_float2(m0, l0);
+                if (x2 + 1 < seg.rows) call.ml[seg.part + x2 + 1] = make_float2(m1, l1);
             }
         }
     }
