@@ -230,6 +230,19 @@ template <typename T, int D> __global__ void __launch_bounds__(256) prefix_join_
             const int x = x0 + lane, count = min(32, n_all - x0);
             const int part = (int)(x < n_shared ? shared0 + (int64_t)x * sh.row_tile : own0 + (int64_t)(x - n_shared) * sh.own_slot());
             const float2 ml = lane < count ? call.ml[part] : make_float2(-INFINITY, 0.0f);
+            // four outputs at a time on their way, the first of them beside the maxima
+            float v[4][V];
+            auto fetch = [&](int y0) {
+#pragma unroll
+                for (int y = 0; y < 4; ++y) {
+                    const float *o = call.o + (int64_t)__shfl_sync(0xffffffffu, part, (y0 + y) & 31) * D + V * lane;
+                    if (y0 + y < count) {
+                        if constexpr (V == 4) *reinterpret_cast<float4 *>(v[y]) = *reinterpret_cast<const float4 *>(o);
+                        else *reinterpret_cast<float2 *>(v[y]) = *reinterpret_cast<const float2 *>(o);
+                    }
+                }
+            };
+            fetch(0);
             float big = fmaxf(m, ml.x);
 #pragma unroll
             for (int k = 16; k > 0; k >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, k));
@@ -242,15 +255,15 @@ template <typename T, int D> __global__ void __launch_bounds__(256) prefix_join_
             m = big;
 #pragma unroll
             for (int i = 0; i < V; ++i) acc[i] = x0 ? __fmul_rn(acc[i], f) : 0.0f;
-#pragma unroll 4
-            for (int y = 0; y < count; ++y) {
-                const float wy = __shfl_sync(0xffffffffu, w, y);
-                const float *o = call.o + (int64_t)__shfl_sync(0xffffffffu, part, y) * D + V * lane;
-                float v[V];
-                if constexpr (V == 4) *reinterpret_cast<float4 *>(v) = *reinterpret_cast<const float4 *>(o);
-                else *reinterpret_cast<float2 *>(v) = *reinterpret_cast<const float2 *>(o);
+            for (int y0 = 0; y0 < count; y0 += 4) {
+                if (y0) fetch(y0);
 #pragma unroll
-                for (int i = 0; i < V; ++i) acc[i] = __fmaf_rn(wy, v[i], acc[i]);
+                for (int y = 0; y < 4; ++y) {
+                    const float wy = __shfl_sync(0xffffffffu, w, (y0 + y) & 31);
+                    if (y0 + y < count)
+#pragma unroll
+                        for (int i = 0; i < V; ++i) acc[i] = __fmaf_rn(wy, v[y][i], acc[i]);
+                }
             }
         }
     }

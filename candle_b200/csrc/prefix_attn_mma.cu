@@ -393,12 +393,21 @@ template <int D> struct Loader {
             const int64_t at = (int64_t)(((id * kv_heads + seg.head) << shift) + (key & (st.page - 1))) * (D * 2);
             const uint8_t *ks = k + at, *vs = v + at;
             const uint32_t vt = to + (uint32_t)sizeof(Step<D>) / 2;
+            if (n >= kStep) {
 #pragma unroll
-            for (int i = 0; i < kPieces; ++i) {
-                const uint32_t o = off[i % kPeriod] + i / kPeriod * 1024;
-                const int bytes = lane / (D / 8) + i * kRows < n ? 16 : 0;
-                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + o), "l"(ks + i * 512), "r"(bytes) : "memory");
-                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(vt + o), "l"(vs + i * 512), "r"(bytes) : "memory");
+                for (int i = 0; i < kPieces; ++i) {
+                    const uint32_t o = off[i % kPeriod] + i / kPeriod * 1024;
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + o), "l"(ks + i * 512) : "memory");
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(vt + o), "l"(vs + i * 512) : "memory");
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < kPieces; ++i) {
+                    const uint32_t o = off[i % kPeriod] + i / kPeriod * 1024;
+                    const int bytes = lane / (D / 8) + i * kRows < n ? 16 : 0;
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + o), "l"(ks + i * 512), "r"(bytes) : "memory");
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(vt + o), "l"(vs + i * 512), "r"(bytes) : "memory");
+                }
             }
             ++step;
         }
