@@ -10,7 +10,21 @@ using namespace cq_attn;
 using cq_kv::State;
 
 constexpr int kThreads = 256, kPlanCtas = 8;
-constexpr int kOwnLeast = 1;            // units of an own segment, at least
+
+// Units per worker of the own line.  f16 and bf16: the four warps of a CTA that have nothing else, and the eight that come when its `units` shared ones are done.  In clocks
+// of a B200 SM: a shared unit takes 4,300 and the first of them 5,000 more, one of the four warps takes 2,800 a step beside them, and twelve warps together are bound by
+// HBM with 400 a step.  All finish together by that; a model that is off by a third leaves the one kind of warps idle for a tenth of the time.
+__device__ __forceinline__ void own_chunks(const Shape &s, int units, int line, int &chunk, int &chunk2) {
+    chunk2 = 1;
+    if (s.own_first == s.own_workers) { chunk = max((line + s.own_workers - 1) / s.own_workers, 1); return; }
+    const int per_cta = (line + s.ctas - 1) / s.ctas;
+    const int beside = units ? (int)min(((int64_t)units * 4300 + 5000) / 2800, (int64_t)per_cta) : 0;          // steps a warp does in that time
+    const int rest = per_cta - kMmaWarps * beside;
+    if (rest <= 0) { chunk = max((per_cta + kMmaWarps - 1) / kMmaWarps, 1); return; }
+    const int share = (rest + kMmaWarps + kMmaHelpers - 1) / (kMmaWarps + kMmaHelpers);
+    chunk = beside + share;
+    chunk2 = share;
+}
 
 // Sum of `v` over the threads before this one, two counts in one 64-bit word; `total` over all.
 __device__ __forceinline__ uint64_t scan_before(uint64_t v, uint64_t *sums, uint64_t &total) {
@@ -137,7 +151,9 @@ __global__ void __launch_bounds__(kThreads) prefix_plan_kernel(const cq_kv_cache
     }
     __syncthreads();
     const int shared_line = (int)(before >> 32), own_line = (int)(uint32_t)before;
-    const int chunk = max((shared_line + sh.ctas - 1) / sh.ctas, 1), own_chunk = max((own_line + sh.own_workers - 1) / sh.own_workers, kOwnLeast);
+    const int chunk = max((shared_line + sh.ctas - 1) / sh.ctas, 1);
+    int own_chunk, own_chunk2;
+    own_chunks(sh, shared_line ? chunk : 0, own_line, own_chunk, own_chunk2);
     auto group_at = [&](int g) {
         const GroupShape gs = pl.shapes[g];
         const int shared = shared_of(g);
@@ -149,9 +165,10 @@ __global__ void __launch_bounds__(kThreads) prefix_plan_kernel(const cq_kv_cache
     for (int i = tid * kPlanCtas + rank; i < workers + nq + sh.groups; i += kPlanCtas * kThreads) {
         if (i < workers) {
             const bool own = i >= sh.ctas;
-            const int w = own ? i - sh.ctas : i, u = w * (own ? own_chunk : chunk);
+            const int w = own ? i - sh.ctas : i, later = w - sh.own_first;
+            const int u = !own ? w * chunk : later < 0 ? w * own_chunk : sh.own_first * own_chunk + later * own_chunk2;
             Start st{};
-            st.left = own ? min(own_line - u, own_chunk) : min(shared_line - u, chunk);
+            st.left = own ? min(own_line - u, later < 0 ? own_chunk : own_chunk2) : min(shared_line - u, chunk);
             if (st.left > 0) {
                 // the last group (query) that begins here or before; those without units begin where the next one does
                 const int *starts = own ? start_of : group_start;
@@ -194,7 +211,7 @@ __global__ void __launch_bounds__(kThreads) prefix_plan_kernel(const cq_kv_cache
             pl.query[x] = q;
         } else pl.groups[i - workers - nq] = group_at(i - workers - nq);
     }
-    if (rank == 0 && tid == 0) { pl.header[0] = shared_line; pl.header[1] = chunk; pl.header[2] = own_line; pl.header[3] = own_chunk; }
+    if (rank == 0 && tid == 0) { pl.header[0] = shared_line; pl.header[1] = chunk; pl.header[2] = own_line; pl.header[3] = own_chunk; pl.header[4] = own_chunk2; }
 }
 
 // One warp per row: lane x weighs segment x - those of the row's shared item, then those of its own one, in the order of their keys - and the
@@ -209,14 +226,14 @@ template <typename T, int D> __global__ void __launch_bounds__(256) prefix_join_
     const int h = div_per(hq, sh), in = hq - h * per, tile = in / sh.own_rows;          // own_rows: 8 or 32
     const int64_t row = (int64_t)n * sh.heads + hq;
     const Query q = pl.query[n];
-    const int chunk = pl.header[1], own_chunk = pl.header[3];
+    const int chunk = pl.header[1], own_chunk = pl.header[3], own_chunk2 = pl.header[4];
     constexpr int V = D / 32;
     float acc[V] = {}, m = -INFINITY, l = 0.0f;
     if (q.len > 0) {
         // segments of an item: its units [start, start + units) of the line, cut at multiples of the chunk
         const int local = h * sh.own_tiles + tile, own_item = n * sh.kv_heads * sh.own_tiles + local;
-        const int own_start = q.start + local * q.units, own_w = own_start / own_chunk;
-        const int n_own = q.units ? (own_start + q.units - 1) / own_chunk - own_w + 1 : 0;
+        const int own_start = q.start + local * q.units, own_w = own_worker(sh, own_start, own_chunk, own_chunk2);
+        const int n_own = q.units ? own_worker(sh, own_start + q.units - 1, own_chunk, own_chunk2) - own_w + 1 : 0;
         int n_shared = 0;
         int64_t shared0 = 0;
         if (q.shared) {
@@ -296,8 +313,8 @@ bool shape_ok(const cq_kv_cache *cache, const cq_prefix_plan *p, const char *who
         status = CQ_ERR_UNSUPPORTED;
         if ((int64_t)p->batch * p->queries > 4096) why = "at most 4096 queries (batch * queries)";
         else if (p->heads / cache->kv_heads > 32) why = "at most 32 query heads per KV head";
-        else if ((int64_t)p->batch * p->queries * p->heads * ((int64_t)cache->max_pages * cache->page_size / 16 + 1) > INT32_MAX)
-            why = "more than 2^35 (query head, key) pairs in one call";
+        else if ((int64_t)p->batch * p->queries * p->heads * ((int64_t)cache->max_pages * cache->page_size / 16 + 1) > (1 << 30))
+            why = "more than 2^34 (query head, key) pairs in one call";
     }
     if (why) {
         std::snprintf(msg, sizeof msg, "%s: %s", who, why);
@@ -306,8 +323,8 @@ bool shape_ok(const cq_kv_cache *cache, const cq_prefix_plan *p, const char *who
     }
     s = Shape{p->batch, p->queries, p->heads, cache->kv_heads, p->groups, cache->head_dim, cache->elem, p->heads / cache->kv_heads};
     s.ctas = p->ctas;
-    if (cache->elem == CQ_F32) { s.row_tile = s.own_rows = 32; s.own_shift = 6; s.own_workers = s.ctas; }
-    else { s.row_tile = 256; s.own_rows = 8; s.own_shift = 4; s.own_workers = s.ctas * kMmaWarps; }
+    if (cache->elem == CQ_F32) { s.row_tile = s.own_rows = 32; s.own_shift = 6; s.own_workers = s.own_first = s.ctas; }
+    else { s.row_tile = 256; s.own_rows = 8; s.own_shift = 4; s.own_first = s.ctas * kMmaWarps; s.own_workers = s.own_first + s.ctas * kMmaHelpers; }
     s.own_tiles = (s.per_kv + s.own_rows - 1) / s.own_rows;
     if (s.per_kv > 1) s.rcp = (unsigned)(((1ull << 32) + s.per_kv - 1) / s.per_kv);
     return true;
@@ -338,7 +355,8 @@ extern "C" int cq_prefix_plan_shape(const cq_kv_cache *cache, cq_prefix_plan *pl
     Shape s;
     if (!shape_ok(cache, plan, "prefix_plan_shape", s)) return 1;
     s.ctas = plan->ctas = (s.elem == CQ_F32 ? 2 : 1) * cq_sm_count();
-    s.own_workers = s.elem == CQ_F32 ? s.ctas : s.ctas * kMmaWarps;
+    s.own_first = s.elem == CQ_F32 ? s.ctas : s.ctas * kMmaWarps;
+    s.own_workers = s.own_first + (s.elem == CQ_F32 ? 0 : s.ctas * kMmaHelpers);
     int64_t items = 0, seqs = 0;
     for (int g = 0; g < plan->groups; ++g) {
         const int n = group_sizes ? group_sizes[g] : plan->groups == 1 ? plan->batch : 1;

@@ -4,7 +4,7 @@
 // rows of consecutive sequences are consecutive.  Two kinds of items cover all (row, key) pairs:
 //   shared : up to `row_tile` rows of one group of sequences x one KV head x the keys of the pages that all of them share;
 //   own    : up to `own_rows` rows of one query x one KV head x the keys behind these pages.
-// An item is a number of units (64 keys of a shared item, 2^own_shift keys of an own one); the units of all items of a kind form a line, which
+// An item is a number of units (128 keys of a shared item, 2^own_shift keys of an own one); the units of all items of a kind form a line, which
 // its workers (CTAs for the shared items; CTAs or warps for the own ones) take in equal parts.  A part of an item that one worker takes
 // is a segment; it leaves (maximum, sum, unnormalised output) per row, and a second kernel joins a row's segments in the order of their keys:
 // m = max m_i,  l = sum 2^(m_i - m) l_i,  o = sum 2^(m_i - m) o_i / l.
@@ -13,7 +13,7 @@
 
 namespace cq_attn {
 
-constexpr int kKeyTile = 64;        // keys of a shared unit
+constexpr int kKeyTile = 128;       // keys of a shared unit
 
 struct Segment {
     int row0, rows;         // rows of the KV head
@@ -38,7 +38,8 @@ struct GroupShape { int query0, rows, item0, row_tiles; };
 
 struct Shape {
     int batch, queries, heads, kv_heads, groups, head_dim, elem, per_kv;
-    int row_tile, ctas, own_rows, own_shift, own_workers;       // 2^own_shift keys an own unit
+    int row_tile, ctas, own_rows, own_shift;                    // 2^own_shift keys an own unit
+    int own_workers, own_first;                                 // workers of the own line; the first own_first have chunks of one size, the others of another
     int own_tiles;          // row tiles of a KV head's query heads
     unsigned rcp;           // ceil(2^32 / query heads per KV head); 0 for one
     __host__ __device__ int n_queries() const { return batch * queries; }
@@ -48,7 +49,7 @@ struct Shape {
 
 // The plan's ints.
 struct Plan {
-    int *header;            // units of the shared line, units per CTA; units of the own line, units per worker
+    int *header;            // units of the shared line, units per CTA; units of the own line, per worker of the first and of the second kind
     GroupShape *shapes;     // [groups], written by the host's part of the plan
     Group *groups;
     Query *query;
@@ -81,6 +82,12 @@ inline int64_t plan_ints(const Shape &s) {
     int64_t n;
     (void)plan_of((int *)nullptr, s, &n);
     return n;
+}
+
+// Which worker has unit u of the own line.
+__host__ __device__ inline int own_worker(const Shape &s, int u, int chunk, int chunk2) {
+    const int first = s.own_first * chunk;
+    return u < first ? u / chunk : s.own_first + (u - first) / chunk2;
 }
 
 // First row of the partial results of segment (item, worker) of a kind, at = item + worker: that sum is another one for every segment of a line.
@@ -167,6 +174,6 @@ __device__ __forceinline__ int div_per(int n, const Shape &s) { return s.rcp ? (
 // The kernels that make the segments' results (prefix_attn_simt.cu: f32; prefix_attn_mma.cu: f16 and bf16).
 void simt_launch(const Call &c, const cq_kv_cache &cache, int layer, const void *q, int64_t q_stride, float scale, cudaStream_t st);
 bool mma_launch(const Call &c, const cq_kv_cache &cache, int layer, const void *q, int64_t q_stride, float scale, cudaStream_t st);
-constexpr int kMmaWarps = 4;            // warps of a CTA of the latter that are workers of the own line
+constexpr int kMmaWarps = 4, kMmaHelpers = 8;       // warps of a CTA of the latter that are workers of the own line from the start, and after the shared items
 
 }  // namespace cq_attn

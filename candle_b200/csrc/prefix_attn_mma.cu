@@ -1,12 +1,13 @@
 // Segments of the shared-prefix attention (prefix_attn.cuh) on the tensor cores: f16 and bf16 caches.
 //
-// Shared items (many rows, keys mostly from L2): tiles of 2 x 128 rows x 64 keys by tcgen05.  S = Q K^T goes to tensor memory; thread r of a
+// Shared items (many rows, keys mostly from L2): tiles of 2 x 128 rows x 128 keys by tcgen05.  S = Q K^T goes to tensor memory; thread r of a
 // half's softmax warps owns row r, reads it there, and writes the weights 2^(s c - m), c = scale log2 e, back over it in 16 bits as the first operand of
-// O += P V.  512 columns: for each half the scores of two tiles, so that one tile's softmax has the products of its neighbours beside it, and the outputs.
+// O += P V.  512 columns, a half's scores and outputs twice: one half's softmax has the other's products beside it.
 //
 // Own items (as many rows as a KV head has query heads, keys from HBM): a warp is a worker of its own, 16 rows x 16 keys a step by mma.sync, with its
 // next steps of keys and values on their way.  Through the first form an item of four rows costs the waits of a whole tile chain - QK, softmax, PV, some
-// 10,000 clocks for 64 KB - where HBM gives an SM 64 KB in 2,850.  These warps run beside the others all the time, so that HBM and tensor cores are both in use.
+// 10,000 clocks for 64 KB - where HBM gives an SM 64 KB in 2,850.  Four such warps run beside the others, so that HBM and tensor
+// cores are both in use, and the softmax warps join them when the shared items are done.
 //
 // In both m is the row's maximum so far, kept until a score passes it by 2^8 (weights up to 256 are as good as any, the sum has the same
 // factor), so that outputs are scaled in the first tiles only.  The sum adds the weights as rounded: rounding moves weight between keys but
@@ -23,21 +24,23 @@ using namespace cq_attn;
 using namespace cq_prompt;
 
 // Warps: 0-3 and 4-7 softmax of a row tile's halves, 8 copies, 9 products, 12-15 own items.
-constexpr int kThreads = 512, kCopyWarp = 8, kMmaWarp = 9, kOwnWarp = 12;
-constexpr int kKvStages = 3, kCols = 512;
+constexpr int kThreads = 512, kCopyWarp = kMmaHelpers, kMmaWarp = 9, kOwnWarp = 12;
+constexpr int kRing = 3, kCols = 512;                        // buffers that hold K, V, K, V, ... of the tiles in turn
 constexpr int kHalfBytes = 128 * 128;                        // 128 rows of 64 elements
-constexpr int kGroup = 256, kO = 128;                        // columns of a half; in it the scores / weights of two tiles and the outputs
+constexpr int kGroup = 256, kO = 128;                        // columns of a half; in it the scores / weights and the outputs
 constexpr int kStep = 16;                                    // keys of a step of an own item
-// registers a thread by warpgroup: 128 * (144 + 144 + 64 + 160) is what the block was launched with, 512 * 128
-constexpr int kRegsSoft = 144, kRegsMisc = 64, kRegsOwn = 160;
+// registers a thread by warpgroup: 128 * (160 + 160 + 64 + 128) is what the block was launched with, 512 * 128
+constexpr int kRegsSoft = 160, kRegsMisc = 64, kRegsOwn = 128;
+static_assert(kCopyWarp == 8 && kMmaWarps == 4, "warp roles");
+static_assert(2 * kRegsSoft + kRegsMisc + kRegsOwn == 512 && kRegsSoft >= 128 && kRegsOwn >= 128 && kRegsMisc <= 128, "setmaxnreg: up only from 128, down only from 128");
 
 template <int D> struct Step { uint8_t k[D / 64][kStep * 128], v[D / 64][kStep * 128]; };
 template <int D> struct Tiles {
     static constexpr int kStages = D == 64 ? 4 : 2;          // steps of an own warp: 64 KB for four of them
-    uint8_t q[2][D / 64][kHalfBytes], k[kKvStages][D / 64][kKeyTile * 128], v[kKvStages][D / 64][kKeyTile * 128];
+    uint8_t q[2][D / 64][kHalfBytes], kv[kRing][D / 64][kHalfBytes];
     Step<D> step[kMmaWarps][kStages];
-    // operands there; K, V free; by half and buffer: scores there, weights there, weights read and outputs there
-    uint64_t q_bar[2], k_bar[kKvStages], v_bar[kKvStages], k_free[kKvStages], v_free[kKvStages], s_bar[2][2], p_bar[2][2], o_bar[2][2];
+    uint64_t full[kRing], free[kRing];
+    uint64_t q_bar[2], s_bar[2], p_bar[2], o_bar[2];         // by half: rows there, scores there, weights there, outputs there
     uint32_t tmem;
     int abort;
 };
@@ -62,26 +65,32 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&v)[16
                  ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]),
                  "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]) : "memory");
 }
-__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&v)[16]) {
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
-                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]),
-                   "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]) : "r"(taddr) : "memory");
-}
 __device__ __forceinline__ float ex2(float x) {
     float r;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
 }
-// two weights in the type's 16 bits, and their sum as rounded
-template <bool BF16> __device__ __forceinline__ uint32_t pack(float a, float b, float &sum) {
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+// 2^x of two exponents in the type's 16 bits; `sum` adds them as rounded
+template <bool BF16> __device__ __forceinline__ uint32_t weights(uint64_t x, uint64_t &sum) {
+    const float a = ex2(__uint_as_float((uint32_t)x)), b = ex2(__uint_as_float((uint32_t)(x >> 32)));
     uint32_t w;
     if constexpr (BF16) {
         asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(b), "f"(a));
-        sum += __uint_as_float(w << 16) + __uint_as_float(w & 0xffff0000u);
+        sum = add2(sum, pack2(w << 16, w & 0xffff0000u));
     } else {
         asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(b), "f"(a));
         const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w));
-        sum += f.x + f.y;
+        sum = add2(sum, pack2f(f.x, f.y));
     }
     return w;
 }
@@ -95,8 +104,7 @@ __device__ __forceinline__ void expect_tx(uint32_t bar, uint32_t bytes) {
 }
 
 // ---- shared items ----
-// Buffers are used in turn: use n of one of N goes to n % N, and waits for the phase that use n - N has completed.  Every barrier belongs to one buffer, so no
-// waiter can fall two phases behind.
+// No waiter can fall two phases behind its barrier: what completes the next phase needs what the waiter does after the wait.
 
 // Softmax of one half of the row tiles.  False: a wait gave up.
 template <int D, bool BF16>
@@ -124,14 +132,12 @@ __device__ bool softmax_part(Tiles<D> &sm, const Call &call, const CUtensorMap &
         float m = -INFINITY, l = 0.0f;
         for (int j = 0; j < seg.units; ++j, ++tile) {
             const int n = seg.key1 - seg.key0 - j * kKeyTile;          // keys of this tile, if fewer than kKeyTile
-            const unsigned b = tile & 1, phase = tile >> 1 & 1;
-            const uint32_t sp = mine + b * kKeyTile;
-            if (!wait_warp(&sm.s_bar[half][b], phase, abort_flag)) return false;
+            if (!wait_warp(&sm.s_bar[half], tile & 1, abort_flag)) return false;
             tc_fence_after();
             if (active) {
-                uint32_t s[2][32];
-                tmem_ld32(sp, s[0]);
-                tmem_ld32(sp + 32, s[1]);
+                uint32_t s[kKeyTile / 32][32];
+#pragma unroll
+                for (int x = 0; x < kKeyTile / 32; ++x) tmem_ld32(mine + 32 * x, s[x]);
                 tmem_ld_wait();
                 if (n < kKeyTile) {
 #pragma unroll
@@ -140,7 +146,10 @@ __device__ bool softmax_part(Tiles<D> &sm, const Call &call, const CUtensorMap &
                 }
                 float mx = -INFINITY, my = -INFINITY;
 #pragma unroll
-                for (int i = 0; i < 32; ++i) { mx = fmaxf(mx, __uint_as_float(s[0][i])); my = fmaxf(my, __uint_as_float(s[1][i])); }
+                for (int i = 0; i < kKeyTile; i += 4) {
+                    mx = max3(mx, __uint_as_float(s[i >> 5][i & 31]), __uint_as_float(s[i >> 5][(i & 31) + 1]));
+                    my = max3(my, __uint_as_float(s[i >> 5][(i & 31) + 2]), __uint_as_float(s[i >> 5][(i & 31) + 3]));
+                }
                 mx = fmaxf(mx, my) * c;
                 if (j == 0) m = mx;
                 else {
@@ -149,46 +158,43 @@ __device__ bool softmax_part(Tiles<D> &sm, const Call &call, const CUtensorMap &
                         const float f = up ? ex2(m - mx) : 1.0f;
                         if (up) m = mx;
                         l *= f;
-                        if (!wait_warp(&sm.o_bar[half][b ^ 1], (tile - 1) >> 1 & 1, abort_flag)) return false;        // the outputs so far
-                        tc_fence_after();
-#pragma unroll
-                        for (int x = 0; x < D / 16; ++x) {
-                            uint32_t o[16];
-                            tmem_ld16(mine + kO + 16 * x, o);
+#pragma unroll 1
+                        for (int x = 0; x < D / 8; ++x) {           // QK of this tile has waited for the outputs so far
+                            uint32_t o[8];
+                            tmem_ld8(mine + kO + 8 * x, o);
                             tmem_ld_wait();
 #pragma unroll
-                            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-                            tmem_st16(mine + kO + 16 * x, o);
+                            for (int i = 0; i < 8; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+                            tmem_st8(mine + kO + 8 * x, o);
                         }
                     }
                 }
                 const float base = m == -INFINITY ? 0.0f : m;
-                float sum0 = 0.0f, sum1 = 0.0f;
+                const uint64_t c2 = pack2f(c, c), base2 = pack2f(-base, -base);
+                uint64_t sum = 0;
 #pragma unroll
-                for (int x = 0; x < 4; ++x) {
-                    uint32_t w[8];
+                for (int x = 0; x < kKeyTile / 32; ++x) {
+                    uint32_t w[16];
 #pragma unroll
-                    for (int i = 0; i < 8; ++i)
-                        w[i] = pack<BF16>(ex2(__fmaf_rn(__uint_as_float(s[x >> 1][16 * (x & 1) + 2 * i]), c, -base)),
-                                          ex2(__fmaf_rn(__uint_as_float(s[x >> 1][16 * (x & 1) + 2 * i + 1]), c, -base)), i & 1 ? sum1 : sum0);
-                    tmem_st8(sp + 8 * x, w);                // over the scores
+                    for (int i = 0; i < 16; ++i) w[i] = weights<BF16>(fma2(pack2(s[x][2 * i], s[x][2 * i + 1]), c2, base2), sum);
+                    tmem_st16(mine + 16 * x, w);            // over scores that have been read
                 }
-                l += sum0 + sum1;
+                l += __uint_as_float((uint32_t)sum) + __uint_as_float((uint32_t)(sum >> 32));
                 tmem_st_wait();
                 tc_fence_before();
             }
             if (n < kKeyTile && half == 0) {                // before either half's product: the second follows the first
-                const unsigned stage = tile % kKvStages;    // the first half has a part in every tile
-                if (!wait_warp(&sm.v_bar[stage], tile / kKvStages & 1, abort_flag)) return false;
+                const unsigned v = 2 * tile + 1, buf = v % kRing;       // the first half has a part in every tile
+                if (!wait_warp(&sm.full[buf], v / kRing & 1, abort_flag)) return false;
                 for (int i = tid; i < (kKeyTile - n) * (D / 8); i += 128) {
                     const int r = n + i / (D / 8), x = i % (D / 8);
-                    *reinterpret_cast<uint4 *>(&sm.v[stage][x >> 3][r * 128 + (x & 7) * 16]) = make_uint4(0, 0, 0, 0);
+                    *reinterpret_cast<uint4 *>(&sm.kv[buf][x >> 3][r * 128 + (x & 7) * 16]) = make_uint4(0, 0, 0, 0);
                 }
                 fence_proxy_async_smem();
             }
-            arrive_warp(&sm.p_bar[half][b], lane);
+            arrive_warp(&sm.p_bar[half], lane);
         }
-        if (!wait_warp(&sm.o_bar[half][(tile - 1) & 1], (tile - 1) >> 1 & 1, abort_flag)) return false;
+        if (!wait_warp(&sm.o_bar[half], (tile - 1) & 1, abort_flag)) return false;
         tc_fence_after();
         if (active) {
             // The outputs go out as 32 x 32 boxes of 128-byte rows, one warp's each, from where Q was.  (Stored by their threads, a row each, they
@@ -225,46 +231,41 @@ __device__ bool softmax_part(Tiles<D> &sm, const Call &call, const CUtensorMap &
 
 template <int D>
 __device__ bool copy_part(Tiles<D> &sm, const cq_kv_cache &cache, const cq_kv::State &st, const Call &call, const CUtensorMap &k_map, const CUtensorMap &v_map) {
-    const int lane = threadIdx.x & 31, page = st.page, shift = 31 - __clz(page), box = min(page, kKeyTile), boxes = page < kKeyTile ? D / 64 : 1;
+    const int lane = threadIdx.x & 31, page = st.page, shift = 31 - __clz(page), boxes = page < kKeyTile ? D / 64 : 1;
     volatile int *abort_flag = &sm.abort;
     SharedWalk walk(call, blockIdx.x);
     Segment seg;
-    unsigned tile = 0, stage = 0, phase = 1;        // phase: of the use before
+    unsigned buf = 0, phase = 1, sent = 0;          // phase: of the use before
     bool ok = true;
     while (ok && walk.next(call, seg)) {
         const int *table = st.tables + (size_t)seg.slot * st.max_pages;
         int base = INT32_MIN / 2, ids = -1;             // page numbers base .. base + 31 of the table, one a lane
-        for (int j = 0; j < seg.units; ++j, ++tile) {
-            const int key = seg.key0 + j * kKeyTile, mine = key + lane * box;
+        for (int j = 0; ok && j < seg.units; ++j) {
+            const int key = seg.key0 + j * kKeyTile, mine = key + lane * page;
             if (((key + kKeyTile - 1) >> shift) - base >= 32) {
                 base = key >> shift;
                 ids = (base + lane) << shift < seg.key1 ? table[base + lane] : -1;
             }
-            int id = __shfl_sync(0xffffffffu, ids, ((mine >> shift) - base) & 31);           // a lane takes a box
-            if (lane * box >= kKeyTile || mine >= seg.key1) id = -1;
+            int id = __shfl_sync(0xffffffffu, ids, ((mine >> shift) - base) & 31);           // a lane takes a page
+            if (lane * page >= kKeyTile || mine >= seg.key1) id = -1;
             else if (id < 0 || id >= st.pages) { id = -1; atomicCAS(st.header, cq_kv::kOk, cq_kv::kBadPage); }
-            const unsigned bytes = (unsigned)__popc(__ballot_sync(0xffffffffu, id >= 0)) * box * D * 2;
-            const int y = ((id * cache.kv_heads + seg.head) << shift) + (mine & (page - 1));
-            if (tile >= kKvStages && !(ok = wait_warp(&sm.k_free[stage], phase, abort_flag))) break;
-            if (lane == 0) expect_tx(cq_smem_u32(&sm.k_bar[stage]), bytes);
-            __syncwarp();
-            if (id >= 0)
-                for (int h = 0; h < boxes; ++h) load_3d(cq_smem_u32(&sm.k[stage][h][lane * box * 128]), &k_map, 0, y, h, cq_smem_u32(&sm.k_bar[stage]));
-            if (tile >= kKvStages && !(ok = wait_warp(&sm.v_free[stage], phase, abort_flag))) break;
-            if (lane == 0) expect_tx(cq_smem_u32(&sm.v_bar[stage]), bytes);
-            __syncwarp();
-            if (id >= 0)
-                for (int h = 0; h < boxes; ++h) load_3d(cq_smem_u32(&sm.v[stage][h][lane * box * 128]), &v_map, 0, y, h, cq_smem_u32(&sm.v_bar[stage]));
-            if (++stage == kKvStages) { stage = 0; phase ^= 1; }
+            const unsigned bytes = (unsigned)__popc(__ballot_sync(0xffffffffu, id >= 0)) * page * D * 2;
+            const int y = (id * cache.kv_heads + seg.head) << shift;
+            for (int kind = 0; kind < 2; ++kind) {
+                if (sent >= kRing && !(ok = wait_warp(&sm.free[buf], phase, abort_flag))) break;
+                const uint32_t bar = cq_smem_u32(&sm.full[buf]);
+                if (lane == 0) expect_tx(bar, bytes);
+                __syncwarp();
+                if (id >= 0)
+                    for (int h = 0; h < boxes; ++h) load_3d(cq_smem_u32(&sm.kv[buf][h][lane * page * 128]), kind ? &v_map : &k_map, 0, y, h, bar);
+                ++sent;
+                if (++buf == kRing) { buf = 0; phase ^= 1; }
+            }
         }
     }
-    if (!ok)                        // leaving early: not before what is on its way has come (a copy that was never sent costs the wait's bound)
-        for (unsigned b = 0; b < kKvStages; ++b)
-            if (tile >= b) {
-                const unsigned last = (tile - b) / kKvStages & 1;          // phase of the newest copy that may be out
-                (void)(cq_mbar_wait_bounded(&sm.k_bar[b], last ^ 1) && cq_mbar_wait_bounded(&sm.k_bar[b], last));
-                (void)(cq_mbar_wait_bounded(&sm.v_bar[b], last ^ 1) && cq_mbar_wait_bounded(&sm.v_bar[b], last));
-            }
+    if (!ok)                        // leaving early: not before what is on its way has come
+        for (unsigned b = 0; b < kRing; ++b)
+            if (sent > b) (void)cq_mbar_wait_bounded(&sm.full[b], (sent - 1 - b) / kRing & 1);
     return ok;
 }
 
@@ -272,69 +273,68 @@ template <int D, bool BF16> __device__ bool mma_part(Tiles<D> &sm, const Call &c
     constexpr uint32_t kTypes = BF16 ? (1u << 7) | (1u << 10) : 0u;
     constexpr uint32_t kIdescQK = (1u << 4) | kTypes | ((uint32_t)kKeyTile >> 3) << 17 | (128u >> 4) << 24;
     constexpr uint32_t kIdescPV = (1u << 4) | kTypes | (1u << 16) | ((uint32_t)D >> 3) << 17 | (128u >> 4) << 24;
-    constexpr uint32_t kHalfK = kKeyTile * 128 >> 4, kBuf = D / 64 * kHalfK, kQ = D / 64 * (kHalfBytes >> 4);
-    const uint32_t qa = uniform(cq_smem_u32(&sm.q[0][0][0]) >> 4), ka = uniform(cq_smem_u32(&sm.k[0][0][0]) >> 4), va = uniform(cq_smem_u32(&sm.v[0][0][0]) >> 4);
-    const uint32_t t0 = uniform(sm.tmem);
+    constexpr uint32_t kBlock = kHalfBytes >> 4, kBuf = D / 64 * kBlock;
+    const uint32_t qa = uniform(cq_smem_u32(&sm.q[0][0][0]) >> 4), kva = uniform(cq_smem_u32(&sm.kv[0][0][0]) >> 4), t0 = uniform(sm.tmem);
     volatile int *abort_flag = &sm.abort;
     SharedWalk walk(call, blockIdx.x);
     Segment seg;
-    unsigned segments[2] = {0, 0}, qk[2] = {0, 0}, pv[2] = {0, 0};          // by half: segments, products under way
-    unsigned k_stage = 0, k_phase = 0, v_stage = 0, v_phase = 0;
-    auto scores = [&](int halves) {             // S = Q K^T of the next tile
-        if (!wait_warp(&sm.k_bar[k_stage], k_phase, abort_flag)) return false;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            if (h >= halves) break;
-            const unsigned b = qk[h] & 1;
-            if (qk[h] >= 2 && !wait_warp(&sm.o_bar[h][b], (qk[h] >> 1 & 1) ^ 1, abort_flag)) return false;          // the weights there have been read
-            tc_fence_after();
-            if (elect_one()) {
-#pragma unroll
-                for (int x = 0; x < D / 16; ++x)
-                    mma_ss(t0 + h * kGroup + b * kKeyTile, qa + h * kQ + (x >> 2) * (kHalfBytes >> 4) + (x & 3) * 2, ka + k_stage * kBuf + (x >> 2) * kHalfK + (x & 3) * 2,
-                           kIdescQK, x > 0);
-                tc_commit(&sm.s_bar[h][b]);
-                if (h == halves - 1) tc_commit(&sm.k_free[k_stage]);
-            }
-            __syncwarp();
-            ++qk[h];
-        }
-        if (++k_stage == kKvStages) { k_stage = 0; k_phase ^= 1; }
-        return true;
-    };
+    unsigned segments[2] = {0, 0}, tiles[2] = {0, 0}, done[2] = {0, 0};             // by half: segments, tiles with QK, with PV under way
+    unsigned buf = 0, phase = 0;
     bool ok = true;
+    auto advance = [&]() { if (++buf == kRing) { buf = 0; phase ^= 1; } };
+    // S = Q K^T of the tile in `buf` for half h; the last half sets the buffer free
+    auto scores = [&](int h, bool last) {
+        if (elect_one()) {
+#pragma unroll
+            for (int x = 0; x < D / 16; ++x)
+                mma_ss(t0 + h * kGroup, qa + h * kBuf + (x >> 2) * kBlock + (x & 3) * 2, kva + buf * kBuf + (x >> 2) * kBlock + (x & 3) * 2, kIdescQK, x > 0);
+            tc_commit(&sm.s_bar[h]);
+            if (last) tc_commit(&sm.free[buf]);
+        }
+        __syncwarp();
+        ++tiles[h];
+    };
     while (ok && walk.next(call, seg)) {
         const int units = (int)uniform((uint32_t)seg.units), halves = uniform((uint32_t)seg.rows) > 128 ? 2 : 1;
-        for (int h = 0; h < halves && ok; ++h) ok = wait_warp(&sm.q_bar[h], segments[h]++ & 1, abort_flag);
-        if (!ok || !(ok = scores(halves))) break;
+        if (!(ok = wait_warp(&sm.full[buf], phase, abort_flag))) break;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            if (h >= halves || !(ok = ok && wait_warp(&sm.q_bar[h], segments[h]++ & 1, abort_flag))) break;
+            tc_fence_after();
+            scores(h, h == halves - 1);
+        }
+        advance();
         for (int j = 0; ok && j < units; ++j) {
-            if (j + 1 < units && !(ok = scores(halves))) break;
-            if (!(ok = wait_warp(&sm.v_bar[v_stage], v_phase, abort_flag))) break;
+            const unsigned v_buf = buf;
+            if (!(ok = wait_warp(&sm.full[buf], phase, abort_flag))) break;
+            advance();                      // to K of the next tile
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                if (h >= halves) break;
-                const unsigned b = pv[h] & 1;
-                if (!(ok = wait_warp(&sm.p_bar[h][b], pv[h] >> 1 & 1, abort_flag))) break;
+                if (h >= halves || !(ok = ok && wait_warp(&sm.p_bar[h], done[h] & 1, abort_flag))) break;
                 tc_fence_after();
                 if (elect_one()) {
 #pragma unroll
                     for (int x = 0; x < kKeyTile / 16; ++x)
-                        mma_ts(t0 + h * kGroup + kO, t0 + h * kGroup + b * kKeyTile + 8 * x, (va + v_stage * kBuf + x * (2048 >> 4)) | kHalfK << 16, kIdescPV, j > 0 || x > 0);
-                    tc_commit(&sm.o_bar[h][b]);
-                    if (h == halves - 1) tc_commit(&sm.v_free[v_stage]);
+                        mma_ts(t0 + h * kGroup + kO, t0 + h * kGroup + 8 * x, (kva + v_buf * kBuf + x * (2048 >> 4)) | kBlock << 16, kIdescPV, j > 0 || x > 0);
+                    tc_commit(&sm.o_bar[h]);
+                    if (h == halves - 1) tc_commit(&sm.free[v_buf]);
                 }
                 __syncwarp();
-                ++pv[h];
+                ++done[h];
+                if (j + 1 < units) {        // the scores go where the weights are: not before those have been read
+                    if (!(ok = (h > 0 || wait_warp(&sm.full[buf], phase, abort_flag)) && wait_warp(&sm.o_bar[h], (done[h] - 1) & 1, abort_flag))) break;
+                    tc_fence_after();
+                    scores(h, h == halves - 1);
+                }
             }
-            if (++v_stage == kKvStages) { v_stage = 0; v_phase ^= 1; }
+            if (j + 1 < units) advance();
         }
     }
     if (!ok)                        // nor before the products have ended
-        for (int h = 0; h < 2; ++h)
-            for (unsigned b = 0; b < 2; ++b) {
-                if (qk[h] > b) (void)cq_mbar_wait_bounded(&sm.s_bar[h][b], (qk[h] - 1 - b) >> 1 & 1);
-                if (pv[h] > b) (void)cq_mbar_wait_bounded(&sm.o_bar[h][b], (pv[h] - 1 - b) >> 1 & 1);
-            }
+        for (int h = 0; h < 2; ++h) {
+            if (tiles[h]) (void)cq_mbar_wait_bounded(&sm.s_bar[h], (tiles[h] - 1) & 1);
+            if (done[h]) (void)cq_mbar_wait_bounded(&sm.o_bar[h], (done[h] - 1) & 1);
+        }
     return ok;
 }
 
@@ -439,18 +439,17 @@ template <bool BF16> __device__ __forceinline__ uint32_t pack(float a, float b, 
 // The warp's share of the own line: S^T = K Q^T (16 keys x 8 rows), O^T += V^T P^T (dims x 8 rows) by mma.sync m16n8k16.  With rows as the narrow side eight of them
 // cost half the products and half the registers that they would cost as half of a 16-row side.  A lane holds rows 2 (lane % 4) and the next, keys (dims)
 // lane / 4 and + 8; the weights change sides by a transposition.
-template <int D, bool BF16>
-__device__ void own_part(Tiles<D> &sm, const cq_kv_cache &cache, const cq_kv::State &st, const Call &call, const uint8_t *__restrict__ k_layer,
-                         const uint8_t *__restrict__ v_layer, const uint8_t *__restrict__ q, int64_t q_stride, float c) {
-    constexpr int kStages = Tiles<D>::kStages;
-    const int lane = threadIdx.x & 31, warp = (threadIdx.x >> 5) - kOwnWarp, g = lane >> 2, x2 = (lane & 3) * 2, per = call.sh.per_kv;
-    const int worker = blockIdx.x * kMmaWarps + warp;
-    const uint32_t steps_at = uniform(cq_smem_u32(sm.step[warp]));
+// `stages_at`: shared memory of kStages steps, `stride` bytes apart.
+template <int D, bool BF16, int kStages>
+__device__ void own_part(uint32_t stages_at, uint32_t stride, int worker, const cq_kv_cache &cache, const cq_kv::State &st, const Call &call,
+                         const uint8_t *__restrict__ k_layer, const uint8_t *__restrict__ v_layer, const uint8_t *__restrict__ q, int64_t q_stride, float c) {
+    const int lane = threadIdx.x & 31, g = lane >> 2, x2 = (lane & 3) * 2, per = call.sh.per_kv;
+    const uint32_t steps_at = uniform(stages_at);
     Loader<D> load(call, worker, 31 - __clz(st.page), k_layer, v_layer, lane);
     OwnWalk walk = load.walk;
     const int units = walk.left;
     if (units <= 0) return;
-    auto send = [&](int i) { load.send(steps_at + i * (uint32_t)sizeof(Step<D>), call, st, cache.kv_heads, lane); };
+    auto send = [&](int i) { load.send(steps_at + i * stride, call, st, cache.kv_heads, lane); };
 #pragma unroll 1
     for (int i = 0; i < kStages; ++i) send(i);
     // this lane's row address in the fragments' 8 x 8 blocks: of K by key and half of a 16-dim step, of V by key and half of a 16-dim tile
@@ -481,7 +480,7 @@ __device__ void own_part(Tiles<D> &sm, const cq_kv_cache &cache, const cq_kv::St
         const int n = seg.key1 - seg.key0 - kStep * step;        // keys of this step, if fewer than 16
         cq_cp_async_wait<kStages - 1>();
         __syncwarp();
-        const uint32_t kb = steps_at + stage * (uint32_t)sizeof(Step<D>), vb = kb + (uint32_t)sizeof(Step<D>) / 2;
+        const uint32_t kb = steps_at + stage * stride, vb = kb + (uint32_t)sizeof(Step<D>) / 2;
         float s[2][4] = {};
 #pragma unroll
         for (int x = 0; x < D / 16; ++x) {
@@ -558,13 +557,8 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_mma_kernel(const cq_kv_cac
     const cq_kv::State st = cq_kv::state_of(cache);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     if (tid == 0) {
-        for (int i = 0; i < 2; ++i) {
-            cq_mbar_init(&sm.q_bar[i], 4);
-            for (int b = 0; b < 2; ++b) { cq_mbar_init(&sm.s_bar[i][b], 1); cq_mbar_init(&sm.p_bar[i][b], 4); cq_mbar_init(&sm.o_bar[i][b], 1); }
-        }
-        for (int i = 0; i < kKvStages; ++i) {
-            cq_mbar_init(&sm.k_bar[i], 1); cq_mbar_init(&sm.v_bar[i], 1); cq_mbar_init(&sm.k_free[i], 1); cq_mbar_init(&sm.v_free[i], 1);
-        }
+        for (int i = 0; i < 2; ++i) { cq_mbar_init(&sm.q_bar[i], 4); cq_mbar_init(&sm.s_bar[i], 1); cq_mbar_init(&sm.p_bar[i], 4); cq_mbar_init(&sm.o_bar[i], 1); }
+        for (int i = 0; i < kRing; ++i) { cq_mbar_init(&sm.full[i], 1); cq_mbar_init(&sm.free[i], 1); }
         sm.abort = 0;
         cq_fence_mbar_init();
     }
@@ -581,6 +575,11 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_mma_kernel(const cq_kv_cac
     if (warp < kCopyWarp) {
         regs_up<kRegsSoft>();
         ok = softmax_part<D, BF16>(sm, call, o_map, q, q_stride, c, warp >> 2);
+        // then own items as well, in the room of Q, K and V: no product or copy is under way when both halves are here
+        asm volatile("bar.sync 3, 256;" ::: "memory");
+        if (!sm.abort)
+            own_part<D, BF16, 2>(cq_smem_u32(&sm.q[0][0][0]) + warp * (uint32_t)sizeof(Step<D>), (uint32_t)sizeof(sm.q), call.sh.own_first + blockIdx.x * kCopyWarp + warp, cache,
+                                 st, call, k_layer, v_layer, q, q_stride, c);
     }
     else if (warp < kOwnWarp) {
         regs_down<kRegsMisc>();
@@ -588,7 +587,8 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_mma_kernel(const cq_kv_cac
         else if (warp == kMmaWarp) ok = mma_part<D, BF16>(sm, call);
     } else {
         regs_up<kRegsOwn>();
-        own_part<D, BF16>(sm, cache, st, call, k_layer, v_layer, q, q_stride, c);
+        own_part<D, BF16, Tiles<D>::kStages>(cq_smem_u32(sm.step[warp - kOwnWarp]), (uint32_t)sizeof(Step<D>), blockIdx.x * kMmaWarps + warp - kOwnWarp, cache, st, call, k_layer,
+                                             v_layer, q, q_stride, c);
     }
     if (!ok && lane == 0) atomicCAS(st.header, cq_kv::kOk, cq_kv::kTimeout);
     tc_fence_before();
@@ -639,7 +639,7 @@ void launch(const Call &c, const cq_kv_cache &cache, const CUtensorMap (&m)[3], 
 bool cq_attn::mma_launch(const Call &c, const cq_kv_cache &cache, int layer, const void *q, int64_t q_stride, float scale, cudaStream_t st) {
     const int64_t rows = (int64_t)cache.pages * cache.kv_heads * cache.page_size, offset = rows * layer * cache.head_dim * 2;
     const uint8_t *k = (const uint8_t *)cache.k + offset, *v = (const uint8_t *)cache.v + offset;
-    const int d = cache.head_dim, box = cache.page_size < kKeyTile ? cache.page_size : kKeyTile, boxes = cache.page_size < kKeyTile ? 1 : d / 64;
+    const int d = cache.head_dim, box = cache.page_size, boxes = box < kKeyTile ? 1 : d / 64;
     CUtensorMap m[3];
     if (!pool_map(k, rows, d, box, boxes, m[0]) || !pool_map(v, rows, d, box, boxes, m[1]) || !part_map(c, m[2])) {
         cq_set_status(CQ_ERR_CUDA, "prefix_attention: cuTensorMapEncodeTiled is not available or refused the pool");
