@@ -108,7 +108,7 @@ enum MetaOp { kReserve, kFork, kFree };
 
 // Three passes: everything is checked; the pages each slot needs are numbered in the order of the list; then the state changes.
 template <int OP>
-__global__ void __launch_bounds__(kMeta) kv_meta_kernel(const cq_kv_cache cache, const int *__restrict__ slots, const int *__restrict__ dst, int n, int arg) {
+__global__ void __launch_bounds__(kMeta) kv_meta_kernel(const cq_kv_cache cache, const int *slots, const int *dst, int n, int arg) {
     extern __shared__ unsigned seen[];              // one bit per slot
     __shared__ int sums[32], err;
     const State s = state_of(cache);

@@ -12,6 +12,7 @@
 #include "../../include/candle_q_b200.h"
 #include "common.cuh"
 
+// Pointers carry no __restrict__: a read-only one would let the compiler move loads over the wait for the kernel before.
 namespace {
 
 constexpr int kThreads = 256, kPart = 8192, kPer = kPart / kThreads, kList = 512, kMaxTop = 32;
@@ -50,111 +51,137 @@ template <typename T> __device__ __forceinline__ float load_f(const T *p) {
     else if constexpr (std::is_same<T, __half>::value) return __half2float(*p);
     else return __bfloat162float(*p);
 }
-template <typename T>
-__device__ __forceinline__ void write_row(const Out &o, const T *row, int64_t r, int vocab, float m, float s, float t) {
-    const bool ok = s > 0.0f && m < INFINITY;       // a NaN or +inf among the logits, or nothing but -inf: no distribution
-    const float ls = logf(s);
-    o.entropy[r] = ok ? ls - __fdiv_rn(t, s) : NAN;
-    if (o.tokens) {
-        const int64_t tok = o.tokens[r];
-        o.logprob[r] = tok < 0 ? 0.0f : tok >= vocab || !ok ? NAN : (load_f(row + tok) - m) - ls;
-    }
-}
 __device__ __forceinline__ void write_top(const Out &o, int64_t r, int top, int rank, uint64_t key, bool ok, float m, float ls) {
     o.top_logprobs[r * top + rank] = ok ? (value_of((uint32_t)(key >> 32)) - m) - ls : NAN;
     o.top_ids[r * top + rank] = ok ? (int64_t)(~(uint32_t)key) : -1;
 }
 
+// 16 bytes that are read once
+__device__ __forceinline__ uint4 load16(const uint4 *p) {
+    uint4 v;
+    asm volatile("ld.global.cs.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p) : "memory");
+    return v;
+}
+template <typename T> __device__ __forceinline__ float element(const uint4 &w, int j) {
+    const uint32_t b[4] = {w.x, w.y, w.z, w.w};
+    if constexpr (sizeof(T) == 4) return __uint_as_float(b[j]);
+    else if constexpr (std::is_same<T, __half>::value) return __half2float(__ushort_as_half((unsigned short)(b[j / 2] >> (16 * (j & 1)))));
+    else return __uint_as_float(j & 1 ? b[j / 2] & 0xffff0000u : b[j / 2] << 16);
+}
+__device__ __forceinline__ float ex2(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+// two f32 operations per instruction
+__device__ __forceinline__ uint64_t pack2(float a, float b) { return (uint64_t)__float_as_uint(b) << 32 | __float_as_uint(a); }
+__device__ __forceinline__ float lo(uint64_t v) { return __uint_as_float((uint32_t)v); }
+__device__ __forceinline__ float hi(uint64_t v) { return __uint_as_float((uint32_t)(v >> 32)); }
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+
+// Issue slots, not HBM, bound the first form of this kernel (some 2,000 a warp, 262 us for 1024 rows of 128256 f32); the parts inside a row have no masks, pairs
+// of elements share an instruction, and the search for alternatives is only as long as `top` asks for.
 template <typename T>
-__global__ void __launch_bounds__(kThreads) logprobs_part_kernel(const T *__restrict__ logits, int64_t stride, int vocab, int parts, int top, Part *__restrict__ part_out,
-                                                                 uint64_t *__restrict__ keys_out) {
+__global__ void __launch_bounds__(kThreads) logprobs_part_kernel(const T *logits, int64_t stride, int vocab, int parts, int top, Part *part_out,
+                                                                 uint64_t *keys_out) {
     constexpr int V = 16 / sizeof(T), N = kPer / V;
+    constexpr uint32_t kLowest = sizeof(T) == 4 ? 0xff800000u : std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u;      // -inf, for what is not there
     __shared__ float red[3][8];
-    __shared__ uint32_t group[64];
+    __shared__ __align__(16) float group[64];
+    __shared__ float least_s;
     __shared__ uint64_t list[kList];
     __shared__ int count;
     __shared__ uint64_t best[8];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int64_t r = blockIdx.x / parts;
-    const int p = blockIdx.x % parts;
+    const int p = blockIdx.x - (int)r * parts;
     cq_pdl_launch_dependents();
     cq_pdl_wait();
     // 16-byte units from the one that holds the row's first element; elements before and behind the row are masked
     const T *row = logits + r * stride;
     const int shift = (int)(((uintptr_t)row & 15) / sizeof(T)), units = (vocab + shift + V - 1) / V, per = (units + parts - 1) / parts;
     const int u0 = p * per, u1 = min(units, u0 + per);
-    const uint4 *src = reinterpret_cast<const uint4 *>(row - shift);
+    const uint4 *src = reinterpret_cast<const uint4 *>(row - shift) + u0 + tid;
     uint4 w[N];
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-        const int u = u0 + i * kThreads + tid;
-        w[i] = u < u1 ? __ldcs(src + u) : make_uint4(0, 0, 0, 0);
-    }
+    for (int i = 0; i < N; ++i) w[i] = u0 + i * kThreads + tid < u1 ? load16(src + i * kThreads) : make_uint4(kLowest, kLowest, kLowest, kLowest);
     float x[kPer];
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) x[i] = element<T>(w[i / V], i % V);
+    auto index_of = [&](int i) { return (u0 + i / V * kThreads + tid) * V + i % V - shift; };
+    auto valid = [&](int i) { return u0 + i / V * kThreads + tid < u1 && (unsigned)index_of(i) < (unsigned)vocab; };
+    if (p == 0 || p == parts - 1)               // the row's ends
+#pragma unroll
+        for (int i = 0; i < kPer; ++i)
+            if (!valid(i)) x[i] = -INFINITY;
     float mine = -INFINITY;
-    uint32_t valid = 0;             // bit per element
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-        const uint32_t b[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
-        const int u = u0 + i * kThreads + tid, e0 = u * V - shift;
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-            float f;
-            if constexpr (sizeof(T) == 4) f = __uint_as_float(b[j]);
-            else if constexpr (std::is_same<T, __half>::value) f = __half2float(__ushort_as_half((unsigned short)(b[j / 2] >> (16 * (j & 1)))));
-            else f = __uint_as_float(j & 1 ? b[j / 2] & 0xffff0000u : b[j / 2] << 16);
-            const bool in = u < u1 && e0 + j >= 0 && e0 + j < vocab;
-            x[i * V + j] = in ? f : -INFINITY;
-            valid |= (uint32_t)in << (i * V + j);
-            mine = fmaxf(mine, x[i * V + j]);
-        }
-    }
-    float g = mine;
-    g = fmaxf(g, __shfl_xor_sync(0xffffffffu, g, 1));
-    g = fmaxf(g, __shfl_xor_sync(0xffffffffu, g, 2));
-    if ((lane & 3) == 0) group[tid >> 2] = ordered(g);
-    float m = g;
+    for (int i = 0; i < kPer; i += 2) mine = max3(mine, x[i], x[i + 1]);
+    float m = mine;
+    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
+    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
+    if (top > 1 && (lane & 3) == 0) group[tid >> 2] = m;
 #pragma unroll
     for (int k = 16; k > 2; k >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, k));
     if (lane == 0) red[0][warp] = m;
     if (tid == 0) count = 0;
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < 8; ++i) m = fmaxf(m, red[0][i]);
+    for (int i = 0; i < 8; i += 2) m = max3(m, red[0][i], red[0][i + 1]);
     const float base = m == -INFINITY ? 0.0f : m;
-    float s = 0.0f, t = 0.0f;
+    const uint64_t nbase = pack2(-base, -base), log2e = pack2(1.44269504f, 1.44269504f);
+    uint64_t s2 = 0, t2 = 0;
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-        const float z = x[i] - base, e = exp2f(z * 1.44269504f);
-        s += e;
-        t = __fmaf_rn(e, fmaxf(z, -150.0f), t);         // e is 0 from there on: -inf must not meet it
+    for (int i = 0; i < kPer; i += 2) {
+        const uint64_t z = add2(pack2(x[i], x[i + 1]), nbase), y = mul2(z, log2e), e = pack2(ex2(lo(y)), ex2(hi(y)));
+        s2 = add2(s2, e);
+        t2 = fma2(e, z, t2);
+    }
+    float s = lo(s2) + hi(s2), t = lo(t2) + hi(t2);
+    if (t != t) {               // 0 times an infinite distance: a logit of -inf has no share in it (from 150 on the weight is 0)
+        t = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+            const float z = x[i] - base;
+            t = __fmaf_rn(ex2(z * 1.44269504f), fmaxf(z, -150.0f), t);
+        }
     }
     s = warp_sum(s);
     t = warp_sum(t);
     if (lane == 0) { red[1][warp] = s; red[2][warp] = t; }
-    // the top-th largest of the 64 groups' maxima
-    uint32_t least = 1;
-    if (top > 0) {
-        const uint32_t a = group[lane], b = group[lane + 32];
-        int ra = 0, rb = 0;
-#pragma unroll 8
-        for (int i = 0; i < 64; ++i) {
-            const uint32_t o = group[i];
-            ra += o > a || (o == a && i < lane);
-            rb += o > b || (o == b && i < lane + 32);
-        }
-        least = __reduce_max_sync(0xffffffffu, ra == top - 1 ? a : rb == top - 1 ? b : 0u);
-        const uint32_t omine = ordered(mine);
-        if (omine >= least && valid) {
+    // the top-th largest of the 64 groups' maxima: a warp ranks eight of them, four lanes each
+    if (top > 1) {
+        const int at = warp * 8 + (lane >> 2), j0 = (lane & 3) * 16;
+        const float v = group[at];
+        int rank = 0;
 #pragma unroll
-            for (int i = 0; i < kPer; ++i) {
-                const uint32_t o = ordered(x[i]);
-                if ((valid >> i & 1) && o >= least) {
-                    const int at = atomicAdd(&count, 1), e = (u0 + i / V * kThreads + tid) * V + i % V - shift;
-                    if (at < kList) list[at] = (uint64_t)o << 32 | (uint32_t)~e;
-                }
-            }
+        for (int j = 0; j < 16; j += 4) {
+            const float4 o = *reinterpret_cast<const float4 *>(&group[j0 + j]);
+            rank += (o.x > v || (o.x == v && j0 + j < at)) + (o.y > v || (o.y == v && j0 + j + 1 < at)) + (o.z > v || (o.z == v && j0 + j + 2 < at)) +
+                    (o.w > v || (o.w == v && j0 + j + 3 < at));
         }
+        rank += __shfl_xor_sync(0xffffffffu, rank, 1);
+        rank += __shfl_xor_sync(0xffffffffu, rank, 2);
+        if (rank == top - 1 && (lane & 3) == 0) least_s = v;
     }
     __syncthreads();
     if (tid == 0) {
@@ -164,6 +191,16 @@ __global__ void __launch_bounds__(kThreads) logprobs_part_kernel(const T *__rest
         part_out[blockIdx.x] = Part{m, s, t, 0.0f};
     }
     if (top == 0) return;
+    const float least = top > 1 ? least_s : m;
+    if (mine >= least) {
+#pragma unroll
+        for (int i = 0; i < kPer; ++i)
+            if (x[i] >= least && valid(i)) {
+                const int at = atomicAdd(&count, 1);
+                if (at < kList) list[at] = (uint64_t)ordered(x[i]) << 32 | (uint32_t)~index_of(i);
+            }
+    }
+    __syncthreads();
     uint64_t *keys = keys_out + (int64_t)blockIdx.x * top;
     const int n = count;
     if (n <= kList) {
@@ -181,8 +218,7 @@ __global__ void __launch_bounds__(kThreads) logprobs_part_kernel(const T *__rest
         uint64_t k = 0;
 #pragma unroll
         for (int i = 0; i < kPer; ++i) {
-            const int e = (u0 + i / V * kThreads + tid) * V + i % V - shift;
-            const uint64_t c = valid >> i & 1 ? (uint64_t)ordered(x[i]) << 32 | (uint32_t)~e : 0;
+            const uint64_t c = valid(i) ? (uint64_t)ordered(x[i]) << 32 | (uint32_t)~index_of(i) : 0;
             if (c < below && c > k) k = c;
         }
         k = warp_max(k);
@@ -196,28 +232,37 @@ __global__ void __launch_bounds__(kThreads) logprobs_part_kernel(const T *__rest
     }
 }
 
-// One CTA per row: the parts' sums, then the best of their lists.  The largest of the parts' last keys is no higher than the row's top-th key.
+// One CTA per row: the parts' sums (first warp) beside the best of their lists.  The largest of the parts' last keys is no higher than the row's top-th key, which leaves few
+// keys to rank.
+constexpr int kJoin = 128, kHeld = 8;           // threads; keys a thread holds
 template <typename T>
-__global__ void __launch_bounds__(128) logprobs_join_kernel(const T *__restrict__ logits, int64_t stride, int vocab, int parts, int top, const Part *__restrict__ part_in,
-                                                            const uint64_t *__restrict__ keys_in, const Out o) {
+__global__ void __launch_bounds__(kJoin) logprobs_join_kernel(const T *logits, int64_t stride, int vocab, int parts, int top, const Part *part_in,
+                                                              const uint64_t *keys_in, const Out o) {
     __shared__ float row_m, row_s;
-    __shared__ uint64_t least_of[4];
+    __shared__ uint64_t least_of[kJoin / 32];
     __shared__ uint64_t list[kList];
     __shared__ int count;
     const int64_t r = blockIdx.x;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, all = parts * top;
     cq_pdl_launch_dependents();
     cq_pdl_wait();
     const Part *part = part_in + r * parts;
-    const uint64_t *keys = keys_in + r * parts * top;
-    if (warp == 0) {
-        float m = -INFINITY;
-        for (int p = lane; p < parts; p += 32) m = fmaxf(m, part[p].m);
+    const uint64_t *keys = keys_in + r * all;
+    // what every row needs is asked for at once
+    uint64_t k[kHeld];
 #pragma unroll
-        for (int k = 16; k > 0; k >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, k));
-        float s = 0.0f, t = 0.0f;
+    for (int i = 0; i < kHeld; ++i) k[i] = tid + i * kJoin < all ? keys[tid + i * kJoin] : 0;
+    if (warp == 0) {
+        const int64_t tok = o.tokens ? o.tokens[r] : -1;
+        const float at_tok = tok >= 0 && tok < vocab ? load_f(logits + r * stride + tok) : 0.0f;
+        float m = -INFINITY, s = 0.0f, t = 0.0f;
+        const Part first = lane < parts ? part[lane] : Part{-INFINITY, 0.0f, 0.0f, 0.0f};
+        m = first.m;
+        for (int p = lane + 32; p < parts; p += 32) m = fmaxf(m, part[p].m);
+#pragma unroll
+        for (int x = 16; x > 0; x >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
         for (int p = lane; p < parts; p += 32) {
-            const Part a = part[p];
+            const Part a = p == lane ? first : part[p];
             if (a.s != 0.0f) {                              // nothing but -inf: no weight, and no difference of infinities
                 const float d = fmaxf(a.m - m, -150.0f), f = expf(d);       // the difference of two finite values may be -inf
                 s = __fmaf_rn(f, a.s, s);
@@ -227,49 +272,52 @@ __global__ void __launch_bounds__(128) logprobs_join_kernel(const T *__restrict_
         s = warp_sum(s);
         t = warp_sum(t);
         if (lane == 0) {
-            write_row(o, logits + r * stride, r, vocab, m, s, t);
+            const bool ok = s > 0.0f && m < INFINITY;       // a NaN or +inf among the logits, or nothing but -inf: no distribution
+            const float ls = logf(s);
+            o.entropy[r] = ok ? ls - __fdiv_rn(t, s) : NAN;
+            if (o.tokens) o.logprob[r] = tok < 0 ? 0.0f : tok >= vocab || !ok ? NAN : (at_tok - m) - ls;
             row_m = m;
             row_s = s;
         }
     }
     if (top == 0) return;
     uint64_t least = 0;
-    for (int p = tid; p < parts; p += 128) {
-        const uint64_t k = keys[(int64_t)p * top + top - 1];
-        least = k > least ? k : least;
-    }
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) least = (tid + i * kJoin) % top == top - 1 && k[i] > least ? k[i] : least;
+    for (int i = tid + kHeld * kJoin; i < all; i += kJoin) least = i % top == top - 1 && keys[i] > least ? keys[i] : least;
     least = warp_max(least);
     if (lane == 0) least_of[warp] = least;
     if (tid == 0) count = 0;
     __syncthreads();
     least = least_of[0];
 #pragma unroll
-    for (int i = 1; i < 4; ++i) least = least_of[i] > least ? least_of[i] : least;
+    for (int i = 1; i < kJoin / 32; ++i) least = least_of[i] > least ? least_of[i] : least;
     const float m = row_m, s = row_s, ls = logf(s);
     const bool ok = s > 0.0f && m < INFINITY;
     if (!ok) {
         if (tid < top) write_top(o, r, top, tid, 0, false, m, ls);
         return;
     }
-    // keys differ, so at most (parts - 1) * (top - 1) + top of them are not below `least`; the list may still be too short for that
-    for (int i = tid; i < parts * top; i += 128) {
-        const uint64_t k = keys[i];
-        if (k >= least && k != 0) {
+    auto take = [&](uint64_t key) {
+        if (key >= least && key != 0) {
             const int at = atomicAdd(&count, 1);
-            if (at < kList) list[at] = k;
+            if (at < kList) list[at] = key;
         }
-    }
+    };
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) take(k[i]);
+    for (int i = tid + kHeld * kJoin; i < all; i += kJoin) take(keys[i]);
     __syncthreads();
+    // keys differ, so at most (parts - 1) * (top - 1) + top of them are not below `least`; where the list is too short for that, all are ranked
     const int n = count;
-    const bool all = n <= kList;
-    const uint64_t *from = all ? list : keys;
-    const int total = all ? n : parts * top;
-    for (int i = tid; i < total; i += 128) {
-        const uint64_t k = from[i];
-        if (k < least || k == 0) continue;
+    const uint64_t *from = n <= kList ? list : keys;
+    const int total = n <= kList ? n : all;
+    for (int i = tid; i < total; i += kJoin) {
+        const uint64_t key = from[i];
+        if (key < least || key == 0) continue;
         int rank = 0;
-        for (int j = 0; j < total; ++j) rank += from[j] > k;
-        if (rank < top) write_top(o, r, top, rank, k, ok, m, ls);
+        for (int j = 0; j < total; ++j) rank += from[j] > key;
+        if (rank < top) write_top(o, r, top, rank, key, ok, m, ls);
     }
 }
 
@@ -281,7 +329,7 @@ void launch(const void *logits, int64_t stride, int rows, int vocab, int top, co
     Part *part = reinterpret_cast<Part *>(scratch);
     uint64_t *keys = reinterpret_cast<uint64_t *>(part + (int64_t)rows * parts);
     cq_launch_k(logprobs_part_kernel<T>, dim3((unsigned)((int64_t)rows * parts)), dim3(kThreads), 0, st, (const T *)logits, stride, vocab, parts, top, part, keys);
-    cq_launch_k(logprobs_join_kernel<T>, dim3((unsigned)rows), dim3(128), 0, st, (const T *)logits, stride, vocab, parts, top, (const Part *)part,
+    cq_launch_k(logprobs_join_kernel<T>, dim3((unsigned)rows), dim3(kJoin), 0, st, (const T *)logits, stride, vocab, parts, top, (const Part *)part,
                 (const uint64_t *)keys, o);
 }
 

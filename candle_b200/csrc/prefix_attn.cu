@@ -12,13 +12,13 @@ using cq_kv::State;
 constexpr int kThreads = 256, kPlanCtas = 8;
 
 // Units per worker of the own line.  f16 and bf16: the four warps of a CTA that have nothing else, and the eight that come when its `units` shared ones are done.  In clocks
-// of a B200 SM: a shared unit takes 4,300 and the first of them 5,000 more, one of the four warps takes 2,800 a step beside them, and twelve warps together are bound by
+// of a B200 SM: a shared unit takes 4,300 and the first of them 5,000 more, one of the four warps takes some 1,700 a step beside them, and twelve warps together are bound by
 // HBM with 400 a step.  All finish together by that; a model that is off by a third leaves the one kind of warps idle for a tenth of the time.
 __device__ __forceinline__ void own_chunks(const Shape &s, int units, int line, int &chunk, int &chunk2) {
     chunk2 = 1;
     if (s.own_first == s.own_workers) { chunk = max((line + s.own_workers - 1) / s.own_workers, 1); return; }
     const int per_cta = (line + s.ctas - 1) / s.ctas;
-    const int beside = units ? (int)min(((int64_t)units * 4300 + 5000) / 2800, (int64_t)per_cta) : 0;          // steps a warp does in that time
+    const int beside = units ? (int)min(((int64_t)units * 4300 + 5000) / 1700, (int64_t)per_cta) : 0;          // steps a warp does in that time
     const int rest = per_cta - kMmaWarps * beside;
     if (rest <= 0) { chunk = max((per_cta + kMmaWarps - 1) / kMmaWarps, 1); return; }
     const int share = (rest + kMmaWarps + kMmaHelpers - 1) / (kMmaWarps + kMmaHelpers);
@@ -66,7 +66,7 @@ __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.w
 // Bound by latency: slots, lengths and tables are three reads that depend on one another, and a warp by itself takes some five clocks an instruction.
 // So the comparison and the records are divided over the CTAs, everything else each does for itself, and divisions are kept out of the way (one CTA of 1024 threads
 // took 16 - 33 us for 64 - 128 sequences).
-__global__ void __launch_bounds__(kThreads) prefix_plan_kernel(const cq_kv_cache cache, const Call call, const int *__restrict__ slots) {
+__global__ void __launch_bounds__(kThreads) prefix_plan_kernel(const cq_kv_cache cache, const Call call, const int *slots) {
     extern __shared__ int dyn[];
     __shared__ uint64_t sums[kThreads / 32];
     __shared__ int most;
@@ -216,7 +216,7 @@ __global__ void __launch_bounds__(kThreads) prefix_plan_kernel(const cq_kv_cache
 
 // One warp per row: lane x weighs segment x - those of the row's shared item, then those of its own one, in the order of their keys - and the
 // outputs are added in that order.
-template <typename T, int D> __global__ void __launch_bounds__(256) prefix_join_kernel(const Call call, T *__restrict__ out) {
+template <typename T, int D> __global__ void __launch_bounds__(256) prefix_join_kernel(const Call call, T *out) {
     const Shape &sh = call.sh;
     const Plan &pl = call.plan;
     cq_pdl_launch_dependents();

@@ -108,7 +108,7 @@ __device__ __forceinline__ void expect_tx(uint32_t bar, uint32_t bytes) {
 
 // Softmax of one half of the row tiles.  False: a wait gave up.
 template <int D, bool BF16>
-__device__ bool softmax_part(Tiles<D> &sm, const Call &call, const CUtensorMap &o_map, const uint8_t *__restrict__ q, int64_t q_stride, float c, int half) {
+__device__ bool softmax_part(Tiles<D> &sm, const Call &call, const CUtensorMap &o_map, const uint8_t *q, int64_t q_stride, float c, int half) {
     const int tid = threadIdx.x & 127, lane = tid & 31, warp = tid >> 5, row = tid, per = call.sh.per_kv;
     const uint32_t mine = sm.tmem + ((uint32_t)(warp * 32) << 16) + half * kGroup;
     volatile int *abort_flag = &sm.abort;
@@ -442,7 +442,7 @@ template <bool BF16> __device__ __forceinline__ uint32_t pack(float a, float b, 
 // `stages_at`: shared memory of kStages steps, `stride` bytes apart.
 template <int D, bool BF16, int kStages>
 __device__ void own_part(uint32_t stages_at, uint32_t stride, int worker, const cq_kv_cache &cache, const cq_kv::State &st, const Call &call,
-                         const uint8_t *__restrict__ k_layer, const uint8_t *__restrict__ v_layer, const uint8_t *__restrict__ q, int64_t q_stride, float c) {
+                         const uint8_t *k_layer, const uint8_t *v_layer, const uint8_t *q, int64_t q_stride, float c) {
     const int lane = threadIdx.x & 31, g = lane >> 2, x2 = (lane & 3) * 2, per = call.sh.per_kv;
     const uint32_t steps_at = uniform(stages_at);
     Loader<D> load(call, worker, 31 - __clz(st.page), k_layer, v_layer, lane);
@@ -550,8 +550,8 @@ __device__ void own_part(uint32_t stages_at, uint32_t stride, int worker, const 
 template <int D, bool BF16>
 __global__ void __launch_bounds__(kThreads, 1) prefix_mma_kernel(const cq_kv_cache cache, const Call call, const __grid_constant__ CUtensorMap k_map,
                                                                  const __grid_constant__ CUtensorMap v_map, const __grid_constant__ CUtensorMap o_map,
-                                                                 const uint8_t *__restrict__ k_layer, const uint8_t *__restrict__ v_layer,
-                                                                 const uint8_t *__restrict__ q, int64_t q_stride, float c) {
+                                                                 const uint8_t *k_layer, const uint8_t *v_layer,
+                                                                 const uint8_t *q, int64_t q_stride, float c) {
     extern __shared__ uint8_t raw[];
     Tiles<D> &sm = *reinterpret_cast<Tiles<D> *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
     const cq_kv::State st = cq_kv::state_of(cache);

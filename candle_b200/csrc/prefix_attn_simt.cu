@@ -71,7 +71,7 @@ template <int D, int R> __device__ __forceinline__ void outputs(const Smem<D> &s
 }
 
 template <typename T, int D>
-__global__ void __launch_bounds__(kThreads) prefix_simt_kernel(const cq_kv_cache cache, const Call call, int layer, const T *__restrict__ q, int64_t q_stride,
+__global__ void __launch_bounds__(kThreads) prefix_simt_kernel(const cq_kv_cache cache, const Call call, int layer, const T *q, int64_t q_stride,
                                                                float c) {
     extern __shared__ __align__(16) uint8_t raw[];
     Smem<D> &sm = *reinterpret_cast<Smem<D> *>(raw);
