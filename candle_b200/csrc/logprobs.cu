@@ -4,18 +4,18 @@
 // (T <= 0, so the entropy is a sum of two terms that are not negative.)  Parts of a row are joined by M = max M_p, f_p = e^(M_p - M),
 // S = sum f_p S_p, T = sum f_p (T_p + S_p (M_p - M)).
 //
-// One read of the logits is the bound.  A CTA holds a part of 8192 elements in registers, 32 a thread, so all its loads are in flight at
-// once and the maximum, the sums and the alternatives need no second read.  The best `top` of a part: 64 groups of four threads have a
-// maximum each, and the top-th largest of these is no higher than the top-th largest element; the elements from there on, some more
-// than `top`, go to a list in shared memory and are ranked by counting.  Ties make the list long (a row of one value has 8192 of
-// them): then the best is taken `top` times instead.
+// One read of the logits is the bound.  A warp walks one segment of a row in chunks of 1024 elements, 32 a lane, the next chunk on its way to shared memory; nothing waits
+// for another warp.  Each lane keeps a maximum, S and T of its own; the maximum follows only where a chunk's is more than 2 higher (S and T have any base near the maximum;
+// lanes, then segments, are joined as above).  The best `top` so far lie in the lanes in order; a chunk whose maximum does not pass the last of them - after the first few
+// nearly every one - costs them a vote.  Else its elements from there on are ranked against the list by counting.  (With a CTA per 8192 elements, a maximum of the
+// CTA first and a list for its candidates, 1024 rows of 128256 f32 took 141 us: a warp in search of candidates held up the seven others.)
 #include "../../include/candle_q_b200.h"
 #include "common.cuh"
 
 // Pointers carry no __restrict__: a read-only one would let the compiler move loads over the wait for the kernel before.
 namespace {
 
-constexpr int kThreads = 256, kPart = 8192, kPer = kPart / kThreads, kList = 512, kMaxTop = 32;
+constexpr int kThreads = 256, kWarps = kThreads / 32, kCtas = 3, kPer = 32, kChunk = 32 * kPer, kList = 512, kMaxTop = 32, kMaxSegments = 128;
 
 // Keys order elements by (value descending, index ascending) as one unsigned comparison; 0: not an element of the row.
 __device__ __forceinline__ uint32_t ordered(float x) {
@@ -31,15 +31,6 @@ __device__ __forceinline__ float warp_sum(float v) {
     for (int m = 16; m > 0; m >>= 1) v += __shfl_xor_sync(0xffffffffu, v, m);
     return v;
 }
-__device__ __forceinline__ uint64_t warp_max(uint64_t v) {
-#pragma unroll
-    for (int m = 16; m > 0; m >>= 1) {
-        const uint64_t o = __shfl_xor_sync(0xffffffffu, v, m);
-        v = o > v ? o : v;
-    }
-    return v;
-}
-
 // A row's values from its joined parts.
 struct Out {
     const int64_t *tokens;
@@ -56,12 +47,6 @@ __device__ __forceinline__ void write_top(const Out &o, int64_t r, int top, int 
     o.top_ids[r * top + rank] = ok ? (int64_t)(~(uint32_t)key) : -1;
 }
 
-// 16 bytes that are read once
-__device__ __forceinline__ uint4 load16(const uint4 *p) {
-    uint4 v;
-    asm volatile("ld.global.cs.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p) : "memory");
-    return v;
-}
 template <typename T> __device__ __forceinline__ float element(const uint4 &w, int j) {
     const uint32_t b[4] = {w.x, w.y, w.z, w.w};
     if constexpr (sizeof(T) == 4) return __uint_as_float(b[j]);
@@ -98,177 +83,247 @@ __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
     return r;
 }
 
-// Issue slots, not HBM, bound the first form of this kernel (some 2,000 a warp, 262 us for 1024 rows of 128256 f32); the parts inside a row have no masks, pairs
-// of elements share an instruction, and the search for alternatives is only as long as `top` asks for.
+template <typename T> struct Warp {
+    static constexpr int kUnits = kPer * (int)sizeof(T) / 16;          // 16-byte units of a chunk, a lane
+    uint4 ring[2][kUnits][32];
+    uint64_t found[64];                                               // candidates not yet in the list
+};
+
 template <typename T>
-__global__ void __launch_bounds__(kThreads) logprobs_part_kernel(const T *logits, int64_t stride, int vocab, int parts, int top, Part *part_out,
-                                                                 uint64_t *keys_out) {
-    constexpr int V = 16 / sizeof(T), N = kPer / V;
+__global__ void __launch_bounds__(kThreads, kCtas) logprobs_segment_kernel(const T *logits, int64_t stride, int vocab, int segments, int per_segment, int total, int top, Part *part_out,
+                                                                           uint64_t *keys_out) {
+    constexpr int V = 16 / sizeof(T), N = Warp<T>::kUnits;
     constexpr uint32_t kLowest = sizeof(T) == 4 ? 0xff800000u : std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u;      // -inf, for what is not there
-    __shared__ float red[3][8];
-    __shared__ __align__(16) float group[64];
-    __shared__ float least_s;
-    __shared__ uint64_t list[kList];
-    __shared__ int count;
-    __shared__ uint64_t best[8];
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int64_t r = blockIdx.x / parts;
-    const int p = blockIdx.x - (int)r * parts;
+    extern __shared__ __align__(16) uint8_t raw[];
+    const int lane = threadIdx.x & 31;
+    Warp<T> &sm = reinterpret_cast<Warp<T> *>(raw)[threadIdx.x >> 5];
     cq_pdl_launch_dependents();
     cq_pdl_wait();
-    // 16-byte units from the one that holds the row's first element; elements before and behind the row are masked
-    const T *row = logits + r * stride;
-    const int shift = (int)(((uintptr_t)row & 15) / sizeof(T)), units = (vocab + shift + V - 1) / V, per = (units + parts - 1) / parts;
-    const int u0 = p * per, u1 = min(units, u0 + per);
-    const uint4 *src = reinterpret_cast<const uint4 *>(row - shift) + u0 + tid;
-    uint4 w[N];
+#pragma unroll 1
+    for (int at = blockIdx.x * kWarps + (threadIdx.x >> 5); at < total; at += gridDim.x * kWarps) {
+        // 16-byte units from the one that holds the row's first element; elements before and behind the row are masked
+        const int r = at / segments, sg = at - r * segments;
+        const T *row = logits + r * stride;
+        const int shift = (int)(((uintptr_t)row & 15) / sizeof(T)), units = (vocab + shift + V - 1) / V;
+        const int u0 = sg * per_segment * N * 32, chunks = min(per_segment, max((units - u0 + N * 32 - 1) / (N * 32), 0));
+        const uint4 *src = reinterpret_cast<const uint4 *>(row - shift) + lane;
+        auto bring = [&](int c) {
+            if (c < chunks) {
+                const int u = u0 + c * N * 32;
 #pragma unroll
-    for (int i = 0; i < N; ++i) w[i] = u0 + i * kThreads + tid < u1 ? load16(src + i * kThreads) : make_uint4(kLowest, kLowest, kLowest, kLowest);
-    float x[kPer];
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) x[i] = element<T>(w[i / V], i % V);
-    auto index_of = [&](int i) { return (u0 + i / V * kThreads + tid) * V + i % V - shift; };
-    auto valid = [&](int i) { return u0 + i / V * kThreads + tid < u1 && (unsigned)index_of(i) < (unsigned)vocab; };
-    if (p == 0 || p == parts - 1)               // the row's ends
-#pragma unroll
-        for (int i = 0; i < kPer; ++i)
-            if (!valid(i)) x[i] = -INFINITY;
-    float mine = -INFINITY;
-#pragma unroll
-    for (int i = 0; i < kPer; i += 2) mine = max3(mine, x[i], x[i + 1]);
-    float m = mine;
-    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
-    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
-    if (top > 1 && (lane & 3) == 0) group[tid >> 2] = m;
-#pragma unroll
-    for (int k = 16; k > 2; k >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, k));
-    if (lane == 0) red[0][warp] = m;
-    if (tid == 0) count = 0;
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < 8; i += 2) m = max3(m, red[0][i], red[0][i + 1]);
-    const float base = m == -INFINITY ? 0.0f : m;
-    const uint64_t nbase = pack2(-base, -base), log2e = pack2(1.44269504f, 1.44269504f);
-    uint64_t s2 = 0, t2 = 0;
-#pragma unroll
-    for (int i = 0; i < kPer; i += 2) {
-        const uint64_t z = add2(pack2(x[i], x[i + 1]), nbase), y = mul2(z, log2e), e = pack2(ex2(lo(y)), ex2(hi(y)));
-        s2 = add2(s2, e);
-        t2 = fma2(e, z, t2);
-    }
-    float s = lo(s2) + hi(s2), t = lo(t2) + hi(t2);
-    if (t != t) {               // 0 times an infinite distance: a logit of -inf has no share in it (from 150 on the weight is 0)
-        t = 0.0f;
-#pragma unroll
-        for (int i = 0; i < kPer; ++i) {
-            const float z = x[i] - base;
-            t = __fmaf_rn(ex2(z * 1.44269504f), fmaxf(z, -150.0f), t);
-        }
-    }
-    s = warp_sum(s);
-    t = warp_sum(t);
-    if (lane == 0) { red[1][warp] = s; red[2][warp] = t; }
-    // the top-th largest of the 64 groups' maxima: a warp ranks eight of them, four lanes each
-    if (top > 1) {
-        const int at = warp * 8 + (lane >> 2), j0 = (lane & 3) * 16;
-        const float v = group[at];
-        int rank = 0;
-#pragma unroll
-        for (int j = 0; j < 16; j += 4) {
-            const float4 o = *reinterpret_cast<const float4 *>(&group[j0 + j]);
-            rank += (o.x > v || (o.x == v && j0 + j < at)) + (o.y > v || (o.y == v && j0 + j + 1 < at)) + (o.z > v || (o.z == v && j0 + j + 2 < at)) +
-                    (o.w > v || (o.w == v && j0 + j + 3 < at));
-        }
-        rank += __shfl_xor_sync(0xffffffffu, rank, 1);
-        rank += __shfl_xor_sync(0xffffffffu, rank, 2);
-        if (rank == top - 1 && (lane & 3) == 0) least_s = v;
-    }
-    __syncthreads();
-    if (tid == 0) {
-        s = red[1][0]; t = red[2][0];
-#pragma unroll
-        for (int i = 1; i < 8; ++i) { s += red[1][i]; t += red[2][i]; }
-        part_out[blockIdx.x] = Part{m, s, t, 0.0f};
-    }
-    if (top == 0) return;
-    const float least = top > 1 ? least_s : m;
-    if (mine >= least) {
-#pragma unroll
-        for (int i = 0; i < kPer; ++i)
-            if (x[i] >= least && valid(i)) {
-                const int at = atomicAdd(&count, 1);
-                if (at < kList) list[at] = (uint64_t)ordered(x[i]) << 32 | (uint32_t)~index_of(i);
+                for (int i = 0; i < N; ++i) {
+                    uint4 *to = &sm.ring[c & 1][i][lane];
+                    if (u + i * 32 + lane < units) cq_cp_async16(to, src + u + i * 32);
+                    else *to = make_uint4(kLowest, kLowest, kLowest, kLowest);
+                }
             }
-    }
-    __syncthreads();
-    uint64_t *keys = keys_out + (int64_t)blockIdx.x * top;
-    const int n = count;
-    if (n <= kList) {
-        for (int i = tid; i < n; i += kThreads) {
-            const uint64_t k = list[i];
-            int rank = 0;
-            for (int j = 0; j < n; ++j) rank += list[j] > k;
-            if (rank < top) keys[rank] = k;
-        }
-        for (int i = n + tid; i < top; i += kThreads) keys[i] = 0;      // a part of fewer elements than `top`
-        return;
-    }
-    uint64_t below = ~0ull;
-    for (int a = 0; a < top; ++a) {
-        uint64_t k = 0;
+            cq_cp_async_commit();
+        };
+        float m = -INFINITY, s = 0.0f, t = 0.0f;
+        uint64_t best = 0;                      // the lane-th best so far
+        float bound = -INFINITY;                // elements from here on may belong to them
+        bring(0);
+#pragma unroll 1
+        for (int c = 0; c < chunks; ++c) {
+            bring(c + 1);
+            cq_cp_async_wait<1>();
+            const int u = u0 + c * N * 32 + lane;
+            const bool edge = u0 + c == 0 || u0 + (c + 1) * N * 32 >= units;            // of the row: with elements that are not of it
+            auto index_of = [&](int i, int j) { return (u + i * 32) * V + j - shift; };
+            float x[kPer];
 #pragma unroll
-        for (int i = 0; i < kPer; ++i) {
-            const uint64_t c = valid(i) ? (uint64_t)ordered(x[i]) << 32 | (uint32_t)~index_of(i) : 0;
-            if (c < below && c > k) k = c;
-        }
-        k = warp_max(k);
-        __syncthreads();
-        if (lane == 0) best[warp] = k;
-        __syncthreads();
-        below = best[0];
+            for (int i = 0; i < N; ++i) {
+                const uint4 w = sm.ring[c & 1][i][lane];
 #pragma unroll
-        for (int i = 1; i < 8; ++i) below = best[i] > below ? best[i] : below;
-        if (tid == 0) keys[a] = below;
+                for (int j = 0; j < V; ++j) x[i * V + j] = element<T>(w, j);
+            }
+            if (edge)
+#pragma unroll
+                for (int i = 0; i < kPer; ++i)
+                    if ((unsigned)index_of(i / V, i % V) >= (unsigned)vocab) x[i] = -INFINITY;
+            float mine = -INFINITY, other = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < kPer; i += 4) { mine = max3(mine, x[i], x[i + 1]); other = max3(other, x[i + 2], x[i + 3]); }
+            mine = fmaxf(mine, other);
+            if (__any_sync(0xffffffffu, mine > m + 2.0f)) {
+                if (mine > m + 2.0f) {
+                    const float d = fmaxf(m - mine, -150.0f), f = ex2(d * 1.44269504f);      // from -inf: S and T are 0
+                    t = f * __fmaf_rn(s, d, t);
+                    s *= f;
+                    m = mine;
+                }
+            }
+            const float base = m == -INFINITY ? 0.0f : m;
+            const uint64_t nbase = pack2(-base, -base), log2e = pack2(1.44269504f, 1.44269504f);
+            uint64_t s2 = 0, t2 = 0;
+#pragma unroll
+            for (int i = 0; i < kPer; i += 2) {
+                const uint64_t z = add2(pack2(x[i], x[i + 1]), nbase), y = mul2(z, log2e), e = pack2(ex2(lo(y)), ex2(hi(y)));
+                s2 = add2(s2, e);
+                t2 = fma2(e, z, t2);
+            }
+            float tc = lo(t2) + hi(t2);
+            if (tc != tc) {             // 0 times an infinite distance: a logit of -inf has no share in it (from 150 on the weight is 0)
+                tc = 0.0f;
+#pragma unroll
+                for (int i = 0; i < kPer; ++i) {
+                    const float z = x[i] - base;
+                    tc = __fmaf_rn(ex2(z * 1.44269504f), fmaxf(z, -150.0f), tc);
+                }
+            }
+            s += lo(s2) + hi(s2);
+            t += tc;
+            if (top == 0) continue;
+            if (top == 1) {                     // a lane's own best, its first among equals
+                if (mine > bound || best == 0) {
+                    int at_i = kPer;
+#pragma unroll
+                    for (int i = kPer - 1; i >= 0; --i)
+                        if (x[i] == mine && (!edge || (u + i / V * 32 < units && (unsigned)index_of(i / V, i % V) < (unsigned)vocab))) at_i = i;
+                    if (at_i < kPer && u + at_i / V * 32 < units) {
+                        best = (uint64_t)ordered(mine) << 32 | (uint32_t)~index_of(at_i / V, at_i % V);
+                        bound = mine;
+                    }
+                }
+                continue;
+            }
+            const unsigned over = __ballot_sync(0xffffffffu, mine >= bound);
+            if (!over) continue;
+            // the top-th largest of the lanes' maxima is no higher than the chunk's top-th element
+            if (__popc(over) >= top) {
+                float *maxima = reinterpret_cast<float *>(sm.found);
+                maxima[lane] = mine;
+                __syncwarp();
+                int rank = 0;
+#pragma unroll
+                for (int y = 0; y < 32; y += 4) {
+                    const float4 v = *reinterpret_cast<const float4 *>(maxima + y);
+                    rank += (v.x > mine || (v.x == mine && y < lane)) + (v.y > mine || (v.y == mine && y + 1 < lane)) + (v.z > mine || (v.z == mine && y + 2 < lane)) +
+                            (v.w > mine || (v.w == mine && y + 3 < lane));
+                }
+                bound = fmaxf(bound, __shfl_sync(0xffffffffu, mine, __ffs(__ballot_sync(0xffffffffu, rank == top - 1)) - 1));
+                __syncwarp();
+            }
+            uint32_t hits = 0;
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) hits |= (uint32_t)(x[i] >= bound) << i;
+            int n = 0;
+            // 32 found ones and the list, each ranked among all
+            auto merge = [&](int from, int count) {
+                __syncwarp();
+                const uint64_t key = lane < count ? sm.found[from + lane] : 0;
+                int rank_list = lane, rank_key = 0;
+#pragma unroll 4
+                for (int y = 0; y < count; ++y) {
+                    const uint64_t k = __shfl_sync(0xffffffffu, key, y);
+                    const int above = __popc(__ballot_sync(0xffffffffu, best > k));
+                    rank_list += k > best;
+                    rank_key += (k > key) + (y == lane ? above : 0);
+                }
+                __syncwarp();
+                // over the keys that were just read
+                if (best != 0 && rank_list < 32) sm.found[from + rank_list] = best;
+                if (key != 0 && rank_key < 32) sm.found[from + rank_key] = key;
+                const int filled = min(32, __popc(__ballot_sync(0xffffffffu, best != 0)) + count);
+                __syncwarp();
+                best = lane < filled ? sm.found[from + lane] : 0;
+                __syncwarp();
+                const uint64_t last = __shfl_sync(0xffffffffu, best, top - 1);
+                if (last != 0) bound = fmaxf(bound, value_of((uint32_t)(last >> 32)));
+            };
+#pragma unroll 1
+            while (__any_sync(0xffffffffu, hits != 0)) {            // one of each lane's at a time
+                const int i = __ffs(hits) - 1, e = index_of(i / V, i % V);
+                const bool there = hits != 0 && u + i / V * 32 < units && (unsigned)e < (unsigned)vocab;
+                const float v = there ? load_f(reinterpret_cast<const T *>(&sm.ring[c & 1][i / V][lane]) + i % V) : 0.0f;
+                const bool in = there && v >= bound;                // it may have risen
+                const unsigned votes = __ballot_sync(0xffffffffu, in);
+                if (in) sm.found[n + __popc(votes & ((1u << lane) - 1))] = (uint64_t)ordered(v) << 32 | (uint32_t)~e;
+                n += __popc(votes);
+                hits &= hits - 1;
+                if (n >= 32) { n -= 32; merge(n, 32); }
+            }
+            if (n) merge(0, n);
+            // later chunks have higher indices: an equal one is no better
+            const uint64_t last = __shfl_sync(0xffffffffu, best, top - 1);
+            bound = last ? value_of((uint32_t)(last >> 32) + 1) : -INFINITY;
+        }
+        // the lanes' sums, relative to their largest maximum
+        float big = m;
+#pragma unroll
+        for (int k = 16; k > 0; k >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, k));
+        const float d = s != 0.0f ? fmaxf(m - big, -150.0f) : 0.0f, f = expf(d);
+        t = warp_sum(f * __fmaf_rn(s, d, t));
+        s = warp_sum(f * s);
+        if (lane == 0) part_out[at] = Part{big, s, t, 0.0f};
+        if (top == 1)
+#pragma unroll
+            for (int k = 16; k > 0; k >>= 1) {
+                const uint64_t o = __shfl_xor_sync(0xffffffffu, best, k);
+                best = o > best ? o : best;
+            }
+        if (lane < top) keys_out[(int64_t)at * top + lane] = best;
     }
 }
 
-// One CTA per row: the parts' sums (first warp) beside the best of their lists.  The largest of the parts' last keys is no higher than the row's top-th key, which leaves few
-// keys to rank.
-constexpr int kJoin = 128, kHeld = 8;           // threads; keys a thread holds
+// One CTA per row: the segments' sums (first warp) beside the best of their lists.  Where q segments have a j-th key from some key on, q j keys are from there on: with
+// q j >= top, the q-th largest of the j-th keys leaves few more than `top` keys to rank.  One such j, with q at most half the segments, and j = top do where the best are
+// spread over the row or lie together; where more than the list holds are left after these, all powers of two are tried.
+constexpr int kJoin = 128;
 template <typename T>
-__global__ void __launch_bounds__(kJoin) logprobs_join_kernel(const T *logits, int64_t stride, int vocab, int parts, int top, const Part *part_in,
-                                                              const uint64_t *keys_in, const Out o) {
+__global__ void __launch_bounds__(kJoin) logprobs_join_kernel(const T *logits, int64_t stride, int vocab, int segments, int top, const Part *part_in, const uint64_t *keys_in,
+                                                              const Out o) {
     __shared__ float row_m, row_s;
-    __shared__ uint64_t least_of[kJoin / 32];
+    __shared__ __align__(16) uint32_t firsts[kMaxSegments];
+    __shared__ uint64_t least;
     __shared__ uint64_t list[kList];
     __shared__ int count;
     const int64_t r = blockIdx.x;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, all = parts * top;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, all = segments * top;
     cq_pdl_launch_dependents();
     cq_pdl_wait();
-    const Part *part = part_in + r * parts;
+    const Part *part = part_in + r * segments;
     const uint64_t *keys = keys_in + r * all;
-    // what every row needs is asked for at once
-    uint64_t k[kHeld];
-#pragma unroll
-    for (int i = 0; i < kHeld; ++i) k[i] = tid + i * kJoin < all ? keys[tid + i * kJoin] : 0;
+    const int j0 = top ? min(top, (2 * top + segments - 1) / segments) : 0;
+    // the q-th largest value among the segments' j-th keys into `least`, if it is larger
+    auto raise = [&](int j) {
+        const uint32_t mine = tid < segments ? (uint32_t)(keys[tid * top + j - 1] >> 32) : 0;
+        __syncthreads();
+        firsts[tid] = mine;
+        __syncthreads();
+        int rank = 0;
+#pragma unroll 2
+        for (int i = 0; i < segments; i += 4) {
+            const uint4 v = *reinterpret_cast<const uint4 *>(&firsts[i]);
+            rank += (v.x > mine || (v.x == mine && i < tid)) + (v.y > mine || (v.y == mine && i + 1 < tid)) + (v.z > mine || (v.z == mine && i + 2 < tid)) +
+                    (v.w > mine || (v.w == mine && i + 3 < tid));
+        }
+        if (tid < segments && rank == (top + j - 1) / j - 1) atomicMax((unsigned long long *)&least, (unsigned long long)mine << 32);
+    };
+    if (tid == 0) { count = 0; least = 0; }
+    if (top > 1) {
+        raise(j0);
+        if (j0 < top && tid < segments) atomicMax((unsigned long long *)&least, (unsigned long long)keys[tid * top + top - 1]);
+    }
     if (warp == 0) {
         const int64_t tok = o.tokens ? o.tokens[r] : -1;
         const float at_tok = tok >= 0 && tok < vocab ? load_f(logits + r * stride + tok) : 0.0f;
+        Part a[kMaxSegments / 32];
         float m = -INFINITY, s = 0.0f, t = 0.0f;
-        const Part first = lane < parts ? part[lane] : Part{-INFINITY, 0.0f, 0.0f, 0.0f};
-        m = first.m;
-        for (int p = lane + 32; p < parts; p += 32) m = fmaxf(m, part[p].m);
+#pragma unroll
+        for (int i = 0; i < kMaxSegments / 32; ++i) {
+            a[i] = lane + 32 * i < segments ? part[lane + 32 * i] : Part{-INFINITY, 0.0f, 0.0f, 0.0f};
+            m = fmaxf(m, a[i].m);
+        }
 #pragma unroll
         for (int x = 16; x > 0; x >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
-        for (int p = lane; p < parts; p += 32) {
-            const Part a = p == lane ? first : part[p];
-            if (a.s != 0.0f) {                              // nothing but -inf: no weight, and no difference of infinities
-                const float d = fmaxf(a.m - m, -150.0f), f = expf(d);       // the difference of two finite values may be -inf
-                s = __fmaf_rn(f, a.s, s);
-                t = __fmaf_rn(f, __fmaf_rn(a.s, d, a.t), t);
+#pragma unroll
+        for (int i = 0; i < kMaxSegments / 32; ++i)
+            if (a[i].s != 0.0f) {                               // nothing but -inf: no weight, and no difference of infinities
+                const float d = fmaxf(a[i].m - m, -150.0f), f = expf(d);        // the difference of two finite values may be -inf
+                s = __fmaf_rn(f, a[i].s, s);
+                t = __fmaf_rn(f, __fmaf_rn(a[i].s, d, a[i].t), t);
             }
-        }
         s = warp_sum(s);
         t = warp_sum(t);
         if (lane == 0) {
@@ -281,63 +336,90 @@ __global__ void __launch_bounds__(kJoin) logprobs_join_kernel(const T *logits, i
         }
     }
     if (top == 0) return;
-    uint64_t least = 0;
-#pragma unroll
-    for (int i = 0; i < kHeld; ++i) least = (tid + i * kJoin) % top == top - 1 && k[i] > least ? k[i] : least;
-    for (int i = tid + kHeld * kJoin; i < all; i += kJoin) least = i % top == top - 1 && keys[i] > least ? keys[i] : least;
-    least = warp_max(least);
-    if (lane == 0) least_of[warp] = least;
-    if (tid == 0) count = 0;
     __syncthreads();
-    least = least_of[0];
-#pragma unroll
-    for (int i = 1; i < kJoin / 32; ++i) least = least_of[i] > least ? least_of[i] : least;
     const float m = row_m, s = row_s, ls = logf(s);
     const bool ok = s > 0.0f && m < INFINITY;
     if (!ok) {
         if (tid < top) write_top(o, r, top, tid, 0, false, m, ls);
         return;
     }
-    auto take = [&](uint64_t key) {
-        if (key >= least && key != 0) {
-            const int at = atomicAdd(&count, 1);
-            if (at < kList) list[at] = key;
+    if (top == 1) {
+        const uint64_t key = tid < segments ? keys[tid] : 0;
+        atomicMax((unsigned long long *)&least, (unsigned long long)key);
+        __syncthreads();
+        if (tid == 0) write_top(o, r, 1, 0, least, true, m, ls);
+        return;
+    }
+    auto collect = [&]() {
+        const uint64_t from_here = least;
+        for (int i = tid; i < all; i += kJoin) {
+            const uint64_t key = keys[i];
+            if (key >= from_here && key != 0) {
+                const int at = atomicAdd(&count, 1);
+                if (at < kList) list[at] = key;
+            }
         }
+        __syncthreads();
     };
-#pragma unroll
-    for (int i = 0; i < kHeld; ++i) take(k[i]);
-    for (int i = tid + kHeld * kJoin; i < all; i += kJoin) take(keys[i]);
-    __syncthreads();
-    // keys differ, so at most (parts - 1) * (top - 1) + top of them are not below `least`; where the list is too short for that, all are ranked
-    const int n = count;
+    collect();
+    if (count > kList) {
+        for (int j = 1; j < top; j *= 2) raise(j);
+        __syncthreads();
+        if (tid == 0) count = 0;
+        __syncthreads();
+        collect();
+    }
+    const uint64_t from_here = least;
+    const int n = count;                        // still too many for the list: all are ranked
     const uint64_t *from = n <= kList ? list : keys;
     const int total = n <= kList ? n : all;
     for (int i = tid; i < total; i += kJoin) {
         const uint64_t key = from[i];
-        if (key < least || key == 0) continue;
+        if (key < from_here || key == 0) continue;
         int rank = 0;
-        for (int j = 0; j < total; ++j) rank += from[j] > key;
+#pragma unroll 4
+        for (int x = 0; x < total; ++x) rank += from[x] > key;
         if (rank < top) write_top(o, r, top, rank, key, ok, m, ls);
     }
 }
 
-int parts_of(int vocab) { return (int)(((int64_t)vocab + 8 + kPart - 1) / kPart); }        // + 8: a row may start inside a 16-byte unit
+int chunks_of(int vocab) { return (int)(((int64_t)vocab + 8 + kChunk - 1) / kChunk); }     // + 8: a row may start inside a 16-byte unit
+
+// Segments of a row: one for every warp that the device holds, or, with more rows than warps, the number up to eight that leaves the fewest chunks to the busiest warp.
+int segments_of(int rows, int vocab) {
+    const int chunks = chunks_of(vocab), warps = kCtas * kWarps * cq_sm_count();
+    int s = rows <= warps ? warps / rows : 1;
+    if (rows > warps) {
+        int64_t least = INT64_MAX;
+        for (int x = 1; x <= 8; ++x) {
+            const int64_t cost = ((int64_t)rows * x + warps - 1) / warps * ((chunks + x - 1) / x);
+            if (cost < least) { least = cost; s = x; }
+        }
+    }
+    if (s > chunks) s = chunks;
+    if (s > kMaxSegments) s = kMaxSegments;
+    const int per = (chunks + s - 1) / s;
+    return (chunks + per - 1) / per;
+}
 
 template <typename T>
 void launch(const void *logits, int64_t stride, int rows, int vocab, int top, const Out &o, void *scratch, cudaStream_t st) {
-    const int parts = parts_of(vocab);
+    const int segments = segments_of(rows, vocab), per = (chunks_of(vocab) + segments - 1) / segments, total = rows * segments;
     Part *part = reinterpret_cast<Part *>(scratch);
-    uint64_t *keys = reinterpret_cast<uint64_t *>(part + (int64_t)rows * parts);
-    cq_launch_k(logprobs_part_kernel<T>, dim3((unsigned)((int64_t)rows * parts)), dim3(kThreads), 0, st, (const T *)logits, stride, vocab, parts, top, part, keys);
-    cq_launch_k(logprobs_join_kernel<T>, dim3((unsigned)rows), dim3(kJoin), 0, st, (const T *)logits, stride, vocab, parts, top, (const Part *)part,
-                (const uint64_t *)keys, o);
+    uint64_t *keys = reinterpret_cast<uint64_t *>(part + total);
+    constexpr int smem = kWarps * (int)sizeof(Warp<T>);
+    cudaFuncSetAttribute(logprobs_segment_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    const int most = kCtas * cq_sm_count(), want = (total + kWarps - 1) / kWarps;
+    cq_launch_k(logprobs_segment_kernel<T>, dim3((unsigned)(want < most ? want : most)), dim3(kThreads), smem, st, (const T *)logits, stride, vocab, segments, per, total, top, part,
+                keys);
+    cq_launch_k(logprobs_join_kernel<T>, dim3((unsigned)rows), dim3(kJoin), 0, st, (const T *)logits, stride, vocab, segments, top, (const Part *)part, (const uint64_t *)keys, o);
 }
 
 }  // namespace
 
 extern "C" size_t cq_token_logprobs_scratch_bytes(int rows, int vocab, int top) {
-    if (rows <= 0 || vocab <= 0 || top < 0 || top > kMaxTop || top > vocab || (int64_t)rows * parts_of(vocab) > INT32_MAX) return 0;
-    return (size_t)rows * parts_of(vocab) * (sizeof(Part) + 8 * (size_t)top);
+    if (rows <= 0 || vocab <= 0 || vocab > (1 << 30) || top < 0 || top > kMaxTop || top > vocab || (int64_t)rows * kMaxSegments > (1 << 30)) return 0;
+    return (size_t)rows * segments_of(rows, vocab) * (sizeof(Part) + 8 * (size_t)top);
 }
 
 extern "C" void cq_token_logprobs(const void *logits, int elem, int64_t row_stride, int rows, int vocab, const int64_t *tokens, int top, float *logprob, float *entropy,
@@ -347,7 +429,7 @@ extern "C" void cq_token_logprobs(const void *logits, int elem, int64_t row_stri
         cq_set_status(CQ_ERR_BAD_ARG, "token_logprobs: null or misaligned pointer, or an element type that is not f32, f16 or bf16");
         return;
     }
-    if (cq_token_logprobs_scratch_bytes(rows, vocab, top) == 0 || row_stride < 0 || vocab > (1 << 30)) {
+    if (cq_token_logprobs_scratch_bytes(rows, vocab, top) == 0 || row_stride < 0) {
         cq_set_status(CQ_ERR_BAD_ARG, "token_logprobs: rows and vocab must be positive, 0 <= top <= min(32, vocab)");
         return;
     }

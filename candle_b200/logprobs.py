@@ -48,12 +48,12 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor | None = None, top
     ids = torch.empty((rows, top), dtype=torch.int64, device=dev)
     if rows:
         lib = capi.lib()
-        nbytes = lib.cq_token_logprobs_scratch_bytes(rows, vocab, top)
-        if nbytes == 0:
-            raise CandleQError(f"token_logprobs: {rows} rows of {vocab} are too many for one call")
-        scratch = torch.empty(nbytes, dtype=torch.uint8, device=dev)
         ptr = lambda t: None if t is None else t.data_ptr()
         with capi.on_device(dev):
+            nbytes = lib.cq_token_logprobs_scratch_bytes(rows, vocab, top)
+            if nbytes == 0:
+                raise CandleQError(f"token_logprobs: {rows} rows of {vocab} are too many for one call")
+            scratch = torch.empty(nbytes, dtype=torch.uint8, device=dev)
             lib.cq_token_logprobs(x.data_ptr(), _ELEM[x.dtype], x.stride(0) if rows > 1 else vocab, rows, vocab, ptr(tokens), top, ptr(logprob), entropy.data_ptr(),
                                   best.data_ptr(), ids.data_ptr(), scratch.data_ptr(), capi.stream_of(dev))
         capi.check("token_logprobs")

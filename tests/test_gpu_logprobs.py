@@ -58,6 +58,17 @@ def test_ties_and_masked_logits(cuda_dev, dtype, vocab):
     assert float(got.logprob[1]) == 0.0 and float(got.entropy[1]) == 0.0 and float(got.logprob[2]) == -float("inf")
 
 
+@pytest.mark.parametrize("rows", [1, 70])
+def test_where_the_best_lie(cuda_dev, rows):
+    """Together, at the row's ends, one in each part of it, ascending, with everything else masked: the search must not depend on it."""
+    vocab, g = 150000, torch.Generator(device="cuda").manual_seed(rows)
+    at = torch.arange(vocab, device="cuda")
+    for values in (torch.where((at >= 5000) & (at < 5040), 1.0 + at / vocab, -torch.inf), torch.where(at % 4000 == 17, at / vocab, -3.0),
+                   at / vocab, -at / vocab, torch.where(at % 1024 < 20, 2.0, torch.where(at > vocab - 9, 3.0, 0.0)), torch.where(at < 31, 1.0, -torch.inf)):
+        x = values.float().repeat(rows, 1)
+        _check(x, torch.randint(0, vocab, (rows,), device="cuda", generator=g), 32)
+
+
 def test_rows_without_a_distribution(cuda_dev):
     x = torch.randn((5, 9000), device="cuda")
     good = token_logprobs(x, torch.zeros(5, dtype=torch.int64, device="cuda"), 4)
