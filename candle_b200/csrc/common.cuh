@@ -116,6 +116,14 @@ static inline cudaError_t cq_launch_cluster_k(void (*kernel)(P...), dim3 grid, d
     return cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(a)...);
 }
 
+// Lets `fn` have `bytes` of dynamic shared memory on the current device; `done` is one flag per device, so that the driver is asked once (1.5 us a call).
+static inline void cq_smem_once(const void *fn, int bytes, bool (&done)[64]) {
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) { (void)cudaGetLastError(); dev = -1; }
+    if (dev >= 0 && done[dev]) return;
+    if (cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) == cudaSuccess && dev >= 0) done[dev] = true;
+}
+
 // SMs of the current device (148 when it cannot be asked).
 static inline int cq_sm_count() {
     static int sms[64] = {};

@@ -408,7 +408,8 @@ void launch(const void *logits, int64_t stride, int rows, int vocab, int top, co
     Part *part = reinterpret_cast<Part *>(scratch);
     uint64_t *keys = reinterpret_cast<uint64_t *>(part + total);
     constexpr int smem = kWarps * (int)sizeof(Warp<T>);
-    cudaFuncSetAttribute(logprobs_segment_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    static bool done[64];
+    cq_smem_once((const void *)logprobs_segment_kernel<T>, smem, done);
     const int most = kCtas * cq_sm_count(), want = (total + kWarps - 1) / kWarps;
     cq_launch_k(logprobs_segment_kernel<T>, dim3((unsigned)(want < most ? want : most)), dim3(kThreads), smem, st, (const T *)logits, stride, vocab, segments, per, total, top, part,
                 keys);

@@ -629,7 +629,8 @@ bool part_map(const Call &c, CUtensorMap &out) {
 template <int D, bool BF16>
 void launch(const Call &c, const cq_kv_cache &cache, const CUtensorMap (&m)[3], const uint8_t *k, const uint8_t *v, const void *q, int64_t q_stride, float scale, cudaStream_t st) {
     constexpr int smem = (int)sizeof(Tiles<D>) + 1024;
-    cudaFuncSetAttribute(prefix_mma_kernel<D, BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    static bool done[64];
+    cq_smem_once((const void *)prefix_mma_kernel<D, BF16>, smem, done);
     cq_launch_k(prefix_mma_kernel<D, BF16>, dim3(c.sh.ctas), dim3(kThreads), smem, st, cache, c, m[0], m[1], m[2], k, v, (const uint8_t *)q, q_stride,
                 (float)(scale * 1.4426950408889634));
 }

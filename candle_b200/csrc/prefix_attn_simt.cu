@@ -173,7 +173,8 @@ __global__ void __launch_bounds__(kThreads) prefix_simt_kernel(const cq_kv_cache
 
 template <typename T, int D>
 void launch(const Call &c, const cq_kv_cache &cache, int layer, const void *q, int64_t q_stride, float scale, cudaStream_t st) {
-    cudaFuncSetAttribute(prefix_simt_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(Smem<D>));
+    static bool done[64];
+    cq_smem_once((const void *)prefix_simt_kernel<T, D>, (int)sizeof(Smem<D>), done);
     cq_launch_k(prefix_simt_kernel<T, D>, dim3(c.sh.ctas), dim3(kThreads), sizeof(Smem<D>), st, cache, c, layer, (const T *)q, q_stride,
                 (float)(scale * 1.4426950408889634));
 }

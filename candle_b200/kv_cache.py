@@ -56,6 +56,7 @@ class PagedKvCache:
                 raise CandleQError(f"PagedKvCache: the pools must be contiguous CUDA tensors {list(shape)} of {dtype}")
         self.k, self.v = pools
         self.device = self.k.device
+        self._index = self.device.index
         lib = capi.lib()
         # rounded up, so that a view of everything keeps its alignment
         self.state = torch.zeros(capi.pad(lib.cq_kv_state_ints(pages, max_seqs, max_pages), 4), dtype=torch.int32, device=self.device)
@@ -72,13 +73,19 @@ class PagedKvCache:
 
     # ---- helpers ----
     def _call(self, fn, *args) -> None:
-        with capi.on_device(self.device):
+        if torch.cuda.current_device() == self._index:
             fn(self._p, *args, capi.stream_of(self.device))
+        else:
+            with torch.cuda.device(self.device):
+                fn(self._p, *args, capi.stream_of(self.device))
         capi.check("PagedKvCache")
 
     def slot_list(self, slots) -> torch.Tensor:
         """Slots as the device reads them: int32, contiguous, on the cache's device.  Such a tensor is taken as it is."""
-        if not isinstance(slots, torch.Tensor):
+        if isinstance(slots, torch.Tensor):
+            if slots.dtype == torch.int32 and slots.device == self.device and slots.dim() == 1 and slots.is_contiguous() and slots.shape[0] <= self.max_seqs:
+                return slots
+        else:
             slots = [slots] if isinstance(slots, int) else list(slots)
             if any(not 0 <= int(s) < self.max_seqs for s in slots):
                 raise CandleQError(f"PagedKvCache: slots are 0 .. {self.max_seqs - 1}")
@@ -135,15 +142,17 @@ class PagedKvCache:
     # ---- keys and values ----
     def _rows(self, t: torch.Tensor, name: str, batch: int, heads: int | None, tokens: int | None):
         """`t` as [batch, tokens, heads, head_dim] with heads side by side and aligned rows at one distance; (tensor, row distance)."""
-        if t.dim() != 4 or t.shape[0] != batch or t.shape[3] != self.head_dim or (heads is not None and t.shape[2] != heads) or \
-                (tokens is not None and t.shape[1] != tokens) or t.device != self.device:
-            raise CandleQError(f"PagedKvCache: {name} must be [batch, tokens, heads, {self.head_dim}] on {self.device}, got {list(t.shape)}")
-        es, d = t.element_size(), self.head_dim
-        stride = t.stride(1) if t.shape[1] > 1 else t.stride(0)
-        if t.stride(3) != 1 or (t.shape[2] > 1 and t.stride(2) != d) or stride < t.shape[2] * d or (t.shape[0] > 1 and t.stride(0) != stride * t.shape[1]) or \
-                stride * es % 16 or t.data_ptr() % 16:
-            t = t.contiguous() if not t.is_contiguous() else t.clone()
-            stride = t.shape[2] * d
+        shape, d = t.shape, self.head_dim
+        if len(shape) != 4 or shape[0] != batch or shape[3] != d or (heads is not None and shape[2] != heads) or (tokens is not None and shape[1] != tokens) or \
+                t.device != self.device:
+            raise CandleQError(f"PagedKvCache: {name} must be [batch, tokens, heads, {d}] on {self.device}, got {list(shape)}")
+        width = shape[2] * d
+        if t.is_contiguous():
+            return (t if t.data_ptr() % 16 == 0 else t.clone()), width
+        stride = t.stride(1) if shape[1] > 1 else t.stride(0)
+        if t.stride(3) != 1 or (shape[2] > 1 and t.stride(2) != d) or stride < width or (batch > 1 and t.stride(0) != stride * shape[1]) or \
+                stride * t.element_size() % 16 or t.data_ptr() % 16:
+            return t.contiguous(), width
         return t, stride
 
     def append(self, layer: int, slots, k: torch.Tensor, v: torch.Tensor, q: torch.Tensor | None = None, rotary=None, neox: bool = False):
@@ -155,7 +164,7 @@ class PagedKvCache:
             raise CandleQError(f"PagedKvCache.append: layer {layer} of {self.layers}")
         if k.dtype not in _ELEM or v.dtype != k.dtype or (q is not None and q.dtype != k.dtype):
             raise CandleQError("PagedKvCache.append: q, k and v must be of one type, f32, f16 or bf16")
-        b = s.numel()
+        b = s.shape[0]
         if b == 0 or k.dim() != 4 or k.shape[1] == 0:
             raise CandleQError("PagedKvCache.append: no slots or no tokens")
         k, ks = self._rows(k, "k", b, self.kv_heads, None)
@@ -172,9 +181,9 @@ class PagedKvCache:
                 if t.dtype != torch.float32 or t.dim() != 2 or t.shape[1] != self.head_dim // 2 or t.shape[0] != cos.shape[0] or t.shape[0] == 0 or \
                         not t.is_contiguous() or t.device != self.device or t.data_ptr() % 16:
                     raise CandleQError(f"PagedKvCache.append: rotary tables must be contiguous, aligned f32 [positions, {self.head_dim // 2}] on {self.device}")
-        ptr = lambda t: None if t is None else t.data_ptr()
-        self._call(capi.lib().cq_kv_append, layer, s.data_ptr(), b, k.shape[1], ptr(q), k.data_ptr(), v.data_ptr(), _ELEM[k.dtype], heads, qs, ks, vs, ptr(cos),
-                   ptr(sin), 0 if cos is None else cos.shape[0], int(neox), ptr(out))
+        self._call(capi.lib().cq_kv_append, layer, s.data_ptr(), b, k.shape[1], None if q is None else q.data_ptr(), k.data_ptr(), v.data_ptr(), _ELEM[k.dtype], heads, qs,
+                   ks, vs, None if cos is None else cos.data_ptr(), None if sin is None else sin.data_ptr(), 0 if cos is None else cos.shape[0], int(neox),
+                   None if out is None else out.data_ptr())
         return out
 
     # ---- attention ----

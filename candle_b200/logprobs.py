@@ -31,30 +31,35 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor | None = None, top
         raise CandleQError("token_logprobs needs CUDA logits [..., vocab]: there is no CPU path")
     if logits.dtype not in _ELEM:
         raise CandleQError(f"Expected f32/f16/bf16, got {logits.dtype}")
-    lead, vocab = logits.shape[:-1], logits.shape[-1]
+    lead, vocab, dev = logits.shape[:-1], logits.shape[-1], logits.device
     if vocab == 0 or not 0 <= top <= min(32, vocab):
         raise CandleQError(f"token_logprobs: 0 <= top <= min(32, vocab), got {top} of {vocab}")
-    x = logits.reshape(-1, vocab) if logits.dim() != 2 else logits
-    rows, dev = x.shape[0], logits.device
-    if x.stride(1) != 1 and vocab > 1 or (rows > 1 and x.stride(0) < 0):
-        x = x.contiguous()
+    flat = len(lead) == 1
+    x = logits if flat else logits.reshape(-1, vocab)
+    rows, step = x.shape[0], x.stride(0)
+    if (x.stride(1) != 1 and vocab > 1) or (rows > 1 and step < 0):
+        x, step = x.contiguous(), vocab
     if tokens is not None:
         if tokens.shape != lead or tokens.is_floating_point() or tokens.dtype == torch.bool or tokens.device != dev:
             raise CandleQError(f"token_logprobs: tokens must be whole numbers of shape {list(lead)} on {dev}")
-        tokens = tokens.reshape(-1).to(torch.int64).contiguous()
-    f32 = dict(dtype=torch.float32, device=dev)
-    logprob = None if tokens is None else torch.empty(rows, **f32)
-    entropy, best = torch.empty(rows, **f32), torch.empty((rows, top), **f32)
+        if not flat:
+            tokens = tokens.reshape(-1)
+        if tokens.dtype != torch.int64 or not tokens.is_contiguous():
+            tokens = tokens.to(torch.int64).contiguous()
+    logprob = None if tokens is None else torch.empty(rows, dtype=torch.float32, device=dev)
+    entropy, best = torch.empty(rows, dtype=torch.float32, device=dev), torch.empty((rows, top), dtype=torch.float32, device=dev)
     ids = torch.empty((rows, top), dtype=torch.int64, device=dev)
     if rows:
         lib = capi.lib()
-        ptr = lambda t: None if t is None else t.data_ptr()
         with capi.on_device(dev):
             nbytes = lib.cq_token_logprobs_scratch_bytes(rows, vocab, top)
             if nbytes == 0:
                 raise CandleQError(f"token_logprobs: {rows} rows of {vocab} are too many for one call")
             scratch = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-            lib.cq_token_logprobs(x.data_ptr(), _ELEM[x.dtype], x.stride(0) if rows > 1 else vocab, rows, vocab, ptr(tokens), top, ptr(logprob), entropy.data_ptr(),
-                                  best.data_ptr(), ids.data_ptr(), scratch.data_ptr(), capi.stream_of(dev))
+            lib.cq_token_logprobs(x.data_ptr(), _ELEM[x.dtype], step if rows > 1 else vocab, rows, vocab, None if tokens is None else tokens.data_ptr(), top,
+                                  None if logprob is None else logprob.data_ptr(), entropy.data_ptr(), best.data_ptr(), ids.data_ptr(), scratch.data_ptr(),
+                                  capi.stream_of(dev))
         capi.check("token_logprobs")
+    if flat:
+        return TokenLogProbs(logprob, entropy, best, ids)
     return TokenLogProbs(None if logprob is None else logprob.view(lead), entropy.view(lead), best.view(*lead, top), ids.view(*lead, top))
