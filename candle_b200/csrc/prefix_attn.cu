@@ -138,7 +138,7 @@ __global__ void __launch_bounds__(kThreads) prefix_plan_kernel(const cq_kv_cache
     for (int i0 = 0; i0 < max(nq, sh.groups); i0 += kThreads) {
         const int i = i0 + tid;
         int n_shared = 0, units = 0;
-        if (i < sh.groups) n_shared = ((shared_of(i) + kKeyTile - 1) / kKeyTile) * hkv * pl.shapes[i].row_tiles;
+        if (i < sh.groups) n_shared = ((shared_of(i) + sh.tile - 1) / sh.tile) * hkv * pl.shapes[i].row_tiles;
         if (i < nq) {
             const int b = t == 1 ? i : i / t, len = len_of[b], shared = len >= t ? shared_of(group_of[b]) : 0, n = len - t + 1 + (i - b * t);
             units = n > shared ? (n - shared + (1 << sh.own_shift) - 1) >> sh.own_shift : 0;
@@ -157,7 +157,7 @@ __global__ void __launch_bounds__(kThreads) prefix_plan_kernel(const cq_kv_cache
     auto group_at = [&](int g) {
         const GroupShape gs = pl.shapes[g];
         const int shared = shared_of(g);
-        return Group{(shared + kKeyTile - 1) / kKeyTile, shared, count_of[g] ? slot_of[first_of[g]] : -1, group_start[g], gs.query0, gs.rows, gs.item0, gs.row_tiles};
+        return Group{(shared + sh.tile - 1) / sh.tile, shared, count_of[g] ? slot_of[first_of[g]] : -1, group_start[g], gs.query0, gs.rows, gs.item0, gs.row_tiles};
     };
     // records, dealt out one a CTA: of the workers, the queries, the groups
     const int workers = sh.ctas + sh.own_workers;
@@ -223,7 +223,7 @@ template <typename T, int D> __global__ void __launch_bounds__(256) prefix_join_
     cq_pdl_wait();
     const int lane = threadIdx.x & 31, per = sh.per_kv, n = blockIdx.y, hq = blockIdx.x * 8 + (threadIdx.x >> 5);
     if (hq >= sh.heads) return;
-    const int h = div_per(hq, sh), in = hq - h * per, tile = in / sh.own_rows;          // own_rows: 8 or 32
+    const int h = div_per(hq, sh), in = hq - h * per, tile = in / sh.own_rows;
     const int64_t row = (int64_t)n * sh.heads + hq;
     const Query q = pl.query[n];
     const int chunk = pl.header[1], own_chunk = pl.header[3], own_chunk2 = pl.header[4];
@@ -323,8 +323,10 @@ bool shape_ok(const cq_kv_cache *cache, const cq_prefix_plan *p, const char *who
     }
     s = Shape{p->batch, p->queries, p->heads, cache->kv_heads, p->groups, cache->head_dim, cache->elem, p->heads / cache->kv_heads};
     s.ctas = p->ctas;
-    if (cache->elem == CQ_F32) { s.row_tile = s.own_rows = 32; s.own_shift = 6; s.own_workers = s.own_first = s.ctas; }
-    else { s.row_tile = 256; s.own_rows = 8; s.own_shift = 4; s.own_first = s.ctas * kMmaWarps; s.own_workers = s.own_first + s.ctas * kMmaHelpers; }
+    s.own_rows = 8;
+    s.own_shift = 4;
+    if (cache->elem == CQ_F32) { s.row_tile = 8; s.tile = 64; s.own_workers = s.own_first = s.ctas; }
+    else { s.row_tile = 256; s.tile = 128; s.own_first = s.ctas * kMmaWarps; s.own_workers = s.own_first + s.ctas * kMmaHelpers; }
     s.own_tiles = (s.per_kv + s.own_rows - 1) / s.own_rows;
     if (s.per_kv > 1) s.rcp = (unsigned)(((1ull << 32) + s.per_kv - 1) / s.per_kv);
     return true;
@@ -354,7 +356,7 @@ bool plan_ready(const cq_prefix_plan *p, const Shape &s, const char *who) {
 extern "C" int cq_prefix_plan_shape(const cq_kv_cache *cache, cq_prefix_plan *plan, const int *group_sizes, int *shapes) {
     Shape s;
     if (!shape_ok(cache, plan, "prefix_plan_shape", s)) return 1;
-    s.ctas = plan->ctas = (s.elem == CQ_F32 ? 2 : 1) * cq_sm_count();
+    s.ctas = plan->ctas = (s.elem == CQ_F32 ? f32_warps(s.head_dim) : 1) * cq_sm_count();
     s.own_first = s.elem == CQ_F32 ? s.ctas : s.ctas * kMmaWarps;
     s.own_workers = s.own_first + (s.elem == CQ_F32 ? 0 : s.ctas * kMmaHelpers);
     int64_t items = 0, seqs = 0;
@@ -397,7 +399,7 @@ extern "C" void cq_prefix_attention(const cq_kv_cache *cache, int layer, const c
     }
     const Call c = call_of(plan, s);
     cudaStream_t st = (cudaStream_t)stream;
-    if (s.elem == CQ_F32) simt_launch(c, *cache, layer, q, q_stride, scale, st);
+    if (s.elem == CQ_F32) f32_launch(c, *cache, layer, q, q_stride, scale, st);
     else if (!mma_launch(c, *cache, layer, q, q_stride, scale, st)) return;
     if (s.head_dim == 128) join_launch<128>(c, out, st);
     else join_launch<64>(c, out, st);

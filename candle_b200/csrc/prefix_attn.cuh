@@ -4,16 +4,14 @@
 // rows of consecutive sequences are consecutive.  Two kinds of items cover all (row, key) pairs:
 //   shared : up to `row_tile` rows of one group of sequences x one KV head x the keys of the pages that all of them share;
 //   own    : up to `own_rows` rows of one query x one KV head x the keys behind these pages.
-// An item is a number of units (128 keys of a shared item, 2^own_shift keys of an own one); the units of all items of a kind form a line, which
-// its workers (CTAs for the shared items; CTAs or warps for the own ones) take in equal parts.  A part of an item that one worker takes
+// An item is a number of units (`tile` keys of a shared item, 2^own_shift of an own one); the units of all items of a kind form a line, which
+// its workers (CTAs or warps) take in equal parts.  A part of an item that one worker takes
 // is a segment; it leaves (maximum, sum, unnormalised output) per row, and a second kernel joins a row's segments in the order of their keys:
 // m = max m_i,  l = sum 2^(m_i - m) l_i,  o = sum 2^(m_i - m) o_i / l.
 #pragma once
 #include "kv_cache.cuh"
 
 namespace cq_attn {
-
-constexpr int kKeyTile = 128;       // keys of a shared unit
 
 struct Segment {
     int row0, rows;         // rows of the KV head
@@ -38,7 +36,8 @@ struct GroupShape { int query0, rows, item0, row_tiles; };
 
 struct Shape {
     int batch, queries, heads, kv_heads, groups, head_dim, elem, per_kv;
-    int row_tile, ctas, own_rows, own_shift;                    // 2^own_shift keys an own unit
+    int row_tile, tile, ctas;                                   // rows of a shared item, keys of a unit of it (a multiple of the largest page or a part of the smallest), workers
+    int own_rows, own_shift;                                    // rows of an own item, 2^own_shift keys a unit
     int own_workers, own_first;                                 // workers of the own line; the first own_first have chunks of one size, the others of another
     int own_tiles;          // row tiles of a KV head's query heads
     unsigned rcp;           // ceil(2^32 / query heads per KV head); 0 for one
@@ -121,8 +120,8 @@ struct SharedWalk {
         s.rows = min(sh.row_tile, g.rows - tile * sh.row_tile);
         s.slot = g.slot;
         s.units = min(left, g.units - unit);
-        s.key0 = unit * kKeyTile;
-        s.key1 = min(g.shared, (unit + s.units) * kKeyTile);
+        s.key0 = unit * sh.tile;
+        s.key1 = min(g.shared, (unit + s.units) * sh.tile);
         s.part = (int)part_shared(sh, g.item0 + head * g.row_tiles + tile + cta);
         left -= s.units;
         unit += s.units;
@@ -171,9 +170,10 @@ struct OwnWalk {
 // n / per for the rows of a call, by a multiplication: exact for n < 2^22, per <= 32, with rcp = ceil(2^32 / per)
 __device__ __forceinline__ int div_per(int n, const Shape &s) { return s.rcp ? (int)__umulhi((unsigned)n, s.rcp) : n; }
 
-// The kernels that make the segments' results (prefix_attn_simt.cu: f32; prefix_attn_mma.cu: f16 and bf16).
-void simt_launch(const Call &c, const cq_kv_cache &cache, int layer, const void *q, int64_t q_stride, float scale, cudaStream_t st);
+// The kernels that make the segments' results (prefix_attn_f32.cu: f32; prefix_attn_mma.cu: f16 and bf16).
+void f32_launch(const Call &c, const cq_kv_cache &cache, int layer, const void *q, int64_t q_stride, float scale, cudaStream_t st);
 bool mma_launch(const Call &c, const cq_kv_cache &cache, int layer, const void *q, int64_t q_stride, float scale, cudaStream_t st);
+constexpr int f32_warps(int head_dim) { return head_dim == 128 ? 6 : 12; }      // of a CTA of the former, one per SM: each is a worker of both lines
 constexpr int kMmaWarps = 4, kMmaHelpers = 8;       // warps of a CTA of the latter that are workers of the own line from the start, and after the shared items
 
 }  // namespace cq_attn

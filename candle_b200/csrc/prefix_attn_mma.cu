@@ -25,7 +25,7 @@ using namespace cq_prompt;
 
 // Warps: 0-3 and 4-7 softmax of a row tile's halves, 8 copies, 9 products, 12-15 own items.
 constexpr int kThreads = 512, kCopyWarp = kMmaHelpers, kMmaWarp = 9, kOwnWarp = 12;
-constexpr int kRing = 3, kCols = 512;                        // buffers that hold K, V, K, V, ... of the tiles in turn
+constexpr int kKeyTile = 128, kRing = 3, kCols = 512;                        // buffers that hold K, V, K, V, ... of the tiles in turn
 constexpr int kHalfBytes = 128 * 128;                        // 128 rows of 64 elements
 constexpr int kGroup = 256, kO = 128;                        // columns of a half; in it the scores / weights and the outputs
 constexpr int kStep = 16;                                    // keys of a step of an own item
