@@ -114,16 +114,32 @@ __global__ void __launch_bounds__(32 * f32_warps(D), 1) prefix_f32_kernel(const 
             float s[2][4] = {};
 #pragma unroll
             for (int x = 0; x < D / 8; ++x) {
-                uint32_t a[4], h[4], f[4], r[4];
+                uint32_t a[4], h[4], r[4];
                 ldsm(a, ka + 32 * x);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) { h[i] = high(a[i]); f[i] = finite_high(a[i]); r[i] = low(a[i]); }
+                for (int i = 0; i < 4; ++i) { h[i] = high(a[i]); r[i] = __float_as_uint(__uint_as_float(a[i]) - __uint_as_float(h[i])); }
                 mma(s[x & 1], r, qh[x][0], qh[x][1]);
-                mma(s[x & 1], f, ql[x][0], ql[x][1]);
+                mma(s[x & 1], h, ql[x][0], ql[x][1]);
                 mma(s[x & 1], h, qh[x][0], qh[x][1]);
             }
 #pragma unroll
             for (int i = 0; i < 4; ++i) s[0][i] += s[1][i];
+            // An infinite key has a NaN for its low part: the scores once more, with care.
+            const float sum = s[0][0] + s[0][1] + s[0][2] + s[0][3];
+            if (__any_sync(0xffffffffu, sum != sum)) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) s[0][i] = 0.0f;
+#pragma unroll
+                for (int x = 0; x < D / 8; ++x) {
+                    uint32_t a[4], h[4], f[4], r[4];
+                    ldsm(a, ka + 32 * x);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) { h[i] = high(a[i]); f[i] = finite_high(a[i]); r[i] = low(a[i]); }
+                    mma(s[0], r, qh[x][0], qh[x][1]);
+                    mma(s[0], f, ql[x][0], ql[x][1]);
+                    mma(s[0], h, qh[x][0], qh[x][1]);
+                }
+            }
             if (g >= n) s[0][0] = s[0][1] = -INFINITY;
             if (g + 8 >= n) s[0][2] = s[0][3] = -INFINITY;
             float mx0 = fmaxf(s[0][0], s[0][2]), mx1 = fmaxf(s[0][1], s[0][3]);
@@ -162,21 +178,45 @@ __global__ void __launch_bounds__(32 * f32_warps(D), 1) prefix_f32_kernel(const 
                 pr[i] = low(w);
             }
 #pragma unroll
-            for (int x = 0; x < D / 16; ++x)
+            for (int x0 = 0; x0 < D / 16; x0 += 4) {            // 64 dims at a time
+                uint32_t w[4][2][4];
+                float care = 0.0f;                              // NaN if a value is not finite
 #pragma unroll
-                for (int y = 0; y < 2; ++y) {                   // keys 8 y .. 8 y + 7
-                    uint32_t h[4], f[4], r[4];
+                for (int x = 0; x < 4; ++x)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const uint32_t w = __float_as_uint(kv.v[8 * y + t + 4 * (i >> 1)][16 * x + g + 8 * (i & 1)]);
-                        h[i] = high(w);
-                        f[i] = finite_high(w);
-                        r[i] = low(w);
-                    }
-                    mma(o[x], r, ph[2 * y], ph[2 * y + 1]);
-                    mma(o[x], f, pr[2 * y], pr[2 * y + 1]);
-                    mma(o[x], h, ph[2 * y], ph[2 * y + 1]);
+                    for (int y = 0; y < 2; ++y)                 // keys 8 y .. 8 y + 7
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const float e = kv.v[8 * y + t + 4 * (i >> 1)][16 * (x0 + x) + g + 8 * (i & 1)];
+                            care = __fmaf_rn(e, 0.0f, care);
+                            w[x][y][i] = __float_as_uint(e);
+                        }
+                if (!__any_sync(0xffffffffu, care != care)) {
+#pragma unroll
+                    for (int x = 0; x < 4; ++x)
+#pragma unroll
+                        for (int y = 0; y < 2; ++y) {
+                            uint32_t h[4], r[4];
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) { h[i] = high(w[x][y][i]); r[i] = __float_as_uint(__uint_as_float(w[x][y][i]) - __uint_as_float(h[i])); }
+                            mma(o[x0 + x], r, ph[2 * y], ph[2 * y + 1]);
+                            mma(o[x0 + x], h, pr[2 * y], pr[2 * y + 1]);
+                            mma(o[x0 + x], h, ph[2 * y], ph[2 * y + 1]);
+                        }
+                } else {
+#pragma unroll
+                    for (int x = 0; x < 4; ++x)
+#pragma unroll
+                        for (int y = 0; y < 2; ++y) {
+                            uint32_t h[4], f[4], r[4];
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) { h[i] = high(w[x][y][i]); f[i] = finite_high(w[x][y][i]); r[i] = low(w[x][y][i]); }
+                            mma(o[x0 + x], r, ph[2 * y], ph[2 * y + 1]);
+                            mma(o[x0 + x], f, pr[2 * y], pr[2 * y + 1]);
+                            mma(o[x0 + x], h, ph[2 * y], ph[2 * y + 1]);
+                        }
                 }
+            }
             __syncwarp();
             load.send(steps[stage], cache, k_layer, v_layer, call, st, lane);
             if (++stage == kStages) stage = 0;

@@ -557,3 +557,24 @@ def test_a_sequence_can_come_and_go(cuda_dev):
     now = cache.attention(0, q, plan)
     keep = [0, 2, 3]
     assert torch.equal(now[keep], was[keep]) and float(now[1].abs().max()) == 0.0
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("dim", [64, 128])
+def test_infinite_values_and_plain_numbers(cuda_dev, dtype, dim):
+    """Queries, keys and values of few significant bits (1, 0.5, infinities): an infinity comes out as the formula has it, also where the other factor leaves
+    nothing behind its first bits."""
+    cache, slots, g = _batch(dtype, 16, dim, 1, [40], [[3, 3]], seed=3)
+    ids = cache.tables[slots[0], :3].long()
+    cache.k[0][cache.tables[slots, :3].long()] = 1.0
+    cache.v[0][cache.tables[slots, :3].long()] = 0.5
+    at = lambda s, n: (0, int(cache.tables[s, n // 16]), 0, n % 16)
+    cache.k[at(slots[0], 41)] = -math.inf            # this sequence's own key: a score of -inf, no weight
+    cache.v[at(slots[1], 42) + (5,)] = math.inf      # one value of the other's
+    q = torch.full((2, 1, 2, dim), 0.5, dtype=dtype, device="cuda")
+    plan = cache.attention_plan(2, 2)
+    plan.update(slots)
+    got = cache.attention(0, q, plan)
+    want = torch.full_like(got, 0.5)
+    want[1, :, :, 5] = math.inf
+    assert torch.equal(got, want)
