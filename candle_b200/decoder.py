@@ -17,10 +17,13 @@ from __future__ import annotations
 
 import dataclasses
 import math
+from typing import NamedTuple
 
 import torch
 
 from . import capi
+from .kv_cache import PagedKvCache
+from .logprobs import token_logprobs
 from .parallel import Gatherer, argmax_sharded, make_gatherer
 from .quantized import GgmlDType, QMatMul, QTensor
 from .synth import random_blocks
@@ -77,6 +80,12 @@ class _Layer:
     pass
 
 
+class Branches(NamedTuple):
+    tokens: torch.Tensor        # int64 [n, steps]
+    logprobs: torch.Tensor      # f32 [n, steps], of these tokens
+    entropy: torch.Tensor       # f32 [n, steps], of the distributions they were taken from
+
+
 class LlamaShapedDecoder:
     def __init__(self, cfg: DecoderConfig, device, rank: int = 0, world: int = 1, batch: int = 1, seed: int = 0, group=None):
         if PIECES % world or cfg.n_kv_heads % world or cfg.vocab % PIECES or cfg.ffn % PIECES:
@@ -118,6 +127,7 @@ class LlamaShapedDecoder:
         self.fuse_quantize = True       # decode steps: producers store Q8_1 containers directly
         self.fuse_rope = True           # decode steps: rotary embedding + cache update inside the attention launch
         self._att_scratch = None        # split-context attention: partial results and arrival counters
+        self.kv = None                  # PagedKvCache, after use_pages()
         self.tap = None                 # tests set a dict here: forward() then records copies of its intermediate tensors
         if world > 1:       # ranks build their shards at different speeds: line up before the first gather, whose polls are bounded
             import torch.distributed as dist
@@ -340,3 +350,96 @@ class LlamaShapedDecoder:
             outs.append(tok)
         self.check()
         return torch.stack(outs, dim=1)
+
+    # ---- several continuations of one prompt, over a cache in pages ---------------------------------------------
+    def use_pages(self, pages: int, page_size: int = 64, max_seqs: int = 64, dtype: torch.dtype = torch.float32) -> PagedKvCache:
+        """Gives the decoder a paged cache of its own, `self.kv` (f32, or a 16-bit type for half the memory and reads), which `branches` uses."""
+        self.kv = PagedKvCache(self.cfg.layers, pages, page_size, self.hkv_l, self.cfg.head_dim, max_seqs, self.cfg.max_pos, dtype=dtype, device=self.device)
+        return self.kv
+
+    def forward_pages(self, tokens: torch.Tensor, slots: torch.Tensor, plan) -> torch.Tensor:
+        """tokens: int64 [B, T], the next ones of the slots (int32 [B]) of `self.kv`, each at its own positions; plan: `kv.attention_plan(B, heads of this rank,
+        queries=T, ...)`.  Returns the logits of the last position, [B, vocab].  The attention's order of additions follows the plan, so the
+        logits are those of `forward` up to f32 rounding, not bit for bit, and so are those of another tensor-parallel width."""
+        cfg, kv, (B, T) = self.cfg, self.kv, tokens.shape
+        hd, q_cols = cfg.head_dim, self.hq_l * cfg.head_dim
+        with torch.cuda.device(self.device):
+            kv.reserve(slots, T)
+            plan.update(slots)
+            x, delta = self.tok_embd.index_select(0, tokens.reshape(-1)), None
+            for li, L in enumerate(self.layers):
+                h = self._norm(x, delta, L.attn_norm)
+                qk, v = L.wqk.forward(h).view(B, T, -1), L.wv.forward(h).view(B, T, self.hkv_l, hd)
+                q = kv.append(li, slots, qk[..., q_cols:].unflatten(-1, (self.hkv_l, hd)), v, q=qk[..., :q_cols].unflatten(-1, (self.hq_l, hd)),
+                              rotary=(self.cos, self.sin))
+                att = kv.attention(li, q, plan)
+                self._rec(f"{li}.q_rot", q), self._rec(f"{li}.att", att)
+                x, delta = self._rest_of_layer(L, x, att.view(B * T, q_cols).float())
+            return self._logits(x, delta, B, T)
+
+    def _rest_of_layer(self, L, x: torch.Tensor, att: torch.Tensor):
+        """A layer from its attention's output (f32) on: (x, the residual not yet added to it)."""
+        h = self._norm(x, L.wo.forward(self.gather(att)), L.ffn_norm)
+        gu = L.gate_up.forward(h)
+        a = torch.empty((x.shape[0], gu.shape[1] // 2), dtype=torch.float32, device=self.device)
+        capi.lib().cq_silu_mul_f32(gu.data_ptr(), a.data_ptr(), a.shape[0], a.shape[1], capi.stream_of(self.device))
+        return x, self.gather(L.down.forward(self.gather(a)))
+
+    def _logits(self, x: torch.Tensor, delta: torch.Tensor, B: int, T: int) -> torch.Tensor:
+        h = self._norm(x, delta, self.out_norm)
+        capi.check("decoder glue")
+        logits = self.gather(self.output.forward(h.view(B, T, -1)[:, -1, :].contiguous()))
+        self._rec("logits", logits)
+        return logits
+
+    def _prompt_pages(self, prompt: torch.Tensor) -> torch.Tensor:
+        """The prompt [1, T] into slot 0: the kernels of `forward` over one layer's worth of contiguous cache, whose keys and values go on to the pages.  Returns the
+        logits of its last position, the bits of `forward`."""
+        cfg, kv, T = self.cfg, self.kv, prompt.shape[1]
+        hd, q_cols, kv_cols, lib = cfg.head_dim, self.hq_l * cfg.head_dim, self.hkv_l * cfg.head_dim, capi.lib()
+        slot, block = torch.zeros(1, dtype=torch.int32, device=self.device), _Layer()
+        with torch.cuda.device(self.device):
+            block.k_cache = torch.zeros((1, self.hkv_l, cfg.max_pos, hd), device=self.device)
+            block.v_cache = torch.zeros_like(block.k_cache)
+            kv.reserve(slot, T)
+            x, delta = self.tok_embd.index_select(0, prompt.reshape(-1)), None
+            for li, L in enumerate(self.layers):
+                h = self._norm(x, delta, L.attn_norm)
+                qk, v = L.wqk.forward(h), L.wv.forward(h)
+                lib.cq_rope_store_kv_f32(qk.data_ptr(), qk.data_ptr() + 4 * q_cols, v.data_ptr(), self.cos.data_ptr(), self.sin.data_ptr(), self.pos.data_ptr(),
+                                         block.k_cache.data_ptr(), block.v_cache.data_ptr(), 1, T, self.hq_l, self.hkv_l, hd, cfg.max_pos, q_cols + kv_cols,
+                                         q_cols + kv_cols, kv_cols, capi.stream_of(self.device))
+                att = torch.empty((T, q_cols), dtype=torch.float32, device=self.device)
+                self._attention(qk, block, 1, T, att, False)
+                kv.append(li, slot, block.k_cache[:, :, :T].transpose(1, 2).contiguous(), v.view(1, T, self.hkv_l, hd))
+                x, delta = self._rest_of_layer(L, x, att)
+            return self._logits(x, delta, 1, T)
+
+    def branches(self, prompt: torch.Tensor, n: int, steps: int) -> Branches:
+        """The `n` (up to 32) most probable first tokens after prompt int64 [1, Tp], each continued greedily to `steps` tokens, with the log probabilities of all tokens and
+        the entropies of the distributions they come from - what a program needs to choose among continuations.  The prompt is read and stored once: the continuations
+        share its pages and one pass of the attention over them.  Needs `use_pages`; starts from an empty cache and leaves it empty."""
+        kv, cfg = self.kv, self.cfg
+        if kv is None:
+            raise ValueError("branches: no paged cache (use_pages)")
+        if prompt.dim() != 2 or prompt.shape[0] != 1 or prompt.shape[1] == 0 or not 1 <= n <= min(32, kv.max_seqs) or steps < 1:
+            raise ValueError(f"branches: prompt [1, tokens], 1 <= n <= {min(32, kv.max_seqs)}, at least one step")
+        if prompt.shape[1] + steps - 1 > cfg.max_pos:
+            raise ValueError(f"prompt of {prompt.shape[1]} tokens plus {steps} steps exceeds max_pos = {cfg.max_pos}")
+        kv.reset()
+        self.reset()
+        best = token_logprobs(self._prompt_pages(prompt), top=n)
+        tokens, logprobs, entropy = [best.top_ids[0]], [best.top_logprobs[0]], [best.entropy.expand(n)]
+        slots = torch.arange(n, dtype=torch.int32, device=self.device)
+        if n > 1:
+            kv.fork(torch.zeros(n - 1, dtype=torch.int32, device=self.device), slots[1:].contiguous())
+        plan = kv.attention_plan(n, self.hq_l)
+        for _ in range(steps - 1):
+            got = token_logprobs(self.forward_pages(tokens[-1].unsqueeze(1), slots, plan), top=1)
+            tokens.append(got.top_ids[:, 0])
+            logprobs.append(got.top_logprobs[:, 0])
+            entropy.append(got.entropy)
+        kv.free(slots)
+        kv.check()
+        self.check()
+        return Branches(torch.stack(tokens, 1), torch.stack(logprobs, 1), torch.stack(entropy, 1))
