@@ -323,15 +323,15 @@ struct AppendArgs {
 };
 
 // A thread takes four rotary pairs of one head: eight consecutive elements (interleaved), or four and the four half a head further.
-// grid.x covers the heads of q, k and v of a row, grid.y the rows; one read and one write of each element, which is the bound.
-template <typename In, typename T>
+// grid.x covers the heads of q, k and v of a row, grid.y the rows, R of them at a time: their elements are asked for before their places are looked up, which is a chain of
+// three reads.  One read and one write of each element are the bound.
+template <typename In, typename T, int R>
 __global__ void __launch_bounds__(128) kv_append_kernel(const cq_kv_cache cache, const AppendArgs a) {
     extern __shared__ unsigned seen[];
     const State s = state_of(cache);
     cq_pdl_launch_dependents();
     cq_pdl_wait();
-    const bool stopped = __syncthreads_or(s.header[0]) != 0;        // other CTAs may add a fault: one answer for this one
-    if (blockIdx.x == 0 && blockIdx.y == 0 && !stopped) {           // a slot named twice would have two writers for its positions
+    if (blockIdx.x == 0 && blockIdx.y == 0) {           // a slot named twice would have two writers for its positions
         for (int i = threadIdx.x; i < (s.max_seqs + 31) / 32; i += 128) seen[i] = 0;
         __syncthreads();
         for (int i = threadIdx.x; i < a.batch; i += 128) {
@@ -339,78 +339,99 @@ __global__ void __launch_bounds__(128) kv_append_kernel(const cq_kv_cache cache,
             if (slot >= 0 && slot < s.max_seqs && (atomicOr(&seen[slot >> 5], 1u << (slot & 31)) >> (slot & 31) & 1)) atomicCAS(s.header, kOk, kBadSlot);
         }
     }
-    const int d = cache.head_dim, per = d / 8, hkv = cache.kv_heads, hq = a.q ? a.hq : 0;
-    const int unit = blockIdx.x * 128 + threadIdx.x, head = unit / per, x = unit % per;
+    const int shift = 31 - __clz(s.page), d = cache.head_dim, log_per = d == 128 ? 4 : 3, hkv = cache.kv_heads, hq = a.q ? a.hq : 0;
+    const int unit = blockIdx.x * 128 + threadIdx.x, head = unit >> log_per, x = unit & ((1 << log_per) - 1);
     if (head >= hq + 2 * hkv) return;
-    const int first = a.neox ? 4 * x : 8 * x, second = a.neox ? first + d / 2 : first + 4;
-    for (int64_t row = blockIdx.y; row < (int64_t)a.batch * a.t; row += gridDim.y) {
-        const int b = (int)(row / a.t), slot = a.slots[b];
-        int pos = -1, page = -1, code = kBadSlot;
-        if (stopped) code = -1;
-        else if (slot >= 0 && slot < s.max_seqs) {
-            pos = s.lens[slot] - a.t + (int)(row % a.t);
-            code = kBadPosition;
-            if (pos >= 0 && pos < s.max_pages * s.page && (!a.cosv || pos < a.max_pos)) {
-                page = s.tables[(size_t)slot * s.max_pages + pos / s.page];
-                code = page >= 0 && page < s.pages ? kOk : kBadPage;
+    const bool is_q = head < hq, is_v = head >= hq + hkv;
+    const int first = a.neox ? 4 * x : 8 * x, second = a.neox ? first + d / 2 : first + 4, own = is_q ? head : is_v ? head - hq - hkv : head - hq;
+    const In *from = reinterpret_cast<const In *>(is_q ? a.q : is_v ? a.v : a.k) + (int64_t)own * d;
+    const int64_t stride = is_q ? a.q_stride : is_v ? a.v_stride : a.k_stride;
+    const int rows = a.batch * a.t, step = gridDim.y;
+    for (int row0 = blockIdx.y; row0 < rows; row0 += R * step) {
+        Vec<In, 4> lo[R], hi[R];
+        int pos[R], page[R], code[R];
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            const In *src = from + (int64_t)min(row0 + i * step, rows - 1) * stride;
+            lo[i] = *reinterpret_cast<const Vec<In, 4> *>(src + first);
+            hi[i] = *reinterpret_cast<const Vec<In, 4> *>(src + second);
+        }
+        const int fault = s.header[0];
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            const int row = min(row0 + i * step, rows - 1), b = a.t == 1 ? row : row / a.t, slot = a.slots[b];
+            pos[i] = page[i] = -1;
+            code[i] = kBadSlot;
+            if (fault) code[i] = -1;
+            else if (slot >= 0 && slot < s.max_seqs) {
+                pos[i] = s.lens[slot] - a.t + (row - b * a.t);
+                code[i] = kBadPosition;
+                if (pos[i] >= 0 && pos[i] < s.max_pages * s.page && (!a.cosv || pos[i] < a.max_pos)) {
+                    page[i] = s.tables[(size_t)slot * s.max_pages + (pos[i] >> shift)];
+                    code[i] = page[i] >= 0 && page[i] < s.pages ? kOk : kBadPage;
+                }
             }
         }
-        const bool is_q = head < hq, is_v = head >= hq + hkv;
-        if (code > kOk && x == 0) atomicCAS(s.header, kOk, code);
-        if (code != kOk && !is_q) continue;
-        const In *src = reinterpret_cast<const In *>(is_q ? a.q : is_v ? a.v : a.k) + row * (is_q ? a.q_stride : is_v ? a.v_stride : a.k_stride) +
-                        (int64_t)(is_q ? head : is_v ? head - hq - hkv : head - hq) * d;
-        const Vec<In, 4> lo = *reinterpret_cast<const Vec<In, 4> *>(src + first), hi = *reinterpret_cast<const Vec<In, 4> *>(src + second);
-        Vec<T, 4> out_lo, out_hi;
-        if (is_v || !a.cosv) {
+        float4 c[R], n[R];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) { out_lo.v[i] = from_f<T>(to_f(lo.v[i])); out_hi.v[i] = from_f<T>(to_f(hi.v[i])); }
-        } else {
-            float4 c = make_float4(0.f, 0.f, 0.f, 0.f), n = c;
-            if (code == kOk) {
-                c = *reinterpret_cast<const float4 *>(a.cosv + (int64_t)pos * (d / 2) + 4 * x);
-                n = *reinterpret_cast<const float4 *>(a.sinv + (int64_t)pos * (d / 2) + 4 * x);
-            }
-            const float cs[4] = {c.x, c.y, c.z, c.w}, sn[4] = {n.x, n.y, n.z, n.w};
-            float p0[4], p1[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                p0[i] = a.neox ? to_f(lo.v[i]) : i < 2 ? to_f(lo.v[2 * (i & 1)]) : to_f(hi.v[2 * (i & 1)]);
-                p1[i] = a.neox ? to_f(hi.v[i]) : i < 2 ? to_f(lo.v[2 * (i & 1) + 1]) : to_f(hi.v[2 * (i & 1) + 1]);
-            }
-            float r0[4], r1[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {               // the operations of cq_rope_store_kv_f32
-                r0[i] = __fmaf_rn(p0[i], cs[i], -__fmul_rn(p1[i], sn[i]));
-                r1[i] = __fmaf_rn(p0[i], sn[i], __fmul_rn(p1[i], cs[i]));
-            }
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                out_lo.v[i] = from_f<T>(a.neox ? r0[i] : i & 1 ? r1[i >> 1] : r0[i >> 1]);
-                out_hi.v[i] = from_f<T>(a.neox ? r1[i] : i & 1 ? r1[2 + (i >> 1)] : r0[2 + (i >> 1)]);
+        for (int i = 0; i < R; ++i) {
+            c[i] = n[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (code[i] == kOk && !is_v && a.cosv) {
+                c[i] = *reinterpret_cast<const float4 *>(a.cosv + (int64_t)pos[i] * (d / 2) + 4 * x);
+                n[i] = *reinterpret_cast<const float4 *>(a.sinv + (int64_t)pos[i] * (d / 2) + 4 * x);
             }
         }
-        T *dst;
-        if (is_q) {
-            if (code != kOk)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) out_lo.v[i] = out_hi.v[i] = from_f<T>(0.0f);
-            dst = reinterpret_cast<T *>(a.q_out) + (row * hq + head) * d;
-        } else {
-            const int h = is_v ? head - hq - hkv : head - hq;
-            dst = reinterpret_cast<T *>(is_v ? cache.v : cache.k) +
-                  ((((int64_t)a.layer * s.pages + page) * hkv + h) * s.page + pos % s.page) * d;
+        for (int i = 0; i < R; ++i) {
+            const int64_t row = row0 + (int64_t)i * step;
+            if (row >= rows) break;
+            if (code[i] > kOk && x == 0) atomicCAS(s.header, kOk, code[i]);
+            if (code[i] != kOk && !is_q) continue;
+            Vec<T, 4> out_lo, out_hi;
+            if (is_v || !a.cosv) {
+#pragma unroll
+                for (int y = 0; y < 4; ++y) { out_lo.v[y] = from_f<T>(to_f(lo[i].v[y])); out_hi.v[y] = from_f<T>(to_f(hi[i].v[y])); }
+            } else {
+                const float cs[4] = {c[i].x, c[i].y, c[i].z, c[i].w}, sn[4] = {n[i].x, n[i].y, n[i].z, n[i].w};
+                float p0[4], p1[4], r0[4], r1[4];
+#pragma unroll
+                for (int y = 0; y < 4; ++y) {
+                    p0[y] = a.neox ? to_f(lo[i].v[y]) : y < 2 ? to_f(lo[i].v[2 * (y & 1)]) : to_f(hi[i].v[2 * (y & 1)]);
+                    p1[y] = a.neox ? to_f(hi[i].v[y]) : y < 2 ? to_f(lo[i].v[2 * (y & 1) + 1]) : to_f(hi[i].v[2 * (y & 1) + 1]);
+                }
+#pragma unroll
+                for (int y = 0; y < 4; ++y) {               // the operations of cq_rope_store_kv_f32
+                    r0[y] = __fmaf_rn(p0[y], cs[y], -__fmul_rn(p1[y], sn[y]));
+                    r1[y] = __fmaf_rn(p0[y], sn[y], __fmul_rn(p1[y], cs[y]));
+                }
+#pragma unroll
+                for (int y = 0; y < 4; ++y) {
+                    out_lo.v[y] = from_f<T>(a.neox ? r0[y] : y & 1 ? r1[y >> 1] : r0[y >> 1]);
+                    out_hi.v[y] = from_f<T>(a.neox ? r1[y] : y & 1 ? r1[2 + (y >> 1)] : r0[2 + (y >> 1)]);
+                }
+            }
+            T *dst;
+            if (is_q) {
+                if (code[i] != kOk)
+#pragma unroll
+                    for (int y = 0; y < 4; ++y) out_lo.v[y] = out_hi.v[y] = from_f<T>(0.0f);
+                dst = reinterpret_cast<T *>(a.q_out) + (row * hq + head) * d;
+            } else
+                dst = reinterpret_cast<T *>(is_v ? cache.v : cache.k) +
+                      (((((int64_t)a.layer * s.pages + page[i]) * hkv + own) << shift) + (pos[i] & (s.page - 1))) * d;
+            *reinterpret_cast<Vec<T, 4> *>(dst + first) = out_lo;
+            *reinterpret_cast<Vec<T, 4> *>(dst + second) = out_hi;
         }
-        *reinterpret_cast<Vec<T, 4> *>(dst + first) = out_lo;
-        *reinterpret_cast<Vec<T, 4> *>(dst + second) = out_hi;
     }
 }
 
 template <typename In, typename T> void append_launch(const cq_kv_cache &c, const AppendArgs &a, cudaStream_t st) {
-    const int units = ((a.q ? a.hq : 0) + 2 * c.kv_heads) * (c.head_dim / 8);
-    const int64_t rows = (int64_t)a.batch * a.t;
-    cq_launch_k(kv_append_kernel<In, T>, dim3((units + 127) / 128, (unsigned)(rows < 65535 ? rows : 65535)), dim3(128), (size_t)(c.max_seqs + 31) / 32 * 4, st,
-                c, a);
+    const unsigned units = ((a.q ? a.hq : 0) + 2 * c.kv_heads) * (c.head_dim / 8), x = (units + 127) / 128, rows = (unsigned)a.batch * a.t;
+    const size_t smem = (size_t)(c.max_seqs + 31) / 32 * 4;
+    // four rows a thread where that still fills the device (16 such CTAs an SM); one where latency counts
+    if (x * rows >= 4u * 16 * cq_sm_count())
+        cq_launch_k(kv_append_kernel<In, T, 4>, dim3(x, (rows + 3) / 4 < 65535 ? (rows + 3) / 4 : 65535), dim3(128), smem, st, c, a);
+    else cq_launch_k(kv_append_kernel<In, T, 1>, dim3(x, rows < 65535 ? rows : 65535), dim3(128), smem, st, c, a);
 }
 
 bool slots_ok(const cq_kv_cache *c, const int *a, const int *b, int n, const char *who) {
@@ -488,6 +509,7 @@ extern "C" void cq_kv_append(const cq_kv_cache *cache, int layer, const int *slo
         cq_set_status(CQ_ERR_BAD_ARG, "kv_append: q_out may be q only with the same type and rows without gaps");
         return;
     }
+    if ((int64_t)batch * t > (1 << 30)) { cq_set_status(CQ_ERR_UNSUPPORTED, "kv_append: at most 2^30 rows in a call"); return; }
     if (batch == 0) return;
     const AppendArgs a{slots, q, k, v, q_out, cosv, sinv, q_stride, k_stride, v_stride, layer, batch, t, hq, max_pos, neox};
     cudaStream_t st = (cudaStream_t)stream;
