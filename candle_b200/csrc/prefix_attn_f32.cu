@@ -1,8 +1,11 @@
 // Segments of the shared-prefix attention (prefix_attn.cuh) of f32 caches: f32 products from three tf32 ones on the tensor cores.
 //
-// x = h + l with h the upper 11 bits of the significand, l = x - h exact and cut to 11 bits by the instruction: a b = h h' + h l' + l h' up to 3 * 2^-22
-// |a b|, where a chain of 128 fused f32 products is good for 128 * 2^-24 at worst.  mma.sync m16n8k8 does 474 products a clock and SM here (measured), so 158
-// of these, against 128 fused products of the f32 pipe that would want their operands from shared memory all the time.
+// x = h + l with h the nearest number of 11 significant bits, l = x - h exact, of either sign and no more than 2^-11 |x|, cut to 11 bits by the instruction:
+// a b = h h' + h l' + l h' up to 2^-24 (l l') and 2^-21 of either sign (the cuts) of |a b|.  (With h cut instead of rounded all errors have one sign: an output was
+// 2e-6 off where plain f32 is 6e-7.)  The instruction's own sums are cut as well, so chains are short: scores have an accumulator for every 32 dims and two for the low parts, and the outputs' products of a step
+// go to fresh ones that are added to the outputs by f32 additions.
+// mma.sync m16n8k8 does 474 products a clock and SM here (measured), so 158 of these, against 128 fused products of the f32 pipe that would want their
+// operands from shared memory all the time.
 //
 // A warp is a worker of both lines: eight rows, S^T = K Q^T (16 keys x 8 rows a step), O^T += V^T P^T (dims x 8 rows), the next step of keys and values on its way by
 // asynchronous copies.  Shared keys are read once for every eight rows, from L2 but for the first: at 16 KB for 16 keys x 8 rows the tensor cores ask
@@ -14,6 +17,9 @@ namespace {
 using namespace cq_attn;
 
 constexpr int kStep = 16, kStages = 2;
+// Weights are up to 2^8, the maximum being let be so far: times 2^-24, which the quotient of the sums loses again, 65536 of them add up to no more than 1, and values of any
+// size do not overflow where their mean does not.  Values lose bits for it below 2^-80.
+constexpr float kDown = 1.0f / (1 << 24);
 
 template <int D> struct Step { float k[kStep][D + 4], v[kStep][D + 8]; };
 
@@ -24,11 +30,14 @@ __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint3
     asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ bool special(uint32_t x) { return (x & 0x7f800000u) == 0x7f800000u; }
-__device__ __forceinline__ uint32_t high(uint32_t x) { return x & 0xffffe000u; }
-// Of an infinity or NaN nothing is left, and it meets the other side's high part only: a low part of 0 would make a NaN of an infinity.
-__device__ __forceinline__ uint32_t low(uint32_t x) { return special(x) ? 0u : __float_as_uint(__uint_as_float(x) - __uint_as_float(high(x))); }
-__device__ __forceinline__ uint32_t finite_high(uint32_t x) { return special(x) ? 0u : high(x); }
+__device__ __forceinline__ uint32_t high(uint32_t x) { return (x + 0x1000u) & 0xffffe000u; }
+__device__ __forceinline__ uint32_t low(uint32_t x, uint32_t h) { return __float_as_uint(__uint_as_float(x) - __uint_as_float(h)); }
+// The same for any number: what would round to infinity is cut.  Of an infinity nothing is left, and it meets the other side's high part only: a low part of 0 would make a
+// NaN of it.  A NaN's low part is a NaN, whatever the cut makes of the high one.
+__device__ __forceinline__ bool infinite(uint32_t x) { return (x & 0x7fffffffu) == 0x7f800000u; }
+__device__ __forceinline__ uint32_t safe_high(uint32_t x) { return (x & 0x7fffffffu) >= 0x7f7ff000u ? x & 0xffffe000u : high(x); }
+__device__ __forceinline__ uint32_t safe_low(uint32_t x) { return infinite(x) ? 0u : low(x, safe_high(x)); }
+__device__ __forceinline__ uint32_t finite_high(uint32_t x) { return infinite(x) ? 0u : safe_high(x); }
 
 // The copies of a warp's steps, ahead of their use and across its segments: the shared line, then the own one.  Sixteen rows of a page are one block of memory, copied 16 bytes
 // a lane; rows behind the last key come as zeros.
@@ -100,8 +109,8 @@ __global__ void __launch_bounds__(32 * f32_warps(D), 1) prefix_f32_kernel(const 
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 const uint32_t w = g < seg.rows ? __float_as_uint(src[8 * x + 4 * i]) : 0u;
-                qh[x][i] = high(w);
-                ql[x][i] = low(w);
+                qh[x][i] = safe_high(w);
+                ql[x][i] = safe_low(w);
             }
         float o[D / 16][4] = {}, m0 = 0.0f, m1 = 0.0f, l0 = 0.0f, l1 = 0.0f;       // rows 2 t and 2 t + 1
 #pragma unroll 1
@@ -111,19 +120,25 @@ __global__ void __launch_bounds__(32 * f32_warps(D), 1) prefix_f32_kernel(const 
             __syncwarp();
             const Step<D> &kv = steps[stage];
             const uint32_t ka = cq_smem_u32(&kv.k[(lane >> 3 & 1) * 8 + (lane & 7)][(lane >> 4) * 4]);
-            float s[2][4] = {};
+            constexpr int kChains = D / 32;
+            float s[kChains][4] = {}, sl[2][4] = {};
 #pragma unroll
             for (int x = 0; x < D / 8; ++x) {
                 uint32_t a[4], h[4], r[4];
                 ldsm(a, ka + 32 * x);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) { h[i] = high(a[i]); r[i] = __float_as_uint(__uint_as_float(a[i]) - __uint_as_float(h[i])); }
-                mma(s[x & 1], r, qh[x][0], qh[x][1]);
-                mma(s[x & 1], h, ql[x][0], ql[x][1]);
-                mma(s[x & 1], h, qh[x][0], qh[x][1]);
+                for (int i = 0; i < 4; ++i) { h[i] = high(a[i]); r[i] = low(a[i], h[i]); }
+                mma(sl[0], r, qh[x][0], qh[x][1]);
+                mma(sl[1], h, ql[x][0], ql[x][1]);
+                mma(s[x % kChains], h, qh[x][0], qh[x][1]);
             }
 #pragma unroll
-            for (int i = 0; i < 4; ++i) s[0][i] += s[1][i];
+            for (int i = 0; i < 4; ++i) {
+                const float small = sl[0][i] + sl[1][i];
+#pragma unroll
+                for (int x = 1; x < kChains; ++x) s[0][i] += s[x][i];
+                s[0][i] += small;
+            }
             // An infinite key has a NaN for its low part: the scores once more, with care.
             const float sum = s[0][0] + s[0][1] + s[0][2] + s[0][3];
             if (__any_sync(0xffffffffu, sum != sum)) {
@@ -134,7 +149,7 @@ __global__ void __launch_bounds__(32 * f32_warps(D), 1) prefix_f32_kernel(const 
                     uint32_t a[4], h[4], f[4], r[4];
                     ldsm(a, ka + 32 * x);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) { h[i] = high(a[i]); f[i] = finite_high(a[i]); r[i] = low(a[i]); }
+                    for (int i = 0; i < 4; ++i) { h[i] = safe_high(a[i]); f[i] = finite_high(a[i]); r[i] = safe_low(a[i]); }
                     mma(s[0], r, qh[x][0], qh[x][1]);
                     mma(s[0], f, ql[x][0], ql[x][1]);
                     mma(s[0], h, qh[x][0], qh[x][1]);
@@ -165,6 +180,8 @@ __global__ void __launch_bounds__(32 * f32_warps(D), 1) prefix_f32_kernel(const 
             }
             const float b0 = m0 == -INFINITY ? 0.0f : m0, b1 = m1 == -INFINITY ? 0.0f : m1;
             float p[4] = {exp2f(__fmaf_rn(s[0][0], c, -b0)), exp2f(__fmaf_rn(s[0][1], c, -b1)), exp2f(__fmaf_rn(s[0][2], c, -b0)), exp2f(__fmaf_rn(s[0][3], c, -b1))};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) p[i] *= kDown;
             l0 += p[0] + p[2];
             l1 += p[1] + p[3];
             // P^T changes sides: this lane's row is g now, its keys t, t + 4, t + 8, t + 12
@@ -175,12 +192,12 @@ __global__ void __launch_bounds__(32 * f32_warps(D), 1) prefix_f32_kernel(const 
                 const float even = __shfl_sync(0xffffffffu, i < 2 ? p[0] : p[2], from), odd = __shfl_sync(0xffffffffu, i < 2 ? p[1] : p[3], from);
                 const uint32_t w = __float_as_uint(g & 1 ? odd : even);
                 ph[i] = high(w);
-                pr[i] = low(w);
+                pr[i] = low(w, ph[i]);
             }
 #pragma unroll
             for (int x0 = 0; x0 < D / 16; x0 += 4) {            // 64 dims at a time
                 uint32_t w[4][2][4];
-                float care = 0.0f;                              // NaN if a value is not finite
+                float care = 0.0f;                              // the largest: infinities, and what would round to one, need care
 #pragma unroll
                 for (int x = 0; x < 4; ++x)
 #pragma unroll
@@ -188,33 +205,41 @@ __global__ void __launch_bounds__(32 * f32_warps(D), 1) prefix_f32_kernel(const 
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
                             const float e = kv.v[8 * y + t + 4 * (i >> 1)][16 * (x0 + x) + g + 8 * (i & 1)];
-                            care = __fmaf_rn(e, 0.0f, care);
+                            care = fmaxf(care, fabsf(e));
                             w[x][y][i] = __float_as_uint(e);
                         }
-                if (!__any_sync(0xffffffffu, care != care)) {
+                if (!__any_sync(0xffffffffu, care > 3e38f)) {
 #pragma unroll
-                    for (int x = 0; x < 4; ++x)
+                    for (int x = 0; x < 4; ++x) {
+                        float hh[4] = {}, hl[4] = {};
 #pragma unroll
                         for (int y = 0; y < 2; ++y) {
                             uint32_t h[4], r[4];
 #pragma unroll
-                            for (int i = 0; i < 4; ++i) { h[i] = high(w[x][y][i]); r[i] = __float_as_uint(__uint_as_float(w[x][y][i]) - __uint_as_float(h[i])); }
-                            mma(o[x0 + x], r, ph[2 * y], ph[2 * y + 1]);
-                            mma(o[x0 + x], h, pr[2 * y], pr[2 * y + 1]);
-                            mma(o[x0 + x], h, ph[2 * y], ph[2 * y + 1]);
+                            for (int i = 0; i < 4; ++i) { h[i] = high(w[x][y][i]); r[i] = low(w[x][y][i], h[i]); }
+                            mma(hl, r, ph[2 * y], ph[2 * y + 1]);
+                            mma(hl, h, pr[2 * y], pr[2 * y + 1]);
+                            mma(hh, h, ph[2 * y], ph[2 * y + 1]);
                         }
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) o[x0 + x][i] += hh[i] + hl[i];
+                    }
                 } else {
 #pragma unroll
-                    for (int x = 0; x < 4; ++x)
+                    for (int x = 0; x < 4; ++x) {
+                        float hh[4] = {}, hl[4] = {};
 #pragma unroll
                         for (int y = 0; y < 2; ++y) {
                             uint32_t h[4], f[4], r[4];
 #pragma unroll
-                            for (int i = 0; i < 4; ++i) { h[i] = high(w[x][y][i]); f[i] = finite_high(w[x][y][i]); r[i] = low(w[x][y][i]); }
-                            mma(o[x0 + x], r, ph[2 * y], ph[2 * y + 1]);
-                            mma(o[x0 + x], f, pr[2 * y], pr[2 * y + 1]);
-                            mma(o[x0 + x], h, ph[2 * y], ph[2 * y + 1]);
+                            for (int i = 0; i < 4; ++i) { h[i] = safe_high(w[x][y][i]); f[i] = finite_high(w[x][y][i]); r[i] = safe_low(w[x][y][i]); }
+                            mma(hl, r, ph[2 * y], ph[2 * y + 1]);
+                            mma(hl, f, pr[2 * y], pr[2 * y + 1]);
+                            mma(hh, h, ph[2 * y], ph[2 * y + 1]);
                         }
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) o[x0 + x][i] += hh[i] + hl[i];
+                    }
                 }
             }
             __syncwarp();

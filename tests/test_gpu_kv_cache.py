@@ -578,3 +578,32 @@ def test_infinite_values_and_plain_numbers(cuda_dev, dtype, dim):
     want = torch.full_like(got, 0.5)
     want[1, :, :, 5] = math.inf
     assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_the_largest_numbers_and_any_nan_in_f32(cuda_dev, dim):
+    """Numbers that would round to infinity when split, where their products are finite, and a NaN with nothing but its last bit set."""
+    cache, slots, g = _batch(torch.float32, 16, dim, 1, [40], [[3, 3]], seed=3)
+    rows = cache.tables[slots, :3].long()
+    big = torch.finfo(torch.float32).max
+    cache.k[0][rows] = 1.0
+    cache.k[0, :, :, :, 4] = 0.0
+    cache.v[0][rows] = 0.5
+    at = lambda s, n: (0, int(cache.tables[s, n // 16]), 0, n % 16)
+    cache.k[at(slots[0], 7) + (2,)] = -big           # a shared key, times 0 of the query
+    cache.k[at(slots[0], 41) + (2,)] = big           # an own one
+    cache.v[at(slots[0], 9) + (3,)] = big            # a shared value
+    cache.v[at(slots[0], 42) + (6,)] = -big
+    cache.v.view(torch.int32)[at(slots[1], 42) + (5,)] = 0x7F800001
+    q = torch.full((2, 1, 2, dim), 0.5, device="cuda")
+    q[..., 2] = 0.0
+    q[..., 4] = big
+    plan = cache.attention_plan(2, 2)
+    plan.update(slots)
+    got = cache.attention(0, q, plan)
+    want = torch.full_like(got, 0.5)
+    want[:, :, :, 3] = big / 43
+    want[0, :, :, 6] = -big / 43
+    want[1, :, :, 5] = math.nan
+    # 43 equal weights: the sums' and the quotient's roundings, and the other values' part of 43 * 0.5 / big.
+    torch.testing.assert_close(got, want, rtol=50 * 2.0 ** -24, atol=0, equal_nan=True)
