@@ -29,6 +29,9 @@ constexpr int kKeyTile = 128, kRing = 3, kCols = 512;                        // 
 constexpr int kHalfBytes = 128 * 128;                        // 128 rows of 64 elements
 constexpr int kGroup = 256, kO = 128;                        // columns of a half; in it the scores / weights and the outputs
 constexpr int kStep = 16;                                    // keys of a step of an own item
+// Weights of bf16 are 2^-24 of what was said, which the quotient of the sums loses again: 65536 of them add up to no more than 1, and values of any size do not overflow where
+// their mean does not.  f16's values cannot overflow an f32 sum, and its weights have no such range.
+template <bool BF16> constexpr float kDown = BF16 ? 24.0f : 0.0f;
 // registers a thread by warpgroup: 128 * (160 + 160 + 64 + 128) is what the block was launched with, 512 * 128
 constexpr int kRegsSoft = 160, kRegsMisc = 64, kRegsOwn = 128;
 static_assert(kCopyWarp == 8 && kMmaWarps == 4, "warp roles");
@@ -169,7 +172,7 @@ __device__ bool softmax_part(Tiles<D> &sm, const Call &call, const CUtensorMap &
                         }
                     }
                 }
-                const float base = m == -INFINITY ? 0.0f : m;
+                const float base = (m == -INFINITY ? 0.0f : m) + kDown<BF16>;
                 const uint64_t c2 = pack2f(c, c), base2 = pack2f(-base, -base);
                 uint64_t sum = 0;
 #pragma unroll
@@ -514,7 +517,7 @@ __device__ void own_part(uint32_t stages_at, uint32_t stride, int worker, const 
                 for (int x = 0; x < D / 16; ++x) { o[x][0] *= f0; o[x][1] *= f1; o[x][2] *= f0; o[x][3] *= f1; }
             }
         }
-        const float b0 = m0 == -INFINITY ? 0.0f : m0, b1 = m1 == -INFINITY ? 0.0f : m1;
+        const float b0 = (m0 == -INFINITY ? 0.0f : m0) + kDown<BF16>, b1 = (m1 == -INFINITY ? 0.0f : m1) + kDown<BF16>;
         const uint32_t p0 = transpose8(pack<BF16>(ex2(__fmaf_rn(s[0][0], c, -b0)), ex2(__fmaf_rn(s[0][1], c, -b1)), l0, l1));
         const uint32_t p1 = transpose8(pack<BF16>(ex2(__fmaf_rn(s[0][2], c, -b0)), ex2(__fmaf_rn(s[0][3], c, -b1)), l0, l1));
 #pragma unroll

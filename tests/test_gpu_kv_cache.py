@@ -607,3 +607,20 @@ def test_the_largest_numbers_and_any_nan_in_f32(cuda_dev, dim):
     want[1, :, :, 5] = math.nan
     # 43 equal weights: the sums' and the quotient's roundings, and the other values' part of 43 * 0.5 / big.
     torch.testing.assert_close(got, want, rtol=50 * 2.0 ** -24, atol=0, equal_nan=True)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("prompt", [40, 700])
+def test_the_largest_values_of_bf16(cuda_dev, dim, prompt):
+    """Sums of many values that are nearly the largest number: no weight passes 1 by a rounding, and no sum of them overflows where the mean does not."""
+    cache, slots, g = _batch(torch.bfloat16, 16, dim, 1, [prompt], [[3] * 9], seed=3)
+    rows = cache.tables[slots].long().clamp(min=0)
+    big = torch.finfo(torch.bfloat16).max
+    cache.k[0][rows] = 1.0
+    cache.v[0][rows] = big
+    q = torch.full((9, 1, 4, dim), 0.3, dtype=torch.bfloat16, device="cuda")
+    plan = cache.attention_plan(9, 4)
+    plan.update(slots)
+    got = cache.attention(0, q, plan).double()
+    # equal weights: what is left are the roundings of the sums (f32) and of the result (2^-8)
+    assert bool(((got - big).abs() <= (2.0 ** -8 + 1e-4) * big).all())
