@@ -369,6 +369,7 @@ __global__ void __launch_bounds__(128) kv_append_kernel(const cq_kv_cache cache,
                 if (pos[i] >= 0 && pos[i] < s.max_pages * s.page && (!a.cosv || pos[i] < a.max_pos)) {
                     page[i] = s.tables[(size_t)slot * s.max_pages + (pos[i] >> shift)];
                     code[i] = page[i] >= 0 && page[i] < s.pages ? kOk : kBadPage;
+                    if (code[i] == kOk && !is_q && s.refs[page[i]] > 1) code[i] = kBadPosition;         // others read it
                 }
             }
         }
@@ -436,7 +437,7 @@ template <typename In, typename T> void append_launch(const cq_kv_cache &c, cons
 
 bool slots_ok(const cq_kv_cache *c, const int *a, const int *b, int n, const char *who) {
     if (!cache_ok(c, who)) return false;
-    if (!a || !b || n < 0 || n > c->max_seqs) {
+    if ((n && (!a || !b)) || n < 0 || n > c->max_seqs) {
         char msg[160];
         std::snprintf(msg, sizeof msg, "%s: null list, or more slots than the cache has", who);
         cq_set_status(CQ_ERR_BAD_ARG, msg);
@@ -531,7 +532,7 @@ extern "C" int cq_kv_take_fault(const cq_kv_cache *cache, void *stream) {
     if (!cache_ok(cache, "kv_take_fault")) return -1;
     static const char *const text[] = {"", "a slot is out of range, named twice, or source and destination at once", "out of pages",
                                        "a sequence would be longer than its table", "fork into a slot that is not empty", "a table names a page that is not there",
-                                       "a position before the sequence, or past its table or the rotary tables", "a wait inside the attention gave up"};
+                                       "a position before the sequence, in a shared page, or past its table or the rotary tables", "a wait inside the attention gave up"};
     int fault = 0;
     const int zero = 0;
     cudaStream_t st = (cudaStream_t)stream;

@@ -13,9 +13,9 @@ of one pool, and a sequence that goes on from another one shares its full pages:
     cache.reserve(slots, 1); plan.update(slots)
     out = cache.attention(layer, q, plan)               # per layer
 
-Nothing here synchronises or looks at the device's numbers: a step can be captured into a CUDA graph (slots given as an int32 tensor).  What the device finds
-wrong - no page left, a slot named twice, ... - leaves the cache as it was, stops every later change, and is raised by `check()`.  Calls on one cache
-are ordered by the caller: one stream, or events between several.
+Nothing here but `check()` waits for the device or looks at its numbers: a step can be captured into a CUDA graph (slots given as an
+int32 tensor of the device).  What the device finds wrong - no page left, a slot named twice, ... - leaves the bookkeeping as it was, stops every later change, and is
+raised by `check()`.  Calls on one cache are ordered by the caller: one stream, or events between several.
 """
 from __future__ import annotations
 
@@ -81,7 +81,7 @@ class PagedKvCache:
         capi.check("PagedKvCache")
 
     def slot_list(self, slots) -> torch.Tensor:
-        """Slots as the device reads them: int32, contiguous, on the cache's device.  Such a tensor is taken as it is."""
+        """Slots as the device reads them: int32, contiguous, on the cache's device.  Such a tensor is taken as it is; numbers of the host are copied there."""
         if isinstance(slots, torch.Tensor):
             if slots.dtype == torch.int32 and slots.device == self.device and slots.dim() == 1 and slots.is_contiguous() and slots.shape[0] <= self.max_seqs:
                 return slots
@@ -89,6 +89,8 @@ class PagedKvCache:
             slots = [slots] if isinstance(slots, int) else list(slots)
             if any(not 0 <= int(s) < self.max_seqs for s in slots):
                 raise CandleQError(f"PagedKvCache: slots are 0 .. {self.max_seqs - 1}")
+            if len(slots) <= self.max_seqs:
+                return torch.tensor(slots, dtype=torch.int32).to(self.device, non_blocking=True)       # pageable memory: copied aside before this returns
             slots = torch.tensor(slots, dtype=torch.int32)
         if slots.dim() != 1 or slots.is_floating_point() or slots.dtype == torch.bool:
             raise CandleQError("PagedKvCache: slots must be a list of whole numbers")
@@ -156,7 +158,8 @@ class PagedKvCache:
         return t, stride
 
     def append(self, layer: int, slots, k: torch.Tensor, v: torch.Tensor, q: torch.Tensor | None = None, rotary=None, neox: bool = False):
-        """Keys and values [batch, tokens, kv_heads, head_dim] (f32, f16, bf16) of the last `tokens` positions of the slots, which `reserve` has added.  With
+        """Keys and values [batch, tokens, kv_heads, head_dim] (f32, f16, bf16) of the last `tokens` positions of the slots, which `reserve` has added (a position in a
+        page that other slots share is a fault).  With
         `rotary` = (cos, sin), each [positions, head_dim / 2] f32, k and q are rotated at their sequence's own positions: pairs (2i, 2i + 1), with `neox`
         (i, i + head_dim / 2).  Returns q [batch, tokens, heads, head_dim] in the cache's type, or None."""
         s = self.slot_list(slots)

@@ -624,3 +624,35 @@ def test_the_largest_values_of_bf16(cuda_dev, dim, prompt):
     got = cache.attention(0, q, plan).double()
     # equal weights: what is left are the roundings of the sums (f32) and of the result (2^-8)
     assert bool(((got - big).abs() <= (2.0 ** -8 + 1e-4) * big).all())
+
+
+def test_append_leaves_shared_pages_alone(cuda_dev):
+    """More tokens than the slot has reserved since its fork would reach into pages that the other one reads."""
+    cache = _make(8, 16, 1, 64, 4, 64, torch.float32)
+    row = lambda b, t: torch.ones((b, t, 1, 64), device="cuda")
+    cache.reserve([0], 20)
+    cache.append(0, [0], row(1, 20), row(1, 20))
+    cache.fork([0], [1])
+    cache.reserve([1], 2)
+    was = cache.k.clone()
+    cache.append(0, [1], 2 * row(1, 6), row(1, 6))          # positions 16 .. 21: pages of its own
+    cache.check()
+    assert float(cache.k[0, int(cache.tables[1, 1]), 0, :6].min()) == 2.0 and torch.equal(cache.k[:, cache.tables[0, :2].long()], was[:, cache.tables[0, :2].long()])
+    cache.append(0, [1], 3 * row(1, 7), row(1, 7))
+    assert torch.equal(cache.k[:, cache.tables[0, :2].long()], was[:, cache.tables[0, :2].long()])
+    _faulted(cache, "shared page")
+    cache.free([0])
+    cache.append(0, [1], 3 * row(1, 7), row(1, 7))          # now it is alone
+    cache.check()
+    assert float(cache.k[0, int(cache.tables[1, 0]), 0, 15, 0]) == 3.0
+
+
+def test_empty_lists_change_nothing(cuda_dev):
+    cache = _make(8, 16, 1, 64, 4, 64, torch.float32)
+    cache.reserve([0], 20)
+    was = cache.state.clone()
+    cache.reserve([], 3), cache.free([]), cache.fork([], []), cache.copy([], []), cache.reserve([0], 0)
+    cache.check()
+    assert torch.equal(cache.state, was)
+    with pytest.raises(capi.CandleQError, match="5 slots"):
+        cache.reserve([0, 1, 2, 3, 0], 1)
