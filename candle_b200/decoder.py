@@ -362,6 +362,8 @@ class LlamaShapedDecoder:
         queries=T, ...)`.  Returns the logits of the last position, [B, vocab].  The attention's order of additions follows the plan, so the
         logits are those of `forward` up to f32 rounding, not bit for bit, and so are those of another tensor-parallel width."""
         cfg, kv, (B, T) = self.cfg, self.kv, tokens.shape
+        if kv is None or (plan.cache, plan.batch, plan.heads, plan.queries) != (kv, B, self.hq_l, T):
+            raise ValueError(f"forward_pages: the plan must be one of this decoder's paged cache for {B} x {T} tokens and {self.hq_l} heads")
         hd, q_cols = cfg.head_dim, self.hq_l * cfg.head_dim
         with torch.cuda.device(self.device):
             kv.reserve(slots, T)
@@ -418,7 +420,8 @@ class LlamaShapedDecoder:
     def branches(self, prompt: torch.Tensor, n: int, steps: int) -> Branches:
         """The `n` (up to 32) most probable first tokens after prompt int64 [1, Tp], each continued greedily to `steps` tokens, with the log probabilities of all tokens and
         the entropies of the distributions they come from - what a program needs to choose among continuations.  The prompt is read and stored once: the continuations
-        share its pages and one pass of the attention over them.  Needs `use_pages`; starts from an empty cache and leaves it empty."""
+        share its pages and one pass of the attention over them.  Logits that are not a distribution (a NaN among them) give the token -1 and NaN.  Needs `use_pages`;
+        starts from an empty cache and leaves it empty."""
         kv, cfg = self.kv, self.cfg
         if kv is None:
             raise ValueError("branches: no paged cache (use_pages)")
@@ -435,7 +438,8 @@ class LlamaShapedDecoder:
             kv.fork(torch.zeros(n - 1, dtype=torch.int32, device=self.device), slots[1:].contiguous())
         plan = kv.attention_plan(n, self.hq_l)
         for _ in range(steps - 1):
-            got = token_logprobs(self.forward_pages(tokens[-1].unsqueeze(1), slots, plan), top=1)
+            # logits that are no distribution have the token -1: it goes on as -1, but is not looked up
+            got = token_logprobs(self.forward_pages(tokens[-1].clamp(min=0).unsqueeze(1), slots, plan), top=1)
             tokens.append(got.top_ids[:, 0])
             logprobs.append(got.top_logprobs[:, 0])
             entropy.append(got.entropy)

@@ -97,3 +97,30 @@ def test_refusals(cuda_dev):
             m.branches(*args)
     with pytest.raises(Exception, match="out of pages"):
         m.branches(_prompt(m, 40), 3, 2)        # three pages, and one more for each of two forks
+
+
+def test_logits_that_are_no_distribution(cuda_dev, monkeypatch):
+    """A NaN among the logits (the quantized products make none of their own: their activations' blocks drop it): tokens of -1 that are not looked up, NaN for
+    their numbers, the cache empty as ever."""
+    m = _model(torch.float32)
+    real = m._logits
+
+    def with_nan(*args):
+        logits = real(*args)
+        logits[:, 7] = float("nan")
+        return logits
+
+    monkeypatch.setattr(m, "_logits", with_nan)
+    got = m.branches(_prompt(m, 20), 3, 4)
+    assert bool((got.tokens == -1).all()) and bool(got.logprobs.isnan().all()) and bool(got.entropy.isnan().all())
+    assert int(m.kv.lens.sum()) == 0 and int(m.kv.refs.sum()) == 0
+
+
+def test_a_plan_of_another_shape_is_refused(cuda_dev):
+    m = _model(torch.float32)
+    slots = torch.arange(2, dtype=torch.int32, device="cuda")
+    tokens = torch.zeros((2, 1), dtype=torch.int64, device="cuda")
+    for plan in (m.kv.attention_plan(3, m.hq_l), m.kv.attention_plan(2, m.hq_l, queries=2), m.kv.attention_plan(2, 2 * m.hq_l)):
+        with pytest.raises(ValueError):
+            m.forward_pages(tokens, slots, plan)
+    assert int(m.kv.lens.sum()) == 0
