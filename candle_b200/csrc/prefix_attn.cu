@@ -214,14 +214,16 @@ __global__ void __launch_bounds__(kThreads) prefix_plan_kernel(const cq_kv_cache
     if (rank == 0 && tid == 0) { pl.header[0] = shared_line; pl.header[1] = chunk; pl.header[2] = own_line; pl.header[3] = own_chunk; pl.header[4] = own_chunk2; }
 }
 
-// One warp per row: lane x weighs segment x - those of the row's shared item, then those of its own one, in the order of their keys - and the
+// W warps per row, each with a share of its segments: lane x weighs segment x of 32 - those of the row's shared item, then those of its own one, in the order of their keys - and the
 // outputs are added in that order.
-template <typename T, int D> __global__ void __launch_bounds__(256) prefix_join_kernel(const Call call, T *out) {
+template <typename T, int D, int W> __global__ void __launch_bounds__(256) prefix_join_kernel(const Call call, T *out) {
+    __shared__ __align__(16) float all_acc[W > 1 ? W : 1][W > 1 ? D : 4];
+    __shared__ float2 all_ml[W];
     const Shape &sh = call.sh;
     const Plan &pl = call.plan;
     cq_pdl_launch_dependents();
     cq_pdl_wait();
-    const int lane = threadIdx.x & 31, per = sh.per_kv, n = blockIdx.y, hq = blockIdx.x * 8 + (threadIdx.x >> 5);
+    const int lane = threadIdx.x & 31, per = sh.per_kv, n = blockIdx.y, warp = threadIdx.x >> 5, hq = W > 1 ? blockIdx.x : blockIdx.x * 8 + warp;
     if (hq >= sh.heads) return;
     const int h = div_per(hq, sh), in = hq - h * per, tile = in / sh.own_rows;
     const int64_t row = (int64_t)n * sh.heads + hq;
@@ -229,6 +231,7 @@ template <typename T, int D> __global__ void __launch_bounds__(256) prefix_join_
     const int chunk = pl.header[1], own_chunk = pl.header[3], own_chunk2 = pl.header[4];
     constexpr int V = D / 32;
     float acc[V] = {}, m = -INFINITY, l = 0.0f;
+    bool some = false;
     if (q.len > 0) {
         // segments of an item: its units [start, start + units) of the line, cut at multiples of the chunk
         const int local = h * sh.own_tiles + tile, own_item = n * sh.kv_heads * sh.own_tiles + local;
@@ -243,8 +246,11 @@ template <typename T, int D> __global__ void __launch_bounds__(256) prefix_join_
         }
         const int n_all = n_shared + n_own;
         const int64_t own0 = part_own(sh, call.shared_items, own_item + own_w) + in - tile * sh.own_rows;
-        for (int x0 = 0; x0 < n_all; x0 += 32) {
-            const int x = x0 + lane, count = min(32, n_all - x0);
+        const int share = (n_all + W - 1) / W, begin = W > 1 ? warp * share : 0, end = W > 1 ? min(n_all, begin + share) : n_all;
+        some = begin < end;
+        for (int x0 = begin; x0 < end; x0 += 32) {
+            const bool more = x0 > begin;
+            const int x = x0 + lane, count = min(32, end - x0);
             const int part = (int)(x < n_shared ? shared0 + (int64_t)x * sh.row_tile : own0 + (int64_t)(x - n_shared) * sh.own_slot());
             const float2 ml = lane < count ? call.ml[part] : make_float2(-INFINITY, 0.0f);
             // four outputs at a time on their way, the first of them beside the maxima
@@ -264,14 +270,14 @@ template <typename T, int D> __global__ void __launch_bounds__(256) prefix_join_
 #pragma unroll
             for (int k = 16; k > 0; k >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, k));
             // all scores so far -inf: no weight can be given, as in the formula (lanes without a segment have none)
-            const float w = lane < count ? exp2f(ml.x - big) : 0.0f, f = x0 ? exp2f(m - big) : 0.0f;
+            const float w = lane < count ? exp2f(ml.x - big) : 0.0f, f = more ? exp2f(m - big) : 0.0f;
             float sum = lane < count ? __fmul_rn(ml.y, w) : 0.0f;
 #pragma unroll
             for (int k = 16; k > 0; k >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, k);
-            l = x0 ? __fmaf_rn(l, f, sum) : sum;
+            l = more ? __fmaf_rn(l, f, sum) : sum;
             m = big;
 #pragma unroll
-            for (int i = 0; i < V; ++i) acc[i] = x0 ? __fmul_rn(acc[i], f) : 0.0f;
+            for (int i = 0; i < V; ++i) acc[i] = more ? __fmul_rn(acc[i], f) : 0.0f;
             for (int y0 = 0; y0 < count; y0 += 4) {
                 if (y0) fetch(y0);
 #pragma unroll
@@ -284,6 +290,27 @@ template <typename T, int D> __global__ void __launch_bounds__(256) prefix_join_
             }
         }
     }
+    if constexpr (W > 1) {                  // the warps' shares, in their order
+        if (lane == 0) all_ml[warp] = make_float2(some ? m : NAN, l);
+#pragma unroll
+        for (int i = 0; i < V; ++i) all_acc[warp][V * lane + i] = acc[i];
+        __syncthreads();
+        if (warp) return;
+        m = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < W; ++w) m = fmaxf(m, all_ml[w].x);
+        l = 0.0f;
+#pragma unroll
+        for (int i = 0; i < V; ++i) acc[i] = 0.0f;
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+            const float2 ml = all_ml[w];
+            const float f = ml.x == ml.x ? exp2f(ml.x - m) : 0.0f;          // NaN: a share without segments
+            l = __fmaf_rn(f, ml.y, l);
+#pragma unroll
+            for (int i = 0; i < V; ++i) acc[i] = __fmaf_rn(f, all_acc[w][V * lane + i], acc[i]);
+        }
+    }
     T *to = out + row * D + V * lane;
 #pragma unroll
     for (int i = 0; i < V; ++i) {
@@ -294,11 +321,20 @@ template <typename T, int D> __global__ void __launch_bounds__(256) prefix_join_
     }
 }
 
+template <int D, int W> void join_launch(const Call &c, void *out, cudaStream_t st) {
+    const dim3 grid((unsigned)(W > 1 ? c.sh.heads : (c.sh.heads + 7) / 8), (unsigned)c.sh.n_queries()), threads(W > 1 ? 32 * W : 256);
+    if (c.sh.elem == CQ_F32) cq_launch_k(prefix_join_kernel<float, D, W>, grid, threads, 0, st, c, (float *)out);
+    else if (c.sh.elem == CQ_F16) cq_launch_k(prefix_join_kernel<__half, D, W>, grid, threads, 0, st, c, (__half *)out);
+    else cq_launch_k(prefix_join_kernel<__nv_bfloat16, D, W>, grid, threads, 0, st, c, (__nv_bfloat16 *)out);
+}
+// Few rows have many segments, a hundred and more where one sequence's keys are divided over the whole device: several warps a row where all of them are on the
+// device at once, 64 an SM.  With plan and attention, in us: 32 rows of 4,000 keys 42 with one warp a row, 18 with eight; 2,048 rows of 8,700 keys 56.6, with two 53.9; but 3,200
+// rows of 300 keys 20.7, with two 22.4, which is where two stop.
 template <int D> void join_launch(const Call &c, void *out, cudaStream_t st) {
-    const dim3 grid((unsigned)((c.sh.heads + 7) / 8), (unsigned)c.sh.n_queries());
-    if (c.sh.elem == CQ_F32) cq_launch_k(prefix_join_kernel<float, D>, grid, dim3(256), 0, st, c, (float *)out);
-    else if (c.sh.elem == CQ_F16) cq_launch_k(prefix_join_kernel<__half, D>, grid, dim3(256), 0, st, c, (__half *)out);
-    else cq_launch_k(prefix_join_kernel<__nv_bfloat16, D>, grid, dim3(256), 0, st, c, (__nv_bfloat16 *)out);
+    const int rows = c.sh.n_queries() * c.sh.heads, warps = 64 * cq_sm_count();
+    if (rows * 8 <= warps) join_launch<D, 8>(c, out, st);
+    else if (rows * 3 <= warps) join_launch<D, 2>(c, out, st);
+    else join_launch<D, 1>(c, out, st);
 }
 
 bool shape_ok(const cq_kv_cache *cache, const cq_prefix_plan *p, const char *who, Shape &s) {
@@ -325,7 +361,7 @@ bool shape_ok(const cq_kv_cache *cache, const cq_prefix_plan *p, const char *who
     s.ctas = p->ctas;
     s.own_rows = 8;
     s.own_shift = 4;
-    if (cache->elem == CQ_F32) { s.row_tile = 8; s.tile = 64; s.own_workers = s.own_first = s.ctas; }
+    if (cache->elem == CQ_F32) { s.row_tile = 8; s.tile = 16; s.own_workers = s.own_first = s.ctas; }
     else { s.row_tile = 256; s.tile = 128; s.own_first = s.ctas * kMmaWarps; s.own_workers = s.own_first + s.ctas * kMmaHelpers; }
     s.own_tiles = (s.per_kv + s.own_rows - 1) / s.own_rows;
     if (s.per_kv > 1) s.rcp = (unsigned)(((1ull << 32) + s.per_kv - 1) / s.per_kv);

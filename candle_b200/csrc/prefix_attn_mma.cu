@@ -589,9 +589,9 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_mma_kernel(const cq_kv_cac
         if (warp == kCopyWarp) ok = copy_part<D>(sm, cache, st, call, k_map, v_map);
         else if (warp == kMmaWarp) ok = mma_part<D, BF16>(sm, call);
     } else {
-        regs_up<kRegsOwn>();
-        own_part<D, BF16, Tiles<D>::kStages>(cq_smem_u32(sm.step[warp - kOwnWarp]), (uint32_t)sizeof(Step<D>), blockIdx.x * kMmaWarps + warp - kOwnWarp, cache, st, call, k_layer,
-                                             v_layer, q, q_stride, c);
+        regs_up<kRegsOwn>();            // workers from the last CTA on: where there is less than one item or tile for each, the first ones have the shared tiles
+        own_part<D, BF16, Tiles<D>::kStages>(cq_smem_u32(sm.step[warp - kOwnWarp]), (uint32_t)sizeof(Step<D>), (gridDim.x - 1 - blockIdx.x) * kMmaWarps + warp - kOwnWarp, cache, st, call,
+                                             k_layer, v_layer, q, q_stride, c);
     }
     if (!ok && lane == 0) atomicCAS(st.header, cq_kv::kOk, cq_kv::kTimeout);
     tc_fence_before();
