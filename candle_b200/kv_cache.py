@@ -146,7 +146,7 @@ class PagedKvCache:
         """`t` as [batch, tokens, heads, head_dim] with heads side by side and aligned rows at one distance; (tensor, row distance)."""
         shape, d = t.shape, self.head_dim
         if len(shape) != 4 or shape[0] != batch or shape[3] != d or (heads is not None and shape[2] != heads) or (tokens is not None and shape[1] != tokens) or \
-                t.device != self.device:
+                t.get_device() != self._index:
             raise CandleQError(f"PagedKvCache: {name} must be [batch, tokens, heads, {d}] on {self.device}, got {list(shape)}")
         width = shape[2] * d
         if t.is_contiguous():
@@ -165,28 +165,33 @@ class PagedKvCache:
         s = self.slot_list(slots)
         if not 0 <= layer < self.layers:
             raise CandleQError(f"PagedKvCache.append: layer {layer} of {self.layers}")
-        if k.dtype not in _ELEM or v.dtype != k.dtype or (q is not None and q.dtype != k.dtype):
+        elem = _ELEM.get(k.dtype)
+        if elem is None or v.dtype != k.dtype or (q is not None and q.dtype != k.dtype):
             raise CandleQError("PagedKvCache.append: q, k and v must be of one type, f32, f16 or bf16")
         b = s.shape[0]
         if b == 0 or k.dim() != 4 or k.shape[1] == 0:
             raise CandleQError("PagedKvCache.append: no slots or no tokens")
-        k, ks = self._rows(k, "k", b, self.kv_heads, None)
-        v, vs = self._rows(v, "v", b, self.kv_heads, k.shape[1])
-        qs, out, heads = 0, None, 0
+        tokens = k.shape[1]
+        k, ks = self._rows(k, "k", b, self.kv_heads, tokens)
+        v, vs = self._rows(v, "v", b, self.kv_heads, tokens)
+        qs, out, heads, q_at, out_at = 0, None, 0, None, None
         if q is not None:
-            q, qs = self._rows(q, "q", b, None, k.shape[1])
+            q, qs = self._rows(q, "q", b, None, tokens)
             heads = q.shape[2]
-            out = torch.empty(q.shape, dtype=self.dtype, device=self.device)
-        cos = sin = None
+            out = torch.empty_like(q, dtype=self.dtype, memory_format=torch.contiguous_format)
+            q_at, out_at = q.data_ptr(), out.data_ptr()
+        cos_at = sin_at = None
+        positions = 0
         if rotary is not None:
             cos, sin = rotary
-            for t in (cos, sin):
-                if t.dtype != torch.float32 or t.dim() != 2 or t.shape[1] != self.head_dim // 2 or t.shape[0] != cos.shape[0] or t.shape[0] == 0 or \
-                        not t.is_contiguous() or t.device != self.device or t.data_ptr() % 16:
-                    raise CandleQError(f"PagedKvCache.append: rotary tables must be contiguous, aligned f32 [positions, {self.head_dim // 2}] on {self.device}")
-        self._call(capi.lib().cq_kv_append, layer, s.data_ptr(), b, k.shape[1], None if q is None else q.data_ptr(), k.data_ptr(), v.data_ptr(), _ELEM[k.dtype], heads, qs,
-                   ks, vs, None if cos is None else cos.data_ptr(), None if sin is None else sin.data_ptr(), 0 if cos is None else cos.shape[0], int(neox),
-                   None if out is None else out.data_ptr())
+            positions = cos.shape[0]
+            cos_at, sin_at = cos.data_ptr(), sin.data_ptr()
+            want = (positions, self.head_dim // 2)
+            if positions == 0 or cos.shape != want or sin.shape != want or cos.dtype != torch.float32 or sin.dtype != torch.float32 or not cos.is_contiguous() or \
+                    not sin.is_contiguous() or cos.get_device() != self._index or sin.get_device() != self._index or (cos_at | sin_at) % 16:
+                raise CandleQError(f"PagedKvCache.append: rotary tables must be contiguous, aligned f32 [positions, {self.head_dim // 2}] on {self.device}")
+        self._call(capi.lib().cq_kv_append, layer, s.data_ptr(), b, tokens, q_at, k.data_ptr(), v.data_ptr(), elem, heads, qs, ks, vs, cos_at, sin_at, positions, int(neox),
+                   out_at)
         return out
 
     # ---- attention ----
@@ -207,7 +212,7 @@ class PagedKvCache:
         if q.dtype != self.dtype:
             raise CandleQError(f"PagedKvCache.attention: q must be of the cache's type, {self.dtype}")
         q, stride = self._rows(q, "q", plan.batch, plan.heads, plan.queries)
-        out = torch.empty((plan.batch, plan.queries, plan.heads, self.head_dim), dtype=self.dtype, device=self.device)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
         self._call(capi.lib().cq_prefix_attention, layer, plan._p, q.data_ptr(), stride, out.data_ptr(), 1.0 / math.sqrt(self.head_dim) if scale is None else scale)
         return out
 
