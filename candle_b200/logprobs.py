@@ -31,24 +31,28 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor | None = None, top
         raise CandleQError("token_logprobs needs CUDA logits [..., vocab]: there is no CPU path")
     if logits.dtype not in _ELEM:
         raise CandleQError(f"Expected f32/f16/bf16, got {logits.dtype}")
-    lead, vocab, dev = logits.shape[:-1], logits.shape[-1], logits.device
+    shape, dev = logits.shape, logits.device
+    vocab, flat = shape[-1], len(shape) == 2
     if vocab == 0 or not 0 <= top <= min(32, vocab):
         raise CandleQError(f"token_logprobs: 0 <= top <= min(32, vocab), got {top} of {vocab}")
-    flat = len(lead) == 1
     x = logits if flat else logits.reshape(-1, vocab)
     rows, step = x.shape[0], x.stride(0)
     if (x.stride(1) != 1 and vocab > 1) or (rows > 1 and step < 0):
         x, step = x.contiguous(), vocab
+    lead = shape[:-1]
+    tokens_at = logprob = logprob_at = None
+    entropy = torch.empty(rows, dtype=torch.float32, device=dev)
     if tokens is not None:
-        if tokens.shape != lead or tokens.is_floating_point() or tokens.dtype == torch.bool or tokens.device != dev:
+        if tokens.shape != lead or tokens.is_floating_point() or tokens.dtype == torch.bool or tokens.get_device() != logits.get_device():
             raise CandleQError(f"token_logprobs: tokens must be whole numbers of shape {list(lead)} on {dev}")
         if not flat:
             tokens = tokens.reshape(-1)
         if tokens.dtype != torch.int64 or not tokens.is_contiguous():
             tokens = tokens.to(torch.int64).contiguous()
-    logprob = None if tokens is None else torch.empty(rows, dtype=torch.float32, device=dev)
-    entropy, best = torch.empty(rows, dtype=torch.float32, device=dev), torch.empty((rows, top), dtype=torch.float32, device=dev)
-    ids = torch.empty((rows, top), dtype=torch.int64, device=dev)
+        logprob = torch.empty_like(entropy)
+        tokens_at, logprob_at = tokens.data_ptr(), logprob.data_ptr()
+    best = torch.empty((rows, top), dtype=torch.float32, device=dev)
+    ids = torch.empty_like(best, dtype=torch.int64)
     if rows:
         lib = capi.lib()
         with capi.on_device(dev):
@@ -56,9 +60,8 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor | None = None, top
             if nbytes == 0:
                 raise CandleQError(f"token_logprobs: {rows} rows of {vocab} are too many for one call")
             scratch = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-            lib.cq_token_logprobs(x.data_ptr(), _ELEM[x.dtype], step if rows > 1 else vocab, rows, vocab, None if tokens is None else tokens.data_ptr(), top,
-                                  None if logprob is None else logprob.data_ptr(), entropy.data_ptr(), best.data_ptr(), ids.data_ptr(), scratch.data_ptr(),
-                                  capi.stream_of(dev))
+            lib.cq_token_logprobs(x.data_ptr(), _ELEM[x.dtype], step if rows > 1 else vocab, rows, vocab, tokens_at, top, logprob_at, entropy.data_ptr(), best.data_ptr(),
+                                  ids.data_ptr(), scratch.data_ptr(), capi.stream_of(dev))
         capi.check("token_logprobs")
     if flat:
         return TokenLogProbs(logprob, entropy, best, ids)
