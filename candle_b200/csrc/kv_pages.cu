@@ -3,6 +3,8 @@
 // The bookkeeping (reference counts, lengths, tables) lives on the device, so that a decode step that grows its sequences, or forks
 // one, is a sequence of launches that a graph can hold.  One CTA does it: a pool has some thousands of pages, and a page's number
 // depends on all that are taken before it.  What it decides, a second kernel copies with the whole device.
+// On a B200, each kernel by itself with cold caches: 63 forks of 16 pages 13 us, bound by some ten reads that depend on one another; the list of a compaction of 320
+// pages 5 us.
 #include <cstdio>
 
 #include "kv_cache.cuh"
@@ -256,7 +258,8 @@ __global__ void __launch_bounds__(kMeta) kv_compact_kernel(const cq_kv_cache cac
 }
 
 // The listed copies over all layers, keys and values.  A warp moves pieces of kPiece bytes, eight 16-byte loads of a lane in flight
-// before the first store.  REMAP: the table entries of moved pages follow (compaction).
+// before the first store.  REMAP: the table entries of moved pages follow (compaction).  Bound by HBM: 64 pages of 32 layers, 1074 MB read and written, in 173 us, 6.2 TB/s
+// (a plain copy of the device: 6.5); 63 part-full pages, 336 MB, in 57 us, 5.9 TB/s.
 constexpr int kPiece = 4096, kCopyThreads = 256;
 template <bool REMAP>
 __global__ void __launch_bounds__(kCopyThreads) kv_copy_kernel(const cq_kv_cache cache) {
@@ -324,7 +327,8 @@ struct AppendArgs {
 
 // A thread takes four rotary pairs of one head: eight consecutive elements (interleaved), or four and the four half a head further.
 // grid.x covers the heads of q, k and v of a row, grid.y the rows, R of them at a time: their elements are asked for before their places are looked up, which is a chain of
-// three reads.  One read and one write of each element are the bound.
+// three reads (a fourth finds whether others read the page).  One read and one write of each element are the bound: 2047 rows of 48 heads of 128, f32, 102 MB in 22.4 us, 4.5 TB/s;
+// 64 rows take 2.6 us, a launch and the chain (both in a graph).
 template <typename In, typename T, int R>
 __global__ void __launch_bounds__(128) kv_append_kernel(const cq_kv_cache cache, const AppendArgs a) {
     extern __shared__ unsigned seen[];

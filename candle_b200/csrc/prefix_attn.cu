@@ -65,7 +65,7 @@ __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.w
 // entries that agree in all its sequences, as far as the shortest context among its queries fills pages.
 // Bound by latency: slots, lengths and tables are three reads that depend on one another, and a warp by itself takes some five clocks an instruction.
 // So the comparison and the records are divided over the CTAs, everything else each does for itself, and divisions are kept out of the way (one CTA of 1024 threads
-// took 16 - 33 us for 64 - 128 sequences).
+// took 16 - 33 us for 64 - 128 sequences).  In a graph: 5.4 us for 8 sequences of 8 pages, 6.6 for 64 of 143, 7.9 for 128 of 264.
 __global__ void __launch_bounds__(kThreads) prefix_plan_kernel(const cq_kv_cache cache, const Call call, const int *slots) {
     extern __shared__ int dyn[];
     __shared__ uint64_t sums[kThreads / 32];

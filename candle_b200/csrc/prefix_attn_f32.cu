@@ -10,6 +10,7 @@
 // A warp is a worker of both lines: eight rows, S^T = K Q^T (16 keys x 8 rows a step), O^T += V^T P^T (dims x 8 rows), the next step of keys and values on its way by
 // asynchronous copies.  Shared keys are read once for every eight rows, from L2 but for the first: at 16 KB for 16 keys x 8 rows the tensor cores ask
 // for 60 bytes a clock of an SM when nothing else is in the way, about what L2 gives.
+// By itself, cold caches: 32 sequences over 4 x 1500 shared keys, 32 heads of 64: 25 us, 0.45 GFLOP; 8 over 512, 32 heads of 128: 9.6 us, all of it latency.
 // Rows of K lie 4 floats more than their length apart and those of V 8 more, so that the fragments' reads meet every bank once.
 #include "prefix_attn.cuh"
 
