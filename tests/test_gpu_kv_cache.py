@@ -656,3 +656,54 @@ def test_empty_lists_change_nothing(cuda_dev):
     assert torch.equal(cache.state, was)
     with pytest.raises(capi.CandleQError, match="5 slots"):
         cache.reserve([0, 1, 2, 3, 0], 1)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("seqs,queries,hkv,per,dim,prompt,own", [(20, 4, 2, 16, 64, 70, 9), (130, 1, 1, 32, 128, 150, 5), (1, 1, 1, 1, 64, 0, 20000), (3, 1, 1, 2, 128, 9000, 40),
+                                                                 (1, 1, 8, 4, 128, 0, 4000)])
+def test_attention_of_many_and_few_rows(cuda_dev, dtype, seqs, queries, hkv, per, dim, prompt, own):
+    """From rows with one or two segments each to one row with more than a thousand: the joins by one, two and eight warps a row, the last in several rounds."""
+    cache, slots, g = _batch(dtype, 64, dim, hkv, [prompt], [[own] * seqs], seed=seqs, extra=1)
+    q = torch.randn((seqs, queries, hkv * per, dim), device="cuda", generator=g).to(dtype)
+    ref, tol = _attention64(cache, 0, q, slots, dim ** -0.5)
+    plan = cache.attention_plan(seqs, hkv * per, queries=queries)
+    plan.update(slots)
+    got = cache.attention(0, q, plan)
+    cache.check()
+    assert bool(((got.double() - ref).abs() <= tol).all()), float((got.double() - ref).abs().max()) / tol
+    assert torch.equal(got, cache.attention(0, q, plan))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_two_plans_on_two_streams(cuda_dev, dtype):
+    """Two batches over one cache at once, eager and from two graphs: each has its own plan, the cache is only read."""
+    cache, slots, g = _batch(dtype, 16, 64, 2, [300, 40], [[20, 30, 40], [7, 9]], seed=4)
+    parts = [torch.tensor(slots[:3], dtype=torch.int32, device="cuda"), torch.tensor(slots[3:], dtype=torch.int32, device="cuda")]
+    qs = [torch.randn((len(p), 1, 8, 64), device="cuda", generator=g).to(dtype) for p in parts]
+    plans = [cache.attention_plan(len(p), 8) for p in parts]
+    streams = [torch.cuda.Stream() for _ in parts]
+
+    def step(i):
+        plans[i].update(parts[i])
+        return cache.attention(0, qs[i], plans[i])
+
+    want = [step(i).clone() for i in range(2)]
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for i in range(2):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[i], stream=streams[i]):
+            outs.append(step(i))
+    for _ in range(5):
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                graphs[i].replay()
+    torch.cuda.synchronize()
+    assert torch.equal(outs[0], want[0]) and torch.equal(outs[1], want[1])
+    for _ in range(5):
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                outs[i] = step(i)
+    torch.cuda.synchronize()
+    assert torch.equal(outs[0], want[0]) and torch.equal(outs[1], want[1])
+    cache.check()
