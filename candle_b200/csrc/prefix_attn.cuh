@@ -17,7 +17,7 @@ struct Segment {
     int row0, rows;         // rows of the KV head
     int head;               // KV head
     int slot;               // whose table holds the pages
-    int key0, key1;         // positions [key0, key1), key0 a multiple of the page size
+    int key0, key1;         // positions [key0, key1), key0 a multiple of 16
     int part;               // first row of the partial results
     int units;
 };

@@ -219,7 +219,7 @@ class PagedKvCache:
 
 class AttentionPlan:
     """The division of a batch's attention into pieces, and the room for their results.  `update(slots)` makes it for the lengths and tables as they are, once a
-    step; all layers use it.  One plan serves one stream at a time."""
+    step; all layers use it.  One plan serves one stream at a time, and like any tensor it must outlive its use on a stream other than the one it was made on."""
 
     def __init__(self, cache: PagedKvCache, batch: int, heads: int, queries: int, groups):
         groups = [batch] if groups is None else [int(g) for g in groups]
