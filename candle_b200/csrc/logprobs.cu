@@ -17,7 +17,7 @@
 // Pointers carry no __restrict__: a read-only one would let the compiler move loads over the wait for the kernel before.
 namespace {
 
-constexpr int kThreads = 256, kWarps = kThreads / 32, kCtas = 3, kPer = 32, kChunk = 32 * kPer, kList = 512, kMaxTop = 32, kMaxSegments = 128;
+constexpr int kThreads = 256, kWarps = kThreads / 32, kCtas = 3, kPer = 32, kChunk = 32 * kPer, kMaxTop = 32, kMaxSegments = 128;
 
 // Keys order elements by (value descending, index ascending) as one unsigned comparison; 0: not an element of the row.
 __device__ __forceinline__ uint32_t ordered(float x) {
@@ -268,64 +268,49 @@ __global__ void __launch_bounds__(kThreads, kCtas) logprobs_segment_kernel(const
     }
 }
 
-// One CTA per row: the segments' sums (first warp) beside the best of their lists.  Where q segments have a j-th key from some key on, q j keys are from there on: with
-// q j >= top, the q-th largest of the j-th keys leaves few more than `top` keys to rank.  One such j, with q at most half the segments, and j = top do where the best are
-// spread over the row or lie together; where more than the list holds are left after these, all powers of two are tried.
-// Four warps do that, a fifth the sums, and all eight look for the keys that remain, which are asked for first.  (Four warps for all of it, one after the other: 2.2 us more
-// for one row of 128256 with 20 alternatives.)
-constexpr int kJoin = 256, kAhead = 8;
+// One CTA per row.  All bring the segments' lists to shared memory; one warp then joins the sums, another one merges the lists, which are in order: a lane has the heads of four, and
+// the largest of all heads is the next one.  (With what remains above a bound ranked by all warps one row of 128256 took, in a graph, 11.1 us for five alternatives and 13.5 for 20;
+// so it takes 6.2 and 10.3.  Where 32 are asked for of 8 rows or more the ranking was 1.3 us faster.)
+constexpr int kJoin = 256;
 template <typename T>
 __global__ void __launch_bounds__(kJoin) logprobs_join_kernel(const T *logits, int64_t stride, int vocab, int segments, int top, const Part *part_in, const uint64_t *keys_in,
                                                               const Out o) {
+    extern __shared__ uint64_t lists[];             // [segments][top]
     __shared__ float row_m, row_s;
-    __shared__ __align__(16) uint32_t firsts[kMaxSegments];
-    __shared__ uint64_t least;
-    __shared__ uint64_t list[kList];
-    __shared__ int count;
+    __shared__ uint64_t best[kMaxTop];
+    constexpr int kLane = kMaxSegments / 32, kAtOnce = 8;
     const int64_t r = blockIdx.x;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, all = segments * top;
     cq_pdl_launch_dependents();
     cq_pdl_wait();
     const Part *part = part_in + r * segments;
     const uint64_t *keys = keys_in + r * all;
-    const int j0 = top ? min(top, (2 * top + segments - 1) / segments) : 0;
-    uint64_t ahead[kAhead];
+    int64_t tok = -1;
+    Part a[kLane];
+    if (warp == 1) {
+        if (o.tokens) tok = o.tokens[r];
 #pragma unroll
-    for (int i = 0; i < kAhead; ++i) ahead[i] = top > 1 && tid + i * kJoin < all ? keys[tid + i * kJoin] : 0;
-    // the q-th largest value among the segments' j-th keys into `least`, if it is larger; the first four warps
-    auto raise = [&](int j) {
-        const uint32_t mine = tid < segments ? (uint32_t)(keys[tid * top + j - 1] >> 32) : 0;
-        asm volatile("bar.sync 1, 128;" ::: "memory");
-        firsts[tid] = mine;
-        asm volatile("bar.sync 1, 128;" ::: "memory");
-        int rank = 0;
-#pragma unroll 2
-        for (int i = 0; i < segments; i += 4) {
-            const uint4 v = *reinterpret_cast<const uint4 *>(&firsts[i]);
-            rank += (v.x > mine || (v.x == mine && i < tid)) + (v.y > mine || (v.y == mine && i + 1 < tid)) + (v.z > mine || (v.z == mine && i + 2 < tid)) +
-                    (v.w > mine || (v.w == mine && i + 3 < tid));
-        }
-        if (tid < segments && rank == (top + j - 1) / j - 1) atomicMax((unsigned long long *)&least, (unsigned long long)mine << 32);
-    };
-    if (tid == 0) { count = 0; least = 0; }
-    if (top > 1 && warp < kMaxSegments / 32) {
-        raise(j0);
-        if (j0 < top && tid < segments) atomicMax((unsigned long long *)&least, (unsigned long long)keys[tid * top + top - 1]);
+        for (int i = 0; i < kLane; ++i) a[i] = lane + 32 * i < segments ? part[lane + 32 * i] : Part{-INFINITY, 0.0f, 0.0f, 0.0f};
     }
-    if (warp == kMaxSegments / 32) {
-        const int64_t tok = o.tokens ? o.tokens[r] : -1;
-        const float at_tok = tok >= 0 && tok < vocab ? load_f(logits + r * stride + tok) : 0.0f;
-        Part a[kMaxSegments / 32];
+#pragma unroll 1
+    for (int i0 = tid; i0 < all; i0 += kAtOnce * blockDim.x) {
+        uint64_t v[kAtOnce];
+#pragma unroll
+        for (int i = 0; i < kAtOnce; ++i) v[i] = i0 + i * (int)blockDim.x < all ? keys[i0 + i * blockDim.x] : 0;
+#pragma unroll
+        for (int i = 0; i < kAtOnce; ++i)
+            if (i0 + i * (int)blockDim.x < all) lists[i0 + i * blockDim.x] = v[i];
+    }
+    const float at_tok = tok >= 0 && tok < vocab ? load_f(logits + r * stride + tok) : 0.0f;
+    __syncthreads();
+    if (warp == 1) {
         float m = -INFINITY, s = 0.0f, t = 0.0f;
 #pragma unroll
-        for (int i = 0; i < kMaxSegments / 32; ++i) {
-            a[i] = lane + 32 * i < segments ? part[lane + 32 * i] : Part{-INFINITY, 0.0f, 0.0f, 0.0f};
-            m = fmaxf(m, a[i].m);
-        }
+        for (int i = 0; i < kLane; ++i) m = fmaxf(m, a[i].m);
 #pragma unroll
         for (int x = 16; x > 0; x >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
 #pragma unroll
-        for (int i = 0; i < kMaxSegments / 32; ++i)
+        for (int i = 0; i < kLane; ++i)
             if (a[i].s != 0.0f) {                               // nothing but -inf: no weight, and no difference of infinities
                 const float d = fmaxf(a[i].m - m, -150.0f), f = expf(d);        // the difference of two finite values may be -inf
                 s = __fmaf_rn(f, a[i].s, s);
@@ -341,56 +326,38 @@ __global__ void __launch_bounds__(kJoin) logprobs_join_kernel(const T *logits, i
             row_m = m;
             row_s = s;
         }
+    } else if (warp == 0) {
+        uint64_t head[kLane], after[kLane];
+        int next[kLane];
+#pragma unroll
+        for (int i = 0; i < kLane; ++i) {
+            const int first = (lane + 32 * i) * top;
+            head[i] = first < all ? lists[first] : 0;
+            after[i] = first < all && top > 1 ? lists[first + 1] : 0;
+            next[i] = first + 2;
+        }
+#pragma unroll 1
+        for (int k = 0; k < top; ++k) {
+            uint64_t mine = head[0];
+#pragma unroll
+            for (int i = 1; i < kLane; ++i) mine = head[i] > mine ? head[i] : mine;
+            const uint32_t hi = __reduce_max_sync(0xffffffffu, (uint32_t)(mine >> 32));
+            const uint32_t lo = __reduce_max_sync(0xffffffffu, (uint32_t)(mine >> 32) == hi ? (uint32_t)mine : 0u);
+            const uint64_t key = (uint64_t)hi << 32 | lo;
+            if (lane == 0) best[k] = key;
+#pragma unroll
+            for (int i = 0; i < kLane; ++i)
+                if (head[i] == key && key != 0) {               // one lane's: indices differ
+                    head[i] = after[i];
+                    after[i] = next[i] < (lane + 32 * i + 1) * top ? lists[next[i]] : 0;
+                    ++next[i];
+                }
+        }
     }
     if (top == 0) return;
     __syncthreads();
-    const float m = row_m, s = row_s, ls = logf(s);
-    const bool ok = s > 0.0f && m < INFINITY;
-    if (!ok) {
-        if (tid < top) write_top(o, r, top, tid, 0, false, m, ls);
-        return;
-    }
-    if (top == 1) {
-        const uint64_t key = tid < segments ? keys[tid] : 0;
-        atomicMax((unsigned long long *)&least, (unsigned long long)key);
-        __syncthreads();
-        if (tid == 0) write_top(o, r, 1, 0, least, true, m, ls);
-        return;
-    }
-    auto collect = [&]() {
-        const uint64_t from_here = least;
-        auto look = [&](uint64_t key) {
-            if (key >= from_here && key != 0) {
-                const int at = atomicAdd(&count, 1);
-                if (at < kList) list[at] = key;
-            }
-        };
-#pragma unroll
-        for (int i = 0; i < kAhead; ++i) look(ahead[i]);
-        for (int i = tid + kAhead * kJoin; i < all; i += kJoin) look(keys[i]);
-        __syncthreads();
-    };
-    collect();
-    if (count > kList) {
-        if (warp < kMaxSegments / 32)
-            for (int j = 1; j < top; j *= 2) raise(j);
-        __syncthreads();
-        if (tid == 0) count = 0;
-        __syncthreads();
-        collect();
-    }
-    const uint64_t from_here = least;
-    const int n = count;                        // still too many for the list: all are ranked
-    const uint64_t *from = n <= kList ? list : keys;
-    const int total = n <= kList ? n : all;
-    for (int i = tid; i < total; i += kJoin) {
-        const uint64_t key = from[i];
-        if (key < from_here || key == 0) continue;
-        int rank = 0;
-#pragma unroll 4
-        for (int x = 0; x < total; ++x) rank += from[x] > key;
-        if (rank < top) write_top(o, r, top, rank, key, ok, m, ls);
-    }
+    const float m = row_m, s = row_s;
+    if (tid < top) write_top(o, r, top, tid, best[tid], s > 0.0f && m < INFINITY, m, logf(s));
 }
 
 int chunks_of(int vocab) { return (int)(((int64_t)vocab + 8 + kChunk - 1) / kChunk); }     // + 8: a row may start inside a 16-byte unit
@@ -423,7 +390,8 @@ void launch(const void *logits, int64_t stride, int rows, int vocab, int top, co
     const int most = kCtas * cq_sm_count(), want = (total + kWarps - 1) / kWarps;
     cq_launch_k(logprobs_segment_kernel<T>, dim3((unsigned)(want < most ? want : most)), dim3(kThreads), smem, st, (const T *)logits, stride, vocab, segments, per, total, top, part,
                 keys);
-    cq_launch_k(logprobs_join_kernel<T>, dim3((unsigned)rows), dim3(top > 1 ? kJoin : kMaxSegments + 32), 0, st, (const T *)logits, stride, vocab, segments, top, (const Part *)part, (const uint64_t *)keys, o);
+    cq_launch_k(logprobs_join_kernel<T>, dim3((unsigned)rows), dim3(top > 1 ? kJoin : 64), 8 * segments * top, st, (const T *)logits, stride, vocab, segments, top, (const Part *)part,
+                (const uint64_t *)keys, o);
 }
 
 }  // namespace
