@@ -3,7 +3,7 @@
 // The bookkeeping (reference counts, lengths, tables) lives on the device, so that a decode step that grows its sequences, or forks
 // one, is a sequence of launches that a graph can hold.  One CTA does it: a pool has some thousands of pages, and a page's number
 // depends on all that are taken before it.  What it decides, a second kernel copies with the whole device.
-// On a B200, each kernel by itself with cold caches: 63 forks of 16 pages 13 us, bound by some ten reads that depend on one another; the list of a compaction of 320
+// On a B200, each kernel by itself with cold caches: 63 forks of 16 pages 10 - 13 us, bound by some ten reads that depend on one another; the list of a compaction of 320
 // pages 5 us.
 #include <cstdio>
 
