@@ -231,7 +231,6 @@ template <typename T, int D, int W> __global__ void __launch_bounds__(256) prefi
     const int chunk = pl.header[1], own_chunk = pl.header[3], own_chunk2 = pl.header[4];
     constexpr int V = D / 32;
     float acc[V] = {}, m = -INFINITY, l = 0.0f;
-    bool some = false;
     if (q.len > 0) {
         // segments of an item: its units [start, start + units) of the line, cut at multiples of the chunk
         const int local = h * sh.own_tiles + tile, own_item = n * sh.kv_heads * sh.own_tiles + local;
@@ -247,7 +246,6 @@ template <typename T, int D, int W> __global__ void __launch_bounds__(256) prefi
         const int n_all = n_shared + n_own;
         const int64_t own0 = part_own(sh, call.shared_items, own_item + own_w) + in - tile * sh.own_rows;
         const int share = (n_all + W - 1) / W, begin = W > 1 ? warp * share : 0, end = W > 1 ? min(n_all, begin + share) : n_all;
-        some = begin < end;
         for (int x0 = begin; x0 < end; x0 += 32) {
             const bool more = x0 > begin;
             const int x = x0 + lane, count = min(32, end - x0);
@@ -269,8 +267,9 @@ template <typename T, int D, int W> __global__ void __launch_bounds__(256) prefi
             float big = fmaxf(m, ml.x);
 #pragma unroll
             for (int k = 16; k > 0; k >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, k));
-            // all scores so far -inf: no weight can be given, as in the formula (lanes without a segment have none)
-            const float w = lane < count ? exp2f(ml.x - big) : 0.0f, f = more ? exp2f(m - big) : 0.0f;
+            // all scores so far -inf: no weight yet, relative to anything finite; where it stays so the quotient of the sums is 0 / 0, a NaN as in the formula
+            const float base = big == -INFINITY ? 0.0f : big;
+            const float w = lane < count ? exp2f(ml.x - base) : 0.0f, f = more ? exp2f(m - base) : 0.0f;
             float sum = lane < count ? __fmul_rn(ml.y, w) : 0.0f;
 #pragma unroll
             for (int k = 16; k > 0; k >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, k);
@@ -291,7 +290,7 @@ template <typename T, int D, int W> __global__ void __launch_bounds__(256) prefi
         }
     }
     if constexpr (W > 1) {                  // the warps' shares, in their order
-        if (lane == 0) all_ml[warp] = make_float2(some ? m : NAN, l);
+        if (lane == 0) all_ml[warp] = make_float2(m, l);            // a share without segments: -inf, no weight
 #pragma unroll
         for (int i = 0; i < V; ++i) all_acc[warp][V * lane + i] = acc[i];
         __syncthreads();
@@ -299,13 +298,14 @@ template <typename T, int D, int W> __global__ void __launch_bounds__(256) prefi
         m = -INFINITY;
 #pragma unroll
         for (int w = 0; w < W; ++w) m = fmaxf(m, all_ml[w].x);
+        const float base = m == -INFINITY ? 0.0f : m;
         l = 0.0f;
 #pragma unroll
         for (int i = 0; i < V; ++i) acc[i] = 0.0f;
 #pragma unroll
         for (int w = 0; w < W; ++w) {
             const float2 ml = all_ml[w];
-            const float f = ml.x == ml.x ? exp2f(ml.x - m) : 0.0f;          // NaN: a share without segments
+            const float f = exp2f(ml.x - base);
             l = __fmaf_rn(f, ml.y, l);
 #pragma unroll
             for (int i = 0; i < V; ++i) acc[i] = __fmaf_rn(f, all_acc[w][V * lane + i], acc[i]);

@@ -128,3 +128,21 @@ def test_no_block_is_lost(cuda_dev, dtype, seqs, heads, prompt, own):
     _one_hot_values(cache)
     q = torch.randn((seqs, 1, heads, 128), device="cuda", generator=g).to(dtype)
     _check(cache, q, slots, None, 128 ** -0.5)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("seqs,heads", [(1, 1), (50, 32), (100, 32)])
+def test_segments_of_nothing_but_minus_infinity(cuda_dev, dtype, seqs, heads):
+    """A long context whose first third has scores of -inf, so that whole segments have no weight, and so has the first of the join's rounds or of its warps' shares (eight,
+    two and one of them a row).  Others have one key.  Nothing but -inf: NaN, as the formula gives."""
+    cache, slots, g = _batch(dtype, 64, 64, 1, [0], [[1] * (seqs - 1) + [20000]], seed=seqs)
+    _one_hot_values(cache)
+    q = torch.rand((seqs, 1, heads, 64), device="cuda", generator=g).to(dtype) + 0.5
+    ids = cache.tables[slots[-1]].long()
+    cache.k[0][ids[:105]] = -math.inf               # 6720 keys
+    _check(cache, q, slots, None, 0.125)
+    cache.k[0][ids] = -math.inf
+    plan = cache.attention_plan(seqs, heads)
+    plan.update(slots)
+    got = cache.attention(0, q, plan)
+    assert bool(torch.isnan(got[-1]).all()) and bool(torch.isfinite(got[:-1]).all())
