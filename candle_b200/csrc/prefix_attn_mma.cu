@@ -4,7 +4,7 @@
 // half's softmax warps owns row r, reads it there, and writes the weights 2^(s c - m), c = scale log2 e, back over it in 16 bits as the first operand of
 // O += P V.  512 columns, a half's scores and outputs twice: one half's softmax has the other's products beside it.
 //
-// Own items (as many rows as a KV head has query heads, keys from HBM): a warp is a worker of its own, 16 rows x 16 keys a step by mma.sync, with its
+// Own items (as many rows as a KV head has query heads, keys from HBM): a warp is a worker of its own, 8 rows x 16 keys a step by mma.sync, with its
 // next steps of keys and values on their way.  Through the first form an item of four rows costs the waits of a whole tile chain - QK, softmax, PV, some
 // 10,000 clocks for 64 KB - where HBM gives an SM 64 KB in 2,850.  Four such warps run beside the others, so that HBM and tensor
 // cores are both in use, and the softmax warps join them when the shared items are done.
@@ -13,8 +13,8 @@
 // and the exponentials would each take 2,050, beside some 220 own steps; 64 over 8191 (9 GFLOP, 185 MB) 41 us.
 //
 // In both m is the row's maximum so far, kept until a score passes it by 2^8 (weights up to 256 are as good as any, the sum has the same
-// factor), so that outputs are scaled in the first tiles only.  The sum adds the weights as rounded: rounding moves weight between keys but
-// not the total.  Keys and values of shared items come by tiled TMA copies of 64 dims and a page at a time, 128-byte swizzle: K as it is
+// factor), so that outputs are scaled in the first tiles only.  The sum adds the weights as rounded: rounding moves weight between keys, but
+// the weights given add up to 1.  Keys and values of shared items come by tiled TMA copies of 64 dims and a page at a time, 128-byte swizzle: K as it is
 // for the first product, V for the second with its rows as the K dimension.  Rows of a tile behind the last key hold whatever the page or the tile
 // before left there: their scores are masked, their values set to zero before the second product, since 0 x NaN is not 0.
 #include <cuda.h>
@@ -33,8 +33,9 @@ constexpr int kHalfBytes = 128 * 128;                        // 128 rows of 64 e
 constexpr int kGroup = 256, kO = 128;                        // columns of a half; in it the scores / weights and the outputs
 constexpr int kStep = 16;                                    // keys of a step of an own item
 // Weights of bf16 are 2^-24 of what was said, which the quotient of the sums loses again: 65536 of them add up to no more than 1, and values of any size do not overflow where
-// their mean does not.  f16's values cannot overflow an f32 sum, and its weights have no such range.
-template <bool BF16> constexpr float kDown = BF16 ? 24.0f : 0.0f;
+// their mean does not.  Those of f16 are 2^7 times that, up to 2^15 of the type's 65504, so that they are rounded by no more than 2^-11 of themselves down to 2^-21 of the
+// kept maximum and by 2^-32 of it below (without: 2^-14 and 2^-25, and 9,000 keys of 2^-24.5 beside one of 1 were 0.6 % off in sum); 2^15 * 65504 * 2^30 keys are finite in f32.
+template <bool BF16> constexpr float kDown = BF16 ? 24.0f : -7.0f;
 // registers a thread by warpgroup: 128 * (160 + 160 + 64 + 128) is what the block was launched with, 512 * 128
 constexpr int kRegsSoft = 160, kRegsMisc = 64, kRegsOwn = 128;
 static_assert(kCopyWarp == 8 && kMmaWarps == 4, "warp roles");

@@ -146,3 +146,37 @@ def test_segments_of_nothing_but_minus_infinity(cuda_dev, dtype, seqs, heads):
     plan.update(slots)
     got = cache.attention(0, q, plan)
     assert bool(torch.isnan(got[-1]).all()) and bool(torch.isfinite(got[:-1]).all())
+
+
+@pytest.mark.parametrize("below", [20.5, 24.5])
+@pytest.mark.parametrize("prompt,own,seqs", [(9000, 20, 40), (0, 9000, 3)])
+def test_one_key_over_many_small_ones_in_f16(cuda_dev, prompt, own, seqs, below):
+    """One key has nearly all the weight, and each of thousands of others 2^-20.5 or 2^-24.5 of it, less than f16's normal numbers: together they are what is left."""
+    cache, slots, g = _batch(torch.float16, 64, 64, 1, [prompt], [[own] * seqs], seed=5)
+    q = torch.zeros((seqs, 1, 4, 64), dtype=torch.float16, device="cuda")
+    q[..., 0] = 1.0
+    written = torch.isfinite(cache.k[0])
+    cache.k[0] = torch.where(written, -below * math.log(2.0), cache.k[0].float()).half()
+    cache.v[0] = torch.where(written, 1.0, cache.v[0].float()).half()
+    for s in [0] if prompt else slots:
+        cache.k[0, int(cache.tables[s, 3]), 0, 11] = 0.0
+        cache.v[0, int(cache.tables[s, 3]), 0, 11] = 0.0
+    got = _check(cache, q, slots, None, 1.0)
+    assert float(got.min()) > 0.0
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("prompt,own", [(9000, 30), (0, 9000)])
+def test_the_largest_values_of_f16(cuda_dev, dim, prompt, own):
+    """All weights at the top of their range and all values the largest number: the sums stay finite and so does their quotient."""
+    cache, slots, g = _batch(torch.float16, 16, dim, 1, [prompt], [[own] * 9], seed=3)
+    q = torch.full((9, 1, 4, dim), 0.5, dtype=torch.float16, device="cuda")
+    big = torch.finfo(torch.float16).max
+    for s in [0] + slots:           # scores that rise by 7.5 in powers of two once: not enough for the maximum to follow
+        n = int(cache.lens[s])
+        at = torch.arange(n, device="cuda")
+        ids = cache.tables[s].long()[at // 16]
+        cache.k[0][ids, :, at % 16] = ((at // 128 % 2) * (7.5 * math.log(2.0) / (0.5 * dim ** 0.5))).half()[:, None, None]
+        cache.v[0][ids, :, at % 16] = big
+    got = _check(cache, q, slots, None, dim ** -0.5)
+    assert float(got.min()) == big
