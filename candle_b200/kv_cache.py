@@ -21,6 +21,7 @@ from __future__ import annotations
 
 import ctypes as C
 import math
+import operator
 
 import numpy as np
 import torch
@@ -29,6 +30,13 @@ from . import capi
 from .capi import CandleQError
 
 _ELEM = {torch.float32: capi.F32, torch.float16: capi.F16, torch.bfloat16: capi.BF16}
+
+
+def _whole(values, what: str) -> list[int]:
+    try:
+        return [operator.index(v) for v in values]
+    except TypeError:
+        raise CandleQError(f"{what} must be a list of whole numbers") from None
 
 
 class PagedKvCache:
@@ -86,16 +94,18 @@ class PagedKvCache:
             if slots.dtype == torch.int32 and slots.device == self.device and slots.dim() == 1 and slots.is_contiguous() and slots.shape[0] <= self.max_seqs:
                 return slots
         else:
-            slots = [slots] if isinstance(slots, int) else list(slots)
-            if any(not 0 <= int(s) < self.max_seqs for s in slots):
+            slots = _whole([slots] if isinstance(slots, int) else slots, "PagedKvCache: slots")
+            if any(not 0 <= s < self.max_seqs for s in slots):
                 raise CandleQError(f"PagedKvCache: slots are 0 .. {self.max_seqs - 1}")
             if len(slots) <= self.max_seqs:
                 return torch.tensor(slots, dtype=torch.int32).to(self.device, non_blocking=True)       # pageable memory: copied aside before this returns
             slots = torch.tensor(slots, dtype=torch.int32)
-        if slots.dim() != 1 or slots.is_floating_point() or slots.dtype == torch.bool:
+        if slots.dim() != 1 or slots.is_floating_point() or slots.is_complex() or slots.dtype == torch.bool:
             raise CandleQError("PagedKvCache: slots must be a list of whole numbers")
         if slots.numel() > self.max_seqs:
             raise CandleQError(f"PagedKvCache: {slots.numel()} slots named, the cache has {self.max_seqs}")
+        if slots.dtype in (torch.int64, torch.uint32, torch.uint64):
+            slots = slots.to(torch.int64).clamp(-1, self.max_seqs)         # what int32 does not hold stays out of range
         return slots.to(device=self.device, dtype=torch.int32).contiguous()
 
     # ---- pages ----
@@ -222,7 +232,7 @@ class AttentionPlan:
     step; all layers use it.  One plan serves one stream at a time, and like any tensor it must outlive its use on a stream other than the one it was made on."""
 
     def __init__(self, cache: PagedKvCache, batch: int, heads: int, queries: int, groups):
-        groups = [batch] if groups is None else [int(g) for g in groups]
+        groups = [batch] if groups is None else _whole(groups, "attention_plan: groups")
         if any(g <= 0 for g in groups) or sum(groups) != batch:
             raise CandleQError(f"attention_plan: groups {groups} must be positive and add up to the batch of {batch}")
         self.cache, self.batch, self.heads, self.queries, self.updated = cache, batch, heads, queries, False
