@@ -325,73 +325,126 @@ struct AppendArgs {
     int layer, batch, t, hq, max_pos, neox;
 };
 
+// What is looked at before any row of an append is stored: each slot, and the pages of its last t positions, at most `per` of them.
+__device__ __forceinline__ int append_fault(const State &s, const AppendArgs &a, int slot, int len, int page, int refs) {
+    if (slot < 0 || slot >= s.max_seqs) return kBadSlot;
+    if (len < a.t || len > s.max_pages * s.page || (a.cosv && len > a.max_pos)) return kBadPosition;
+    if (page < 0 || page >= s.pages) return kBadPage;
+    return refs > 1 ? kBadPosition : kOk;                   // others read it
+}
+// The table entry of position `pos` of a slot, kept inside the tables so that it can be read before slot and position are known to be right.
+__device__ __forceinline__ int entry_of(const State &s, int slot, int pos, int shift) {
+    const bool there = slot >= 0 && slot < s.max_seqs;
+    return there ? slot * s.max_pages + min(max(pos >> shift, 0), s.max_pages - 1) : 0;
+}
+// The item-th check by itself; `seen`: the slots that were named so far.
+__device__ __forceinline__ int append_check(const State &s, const AppendArgs &a, unsigned *seen, int item, int per, int shift) {
+    const int b = item / per, j = item - b * per, slot = a.slots[b];
+    if (slot < 0 || slot >= s.max_seqs) return kBadSlot;
+    if (j == 0 && atomicOr(&seen[slot >> 5], 1u << (slot & 31)) >> (slot & 31) & 1) return kBadSlot;
+    const int len = s.lens[slot], pos = min(((len - a.t) >> shift << shift) + (j << shift), len - 1), page = s.tables[entry_of(s, slot, pos, shift)];
+    return append_fault(s, a, slot, len, page, page >= 0 && page < s.pages ? s.refs[page] : 0);
+}
+
+// The checks of a call with many: a fault before the rows' kernel looks for one.
+__global__ void __launch_bounds__(kMeta) kv_append_check_kernel(const cq_kv_cache cache, const AppendArgs a, int per) {
+    extern __shared__ unsigned seen[];
+    __shared__ int err;
+    const State s = state_of(cache);
+    const int shift = 31 - __clz(s.page);
+    for (int i = threadIdx.x; i < (s.max_seqs + 31) / 32; i += kMeta) seen[i] = 0;
+    if (threadIdx.x == 0) err = kOk;
+    cq_pdl_launch_dependents();
+    __syncthreads();
+    cq_pdl_wait();
+    int wrong = kOk;
+#pragma unroll 4
+    for (int64_t item = threadIdx.x; item < (int64_t)a.batch * per; item += kMeta) wrong = max(wrong, append_check(s, a, seen, (int)item, per, shift));
+    if (wrong) atomicMax(&err, wrong);
+    __syncthreads();
+    if (threadIdx.x == 0 && err) atomicCAS(s.header, kOk, err);
+}
+
 // A thread takes four rotary pairs of one head: eight consecutive elements (interleaved), or four and the four half a head further.
 // grid.x covers the heads of q, k and v of a row, grid.y the rows, R of them at a time: their elements are asked for before their places are looked up, which is a chain of
-// three reads (a fourth finds whether others read the page).  One read and one write of each element are the bound: 2047 rows of 48 heads of 128, f32, 102 MB in 22.4 us, 4.5 TB/s;
-// 64 rows take 2.6 us, a launch and the chain (both in a graph).
+// three reads, with cos and sin at its end.  Every CTA makes all `checks` of the call, one a thread beside its first rows' chain, so all of them come to the same answer without
+// a word between them, and a call is stored whole or not at all.  (0.25 us of 64 rows; an arrival counter, so that a fault shows when all CTAs have read that there was none
+// before, took 2.5 ns a CTA: 300 rows 9.1 us.)
+// One read and one write of each element are the bound: 2047 rows of 48 heads of 128, f32, 102 MB in 21.4 us, 4.8 TB/s; 64 rows take 2.95 us, a launch and the chain, 300 rows 5.1
+// (all in a graph).
 template <typename In, typename T, int R>
-__global__ void __launch_bounds__(128) kv_append_kernel(const cq_kv_cache cache, const AppendArgs a) {
+__global__ void __launch_bounds__(128) kv_append_kernel(const cq_kv_cache cache, const AppendArgs a, int checks, int per) {
     extern __shared__ unsigned seen[];
     const State s = state_of(cache);
+    const int tid = threadIdx.x;
     cq_pdl_launch_dependents();
-    cq_pdl_wait();
-    if (blockIdx.x == 0 && blockIdx.y == 0) {           // a slot named twice would have two writers for its positions
-        for (int i = threadIdx.x; i < (s.max_seqs + 31) / 32; i += 128) seen[i] = 0;
+    if (checks && a.batch > 1) {
+        for (int i = tid; i < (s.max_seqs + 31) / 32; i += 128) seen[i] = 0;
         __syncthreads();
-        for (int i = threadIdx.x; i < a.batch; i += 128) {
-            const int slot = a.slots[i];
-            if (slot >= 0 && slot < s.max_seqs && (atomicOr(&seen[slot >> 5], 1u << (slot & 31)) >> (slot & 31) & 1)) atomicCAS(s.header, kOk, kBadSlot);
-        }
     }
+    cq_pdl_wait();
     const int shift = 31 - __clz(s.page), d = cache.head_dim, log_per = d == 128 ? 4 : 3, hkv = cache.kv_heads, hq = a.q ? a.hq : 0;
-    const int unit = blockIdx.x * 128 + threadIdx.x, head = unit >> log_per, x = unit & ((1 << log_per) - 1);
-    if (head >= hq + 2 * hkv) return;
+    const int unit = blockIdx.x * 128 + tid, x = unit & ((1 << log_per) - 1);
+    const bool there = unit >> log_per < hq + 2 * hkv;              // the last CTA's other threads only check
+    const int head = there ? unit >> log_per : 0;
     const bool is_q = head < hq, is_v = head >= hq + hkv;
     const int first = a.neox ? 4 * x : 8 * x, second = a.neox ? first + d / 2 : first + 4, own = is_q ? head : is_v ? head - hq - hkv : head - hq;
     const In *from = reinterpret_cast<const In *>(is_q ? a.q : is_v ? a.v : a.k) + (int64_t)own * d;
     const int64_t stride = is_q ? a.q_stride : is_v ? a.v_stride : a.k_stride;
     const int rows = a.batch * a.t, step = gridDim.y;
+    const int fault = s.header[0];
+    int wrong = kOk;
+    for (int item = tid + 128; item < checks; item += 128) wrong = max(wrong, append_check(s, a, seen, item, per, shift));
+    bool stop = false;
     for (int row0 = blockIdx.y; row0 < rows; row0 += R * step) {
         Vec<In, 4> lo[R], hi[R];
-        int pos[R], page[R], code[R];
+        int pos[R], page[R];
 #pragma unroll
         for (int i = 0; i < R; ++i) {
             const In *src = from + (int64_t)min(row0 + i * step, rows - 1) * stride;
             lo[i] = *reinterpret_cast<const Vec<In, 4> *>(src + first);
             hi[i] = *reinterpret_cast<const Vec<In, 4> *>(src + second);
         }
-        const int fault = s.header[0];
+        // The chains: those of the rows and, the first time, that of a check.  All read inside the tables, whatever the numbers are; what they mean is looked at behind.
+        const bool check = row0 == blockIdx.y && tid < checks;
+        int slot[R + 1], len[R + 1], entry[R + 1];
+#pragma unroll
+        for (int i = 0; i <= R; ++i) {
+            const int row = min(row0 + i * step, rows - 1), b = i < R ? (a.t == 1 ? row : row / a.t) : check ? (per == 1 ? tid : tid / per) : 0;
+            slot[i] = a.slots[b];
+            if (i < R) pos[i] = row - b * a.t - a.t;
+        }
+        const int j = per == 1 ? 0 : tid % per;
+        unsigned twice = 0;                     // a slot named twice would have two writers for its positions
+        if (check && a.batch > 1 && j == 0 && slot[R] >= 0 && slot[R] < s.max_seqs) twice = atomicOr(&seen[slot[R] >> 5], 1u << (slot[R] & 31)) >> (slot[R] & 31) & 1;
+#pragma unroll
+        for (int i = 0; i <= R; ++i) len[i] = s.lens[slot[i] >= 0 && slot[i] < s.max_seqs ? slot[i] : 0];
 #pragma unroll
         for (int i = 0; i < R; ++i) {
-            const int row = min(row0 + i * step, rows - 1), b = a.t == 1 ? row : row / a.t, slot = a.slots[b];
-            pos[i] = page[i] = -1;
-            code[i] = kBadSlot;
-            if (fault) code[i] = -1;
-            else if (slot >= 0 && slot < s.max_seqs) {
-                pos[i] = s.lens[slot] - a.t + (row - b * a.t);
-                code[i] = kBadPosition;
-                if (pos[i] >= 0 && pos[i] < s.max_pages * s.page && (!a.cosv || pos[i] < a.max_pos)) {
-                    page[i] = s.tables[(size_t)slot * s.max_pages + (pos[i] >> shift)];
-                    code[i] = page[i] >= 0 && page[i] < s.pages ? kOk : kBadPage;
-                    if (code[i] == kOk && !is_q && s.refs[page[i]] > 1) code[i] = kBadPosition;         // others read it
-                }
-            }
+            pos[i] += len[i];
+            entry[i] = entry_of(s, slot[i], pos[i], shift);
         }
+        entry[R] = entry_of(s, slot[R], min(((len[R] - a.t) >> shift << shift) + (j << shift), len[R] - 1), shift);
+#pragma unroll
+        for (int i = 0; i < R; ++i) page[i] = s.tables[entry[i]];
+        const int check_page = s.tables[entry[R]];
         float4 c[R], n[R];
 #pragma unroll
-        for (int i = 0; i < R; ++i) {
-            c[i] = n[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (code[i] == kOk && !is_v && a.cosv) {
-                c[i] = *reinterpret_cast<const float4 *>(a.cosv + (int64_t)pos[i] * (d / 2) + 4 * x);
-                n[i] = *reinterpret_cast<const float4 *>(a.sinv + (int64_t)pos[i] * (d / 2) + 4 * x);
+        for (int i = 0; i < R; ++i)
+            if (!is_v && a.cosv) {
+                const int64_t at = (int64_t)min(max(pos[i], 0), a.max_pos - 1) * (d / 2) + 4 * x;
+                c[i] = *reinterpret_cast<const float4 *>(a.cosv + at);
+                n[i] = *reinterpret_cast<const float4 *>(a.sinv + at);
             }
+        if (row0 == blockIdx.y) {
+            if (check) wrong = max(wrong, twice ? (int)kBadSlot : append_fault(s, a, slot[R], len[R], check_page, s.refs[check_page >= 0 && check_page < s.pages ? check_page : 0]));
+            stop = checks ? __syncthreads_or(fault | wrong) != 0 : fault != 0;
+            if (wrong && blockIdx.x == 0 && blockIdx.y == 0) atomicCAS(s.header, kOk, wrong);
         }
 #pragma unroll
         for (int i = 0; i < R; ++i) {
             const int64_t row = row0 + (int64_t)i * step;
-            if (row >= rows) break;
-            if (code[i] > kOk && x == 0) atomicCAS(s.header, kOk, code[i]);
-            if (code[i] != kOk && !is_q) continue;
+            if (row >= rows || !there || (stop && !is_q)) break;
             Vec<T, 4> out_lo, out_hi;
             if (is_v || !a.cosv) {
 #pragma unroll
@@ -417,7 +470,7 @@ __global__ void __launch_bounds__(128) kv_append_kernel(const cq_kv_cache cache,
             }
             T *dst;
             if (is_q) {
-                if (code[i] != kOk)
+                if (stop)
 #pragma unroll
                     for (int y = 0; y < 4; ++y) out_lo.v[y] = out_hi.v[y] = from_f<T>(0.0f);
                 dst = reinterpret_cast<T *>(a.q_out) + (row * hq + head) * d;
@@ -430,13 +483,20 @@ __global__ void __launch_bounds__(128) kv_append_kernel(const cq_kv_cache cache,
     }
 }
 
+// Up to this many checks every CTA makes them all (2047 rows over pages of 16: 129, two a thread); beyond, a kernel before it.
+constexpr int kChecksInside = 512;
+
 template <typename In, typename T> void append_launch(const cq_kv_cache &c, const AppendArgs &a, cudaStream_t st) {
     const unsigned units = ((a.q ? a.hq : 0) + 2 * c.kv_heads) * (c.head_dim / 8), x = (units + 127) / 128, rows = (unsigned)a.batch * a.t;
     const size_t smem = (size_t)(c.max_seqs + 31) / 32 * 4;
+    const int per = (a.t + c.page_size - 2) / c.page_size + 1;             // pages that t positions can lie in
+    const bool inside = (int64_t)a.batch * per <= kChecksInside;
+    const int checks = inside ? a.batch * per : 0;
+    if (!inside) cq_launch_k(kv_append_check_kernel, dim3(1), dim3(kMeta), smem, st, c, a, per);
     // four rows a thread where that still fills the device (16 such CTAs an SM); one where latency counts
     if (x * rows >= 4u * 16 * cq_sm_count())
-        cq_launch_k(kv_append_kernel<In, T, 4>, dim3(x, (rows + 3) / 4 < 65535 ? (rows + 3) / 4 : 65535), dim3(128), smem, st, c, a);
-    else cq_launch_k(kv_append_kernel<In, T, 1>, dim3(x, rows < 65535 ? rows : 65535), dim3(128), smem, st, c, a);
+        cq_launch_k(kv_append_kernel<In, T, 4>, dim3(x, (rows + 3) / 4 < 65535 ? (rows + 3) / 4 : 65535), dim3(128), smem, st, c, a, checks, per);
+    else cq_launch_k(kv_append_kernel<In, T, 1>, dim3(x, rows < 65535 ? rows : 65535), dim3(128), smem, st, c, a, checks, per);
 }
 
 bool slots_ok(const cq_kv_cache *c, const int *a, const int *b, int n, const char *who) {

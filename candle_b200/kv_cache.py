@@ -169,7 +169,7 @@ class PagedKvCache:
 
     def append(self, layer: int, slots, k: torch.Tensor, v: torch.Tensor, q: torch.Tensor | None = None, rotary=None, neox: bool = False):
         """Keys and values [batch, tokens, kv_heads, head_dim] (f32, f16, bf16) of the last `tokens` positions of the slots, which `reserve` has added (a position in a
-        page that other slots share is a fault).  With
+        page that other slots share is a fault; with a fault in any row nothing is stored, and zeros are returned).  With
         `rotary` = (cos, sin), each [positions, head_dim / 2] f32, k and q are rotated at their sequence's own positions: pairs (2i, 2i + 1), with `neox`
         (i, i + head_dim / 2).  Returns q [batch, tokens, heads, head_dim] in the cache's type, or None."""
         s = self.slot_list(slots)

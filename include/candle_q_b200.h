@@ -432,7 +432,8 @@ int cq_glue_position_overflow_flag(void);
  *                   (i, i + head_dim / 2).  q, k, v: batch * t rows of q_stride / k_stride / v_stride elements of type
  *                   in_elem, heads side by side, rows 16-byte aligned; q_out: [batch, t, hq, head_dim] of the cache's type
  *                   (it may be q itself where type and stride agree).  q and q_out may be null.  Sums in f32, one rounding.
- *                   A row that cannot be stored gives q_out zeros and a fault; so is one in a page that other slots share.
+ *                   One row that cannot be stored - a position not reserved, past the rotary tables or in a page that other
+ *                   slots share, a slot named twice - is a fault: nothing is stored then, and q_out is zeros.
  *   cq_kv_take_fault : the fault of the cache (0: none; 1 slot, 2 out of pages, 3 too long, 4 occupied, 5 page number, 6 position, 7 a wait inside the attention),
  *                   which is cleared; synchronises the stream and sets the status.  -1: the CUDA call failed. */
 typedef struct cq_kv_cache {

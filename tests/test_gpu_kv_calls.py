@@ -38,3 +38,53 @@ def test_lists_of_other_than_whole_numbers_are_refused(cuda_dev):
     with pytest.raises(capi.CandleQError, match="whole numbers"):
         cache.attention_plan(2, 1, groups=[1.5, 1])
     assert cache.lens.tolist() == [0, 0, 0, 0]
+
+
+KINDS = {"slot": "out of range", "twice": "named twice", "long": "position", "rotary": "position", "shared": "shared page", "table": "not there"}
+
+
+@pytest.mark.parametrize("kind", list(KINDS))
+@pytest.mark.parametrize("where", [0, 2])
+@pytest.mark.parametrize("batch,t,page,hkv,hq", [(3, 1, 16, 1, 1), (3, 40, 16, 3, 5), (3, 3000, 64, 4, 4), (3, 3000, 16, 1, 2), (300, 1, 16, 2, 2), (600, 2, 16, 1, 1)])
+def test_a_faulted_append_does_nothing(cuda_dev, kind, where, batch, t, page, hkv, hq):
+    """One slot of many cannot be stored, the first or the last: nothing is stored, no query given, whoever finds it; a second call does nothing either; the state is as it was, and
+    once the fault is taken the call without that slot does all.  From one check to one a thread, several a thread (300 and 141 of them), and more (564, 1200)."""
+    if kind == "rotary" and where == 0:
+        pytest.skip("the tables end for the longest sequence")
+    per = -(-(t + 40) // page)
+    cache = _make((batch + 1) * per + 2, page, hkv, 64, batch + 2, per * page, torch.bfloat16)
+    g = torch.Generator(device="cuda").manual_seed(batch + t)
+    every = torch.arange(batch, dtype=torch.int32, device="cuda")
+    bad = 0 if where == 0 else batch - 1
+    cache.reserve(every, t)
+    cache.reserve([bad], 20)                    # the longest
+    slots, rotary = every.clone(), (torch.ones((t + 20, 32), device="cuda"), torch.zeros((t + 20, 32), device="cuda"))
+    if kind == "slot":
+        slots[bad] = batch + 2
+    elif kind == "twice":
+        slots[bad] = 1
+    elif kind == "long":
+        slots[bad] = batch + 1                  # an empty one
+    elif kind == "rotary":
+        rotary = tuple(x[:-1].contiguous() for x in rotary)
+    elif kind == "shared":                      # in the middle of a prompt, else the page of the row
+        cache.refs[cache.tables[bad, (int(cache.lens[bad]) - 1 - t // 2) // page].long()] += 1
+    else:
+        cache.tables[bad, (int(cache.lens[bad]) - 1 - t // 2) // page] = cache.pages
+    q, k, v = (torch.randn((batch, t, h, 64), device="cuda", generator=g).to(torch.bfloat16) for h in (hq, hkv, hkv))
+    was = cache.k.clone(), cache.v.clone(), cache.state[16:].clone()
+    for _ in range(2):
+        assert float(cache.append(0, slots, k, v, q=q, rotary=rotary).abs().max()) == 0.0
+        good = every[:1] if bad else every[1:2]
+        assert float(cache.append(0, good, k[:1], v[:1], q=q[:1]).abs().max()) == 0.0
+        cache.reserve(good, 0 if t > 1 else 1)
+        assert torch.equal(cache.k, was[0]) and torch.equal(cache.v, was[1]) and torch.equal(cache.state[16:], was[2])
+        _faulted(cache, KINDS[kind])
+    rest = torch.cat([every[:bad], every[bad + 1:]])
+    pick = rest.long()
+    assert torch.equal(cache.append(0, rest, k[pick], v[pick], q=q[pick], rotary=rotary), q[pick])
+    cache.check()
+    for i in rest.tolist()[:3] + rest.tolist()[-3:]:
+        at = torch.arange(int(cache.lens[i]) - t, int(cache.lens[i]), device="cuda")
+        ids = cache.tables[i].long()[at // page]
+        assert torch.equal(cache.k[0][ids, :, at % page], k[i]) and torch.equal(cache.v[0][ids, :, at % page], v[i])
