@@ -47,7 +47,7 @@ template <int D> struct Tiles {
     uint8_t q[2][D / 64][kHalfBytes], kv[kRing][D / 64][kHalfBytes];
     Step<D> step[kMmaWarps][kStages];
     uint64_t full[kRing], free[kRing];
-    uint64_t q_bar[2], s_bar[2], p_bar[2], o_bar[2];         // by half: rows there, scores there, weights there, outputs there
+    uint64_t q_bar[2], s_bar[2], p_bar[2], o_bar[2], e_bar[2];         // by half: rows there, scores there, weights there, outputs there, outputs on their way out
     uint32_t tmem;
     int abort;
 };
@@ -121,7 +121,7 @@ __device__ bool softmax_part(Tiles<D> &sm, const Call &call, const CUtensorMap &
     volatile int *abort_flag = &sm.abort;
     SharedWalk walk(call, blockIdx.x);
     Segment seg;
-    unsigned tile = 0;                      // of this half
+    unsigned tile = 0, segments = 0;        // of this half
     while (walk.next(call, seg)) {
         const int rows = min(seg.rows - half * 128, 128), row0 = seg.row0 + half * 128;
         if (rows <= 0) continue;
@@ -230,7 +230,8 @@ __device__ bool softmax_part(Tiles<D> &sm, const Call &call, const CUtensorMap &
             tc_fence_before();
         }
         if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
-        asm volatile("bar.sync %0, 128;" ::"r"(1 + half) : "memory");           // before the next Q
+        arrive_warp(&sm.e_bar[half], lane);                 // before the next Q; not a barrier without a limit, since a warp may have given up
+        if (!wait_warp(&sm.e_bar[half], segments++ & 1, abort_flag)) return false;
     }
     if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
     return true;
@@ -564,7 +565,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_mma_kernel(const cq_kv_cac
     const cq_kv::State st = cq_kv::state_of(cache);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     if (tid == 0) {
-        for (int i = 0; i < 2; ++i) { cq_mbar_init(&sm.q_bar[i], 4); cq_mbar_init(&sm.s_bar[i], 1); cq_mbar_init(&sm.p_bar[i], 4); cq_mbar_init(&sm.o_bar[i], 1); }
+        for (int i = 0; i < 2; ++i) { cq_mbar_init(&sm.q_bar[i], 4); cq_mbar_init(&sm.s_bar[i], 1); cq_mbar_init(&sm.p_bar[i], 4); cq_mbar_init(&sm.o_bar[i], 1); cq_mbar_init(&sm.e_bar[i], 4); }
         for (int i = 0; i < kRing; ++i) { cq_mbar_init(&sm.full[i], 1); cq_mbar_init(&sm.free[i], 1); }
         sm.abort = 0;
         cq_fence_mbar_init();
