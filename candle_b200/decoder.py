@@ -421,7 +421,7 @@ class LlamaShapedDecoder:
         """The `n` (up to 32) most probable first tokens after prompt int64 [1, Tp], each continued greedily to `steps` tokens, with the log probabilities of all tokens and
         the entropies of the distributions they come from - what a program needs to choose among continuations.  The prompt is read and stored once: the continuations
         share its pages and one pass of the attention over them.  Logits that are not a distribution (a NaN among them) give the token -1 and NaN.  Needs `use_pages`;
-        starts from an empty cache and leaves it empty."""
+        starts from an empty cache and leaves it empty, also when it fails."""
         kv, cfg = self.kv, self.cfg
         if kv is None:
             raise ValueError("branches: no paged cache (use_pages)")
@@ -431,19 +431,21 @@ class LlamaShapedDecoder:
             raise ValueError(f"prompt of {prompt.shape[1]} tokens plus {steps} steps exceeds max_pos = {cfg.max_pos}")
         kv.reset()
         self.reset()
-        best = token_logprobs(self._prompt_pages(prompt), top=n)
-        tokens, logprobs, entropy = [best.top_ids[0]], [best.top_logprobs[0]], [best.entropy.expand(n)]
-        slots = torch.arange(n, dtype=torch.int32, device=self.device)
-        if n > 1:
-            kv.fork(torch.zeros(n - 1, dtype=torch.int32, device=self.device), slots[1:].contiguous())
-        plan = kv.attention_plan(n, self.hq_l)
-        for _ in range(steps - 1):
-            # logits that are no distribution have the token -1: it goes on as -1, but is not looked up
-            got = token_logprobs(self.forward_pages(tokens[-1].clamp(min=0).unsqueeze(1), slots, plan), top=1)
-            tokens.append(got.top_ids[:, 0])
-            logprobs.append(got.top_logprobs[:, 0])
-            entropy.append(got.entropy)
-        kv.free(slots)
-        kv.check()
-        self.check()
+        try:
+            best = token_logprobs(self._prompt_pages(prompt), top=n)
+            tokens, logprobs, entropy = [best.top_ids[0]], [best.top_logprobs[0]], [best.entropy.expand(n)]
+            slots = torch.arange(n, dtype=torch.int32, device=self.device)
+            if n > 1:
+                kv.fork(torch.zeros(n - 1, dtype=torch.int32, device=self.device), slots[1:].contiguous())
+            plan = kv.attention_plan(n, self.hq_l)
+            for _ in range(steps - 1):
+                # logits that are no distribution have the token -1: it goes on as -1, but is not looked up
+                got = token_logprobs(self.forward_pages(tokens[-1].clamp(min=0).unsqueeze(1), slots, plan), top=1)
+                tokens.append(got.top_ids[:, 0])
+                logprobs.append(got.top_logprobs[:, 0])
+                entropy.append(got.entropy)
+            kv.check()
+            self.check()
+        finally:
+            kv.reset()
         return Branches(torch.stack(tokens, 1), torch.stack(logprobs, 1), torch.stack(entropy, 1))

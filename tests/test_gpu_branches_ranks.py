@@ -105,3 +105,18 @@ def test_branches_of_two_ranks(cuda_dev, monkeypatch, dtype, n_tokens, n, steps)
     for a, b in zip(got[0], want):
         assert a.shape == b.shape and torch.equal(a[:, 0], b[:, 0])
     assert checked.count(0) == checked.count(1) == cfg.layers * (steps - 1)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_the_cache_is_left_empty(cuda_dev, dtype):
+    """Also where there were too few pages, found at the end."""
+    m = LlamaShapedDecoder(DecoderConfig.tiny(), "cuda:0", batch=1, seed=5)
+    kv = m.use_pages(4, page_size=16, max_seqs=3, dtype=dtype)
+    prompt = torch.zeros((1, 20), dtype=torch.int64, device="cuda")
+    m.branches(prompt, 3, 2)
+    assert not bool(kv.lens.any()) and not bool(kv.refs.any()) and bool((kv.tables == -1).all())
+    with pytest.raises(Exception, match="out of pages"):
+        m.branches(prompt, 3, 20)
+    assert not bool(kv.lens.any()) and not bool(kv.refs.any()) and bool((kv.tables == -1).all())
+    kv.check()
+    m.branches(prompt, 3, 2)
