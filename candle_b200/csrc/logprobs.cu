@@ -1,8 +1,9 @@
 // Log probabilities of given tokens, the entropy of their distributions, and the best alternatives, from rows of logits.
 //
-//   M = max x,  S = sum e^(x - M),  T = sum e^(x - M) (x - M):   log p(t) = (x_t - M) - ln S,   entropy = ln S - T / S
-// (T <= 0, so the entropy is a sum of two terms that are not negative.)  Parts of a row are joined by M = max M_p, f_p = e^(M_p - M),
-// S = sum f_p S_p, T = sum f_p (T_p + S_p (M_p - M)).
+//   S = sum e^(x - M),  T = sum e^(x - M) (x - M):   log p(t) = (x_t - M) - ln S,   entropy = ln S - T / S
+// with any M near the maximum: here an element of the row, the maximum or no more than 2 below it.  With the maximum T <= 0 and the entropy is a sum of two terms that are not
+// negative.  With less T may be positive and the entropy a difference, but not a small one: M's own element has at least e^-2 of the largest weight then, so that the entropy is
+// 0.36 or more.  Parts of a row are joined by M = max M_p, f_p = e^(M_p - M), S = sum f_p S_p, T = sum f_p (T_p + S_p (M_p - M)).
 //
 // One read of the logits is the bound.  A warp walks one segment of a row in chunks of 1024 elements, 32 a lane, the next chunk on its way to shared memory; nothing waits
 // for another warp.  Each lane keeps a maximum, S and T of its own; the maximum follows only where a chunk's is more than 2 higher (S and T have any base near the maximum;

@@ -1,7 +1,7 @@
 // Segments of the shared-prefix attention (prefix_attn.cuh) of f32 caches: f32 products from three tf32 ones on the tensor cores.
 //
-// x = h + l with h the nearest number of 11 significant bits, l = x - h exact, of either sign and no more than 2^-11 |x|, cut to 11 bits by the instruction:
-// a b = h h' + h l' + l h' up to 2^-24 (l l') and 2^-21 of either sign (the cuts) of |a b|.  (With h cut instead of rounded all errors have one sign: an output was
+// x = h + l with h the nearest number of 11 significant bits, l = x - h exact, of either sign, no more than 2^-11 |x| and 12 bits long, cut to 11 by the instruction:
+// a b = h h' + h l' + l h' up to 2^-22 (l l', of either sign) and 2^-23 for each of the two cuts, together 2^-21 of |a b|.  (With h cut instead of rounded all errors have one sign: an output was
 // 2e-6 off where plain f32 is 6e-7.)  The instruction's own sums are cut as well, so chains are short: scores have an accumulator for every 32 dims and two for the low parts, and the outputs' products of a step
 // go to fresh ones that are added to the outputs by f32 additions.
 // mma.sync m16n8k8 does 474 products a clock and SM here (measured), so 158 of these, against 128 fused products of the f32 pipe that would want their

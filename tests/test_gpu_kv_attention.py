@@ -5,7 +5,7 @@ Values are one-hot by blocks of 16 positions, so that an output is the weight of
 
 Tolerance, for each output by itself.  With weights w (1 + d), |d| <= e, the quotient sum w v / sum w moves by at most 2 e / (1 - e) sum p |v|; the result is rounded once, u |out|.
 e has
-  the score's error: f32 products of three tf32 ones drop l l', 2^-22 of |a b|, and cut both l's, 2^-21 each: 1.25 * 2^-20; f16 and bf16 products are exact; the sums over d are cut,
+  the score's error: f32 products of three tf32 ones drop l l', 2^-22 of |a b|, and cut both l's by a bit, 2^-23 each; f16 and bf16 products are exact; the sums over d are cut,
     (d / 8 + 8) 2^-23 of sum |q k|; scale, log2 e and the difference from the maximum are rounded, 4 * 2^-24 of the largest |score|, and 2^-22 is ex2's own;
   the weight's rounding to 16 bits, u, in the product and in the sum alike;
   sums of weights: a step for every 16 keys of the longest context and 64 for lanes, warps and the join, 2^-23 each.
@@ -55,7 +55,7 @@ def _exact(cache, layer, q, slots, scale):
         terms = max(terms, float(torch.matmul(qi.abs(), finite.transpose(1, 2)).max()) * scale)
         score = max(score, float(sc[torch.isfinite(sc)].abs().max()) if bool(torch.isfinite(sc).any()) else 0.0)
     u, f32, n = U[cache.dtype], cache.dtype == torch.float32, max(lens)
-    e = terms * ((1.25 * 2.0 ** -20 if f32 else 0.0) + (d / 8 + 8) * 2.0 ** -23) + score * 4 * 2.0 ** -24 + 2.0 ** -22 + (0.0 if f32 else u) + (n / 16 + 64) * 2.0 ** -23
+    e = terms * ((2.0 ** -21 if f32 else 0.0) + (d / 8 + 8) * 2.0 ** -23) + score * 4 * 2.0 ** -24 + 2.0 ** -22 + (0.0 if f32 else u) + (n / 16 + 64) * 2.0 ** -23
     tol = 2 * e / (1 - e) * size + u * out.abs()
     return out, tol + (n * 2.0 ** -32 * float(size.max()) * 2 if cache.dtype == torch.float16 else 0.0)
 
