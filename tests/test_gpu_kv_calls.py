@@ -3,6 +3,7 @@ import pytest
 import torch
 
 from candle_b200 import capi
+from candle_b200.kv_cache import PagedKvCache
 from test_gpu_kv_cache import _make
 
 pytestmark = pytest.mark.gpu
@@ -88,3 +89,38 @@ def test_a_faulted_append_does_nothing(cuda_dev, kind, where, batch, t, page, hk
         at = torch.arange(int(cache.lens[i]) - t, int(cache.lens[i]), device="cuda")
         ids = cache.tables[i].long()[at // page]
         assert torch.equal(cache.k[0][ids, :, at % page], k[i]) and torch.equal(cache.v[0][ids, :, at % page], v[i])
+
+
+@pytest.mark.parametrize("dtype,pages", [(torch.bfloat16, 34000), (torch.float32, 17100)])
+def test_pools_beyond_32_bits(cuda_dev, dtype, pages):
+    """Pages whose elements, or bytes, are numbered beyond 2^32: stored, forked, moved and read there as in a small pool."""
+    shape = (1, pages, 8, 128, 128)
+    torch.cuda.empty_cache()
+    big = PagedKvCache(1, pages, 128, 8, 128, 6, 1024, dtype=dtype, pools=tuple(torch.empty(shape, dtype=dtype, device="cuda") for _ in range(2)))
+    small = PagedKvCache(1, 48, 128, 8, 128, 6, 1024, dtype=dtype)
+    big.refs[:pages - 40] = 1                   # taken by others
+    assert (pages - 40) * 8 * 128 * 128 * big.k.element_size() > 1 << 32
+    g = torch.Generator(device="cuda").manual_seed(3)
+    q, k, v = (torch.randn((1, 700, h, 128), device="cuda", generator=g).to(dtype) for h in (32, 8, 8))
+    step_q = torch.randn((5, 1, 32, 128), device="cuda", generator=g).to(dtype)
+    outs = []
+    for c in (big, small):
+        c.reserve([0], 700)
+        c.append(0, [0], k, v)
+        c.fork([0] * 4, [1, 2, 3, 4])
+        c.reserve([0, 1, 2, 3, 4], 1)
+        c.append(0, [0, 1, 2, 3, 4], k[0, :5, None], v[0, :5, None])
+        plan = c.attention_plan(5, 32)
+        plan.update([0, 1, 2, 3, 4])
+        outs.append([c.attention(0, step_q, plan)])
+        c.copy([2], [5])
+        c.free([1, 2])
+        if c is big:
+            c.refs[:30] = 0                     # room at the front, the others' pages stay
+        c.compact()
+        plan.update([0, 3, 4, 5, 5])
+        outs[-1].append(c.attention(0, step_q, plan))
+        c.check()
+    assert int(big.tables.max()) < pages - 40 + 30 and int(big.tables[0, 0]) < 30
+    for a, b in zip(*outs):
+        assert torch.equal(a, b) and bool(torch.isfinite(a).all())
