@@ -4,7 +4,7 @@
 // one, is a sequence of launches that a graph can hold.  One CTA does it: a pool has some thousands of pages, and a page's number
 // depends on all that are taken before it.  What it decides, a second kernel copies with the whole device.
 // On a B200, each kernel by itself with cold caches: 63 forks of 16 pages 10 - 13 us, bound by some ten reads that depend on one another; the list of a compaction of 320
-// pages 5 us.
+// pages 5 us.  In a graph: a token reserved for 1 / 64 / 128 sequences 3.0 / 3.7 / 4.5 us, 16 pages each freed 3.0 / 4.8 / 7.1.
 #include <cstdio>
 
 #include "kv_cache.cuh"

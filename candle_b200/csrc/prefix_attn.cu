@@ -13,7 +13,8 @@ constexpr int kThreads = 256, kPlanCtas = 8;
 
 // Units per worker of the own line.  f16 and bf16: the four warps of a CTA that have nothing else, and the eight that come when its `units` shared ones are done.  In clocks
 // of a B200 SM: a shared unit takes 4,300 and the first of them 5,000 more, one of the four warps takes some 1,700 a step beside them, and twelve warps together are bound by
-// HBM with 400 a step.  All finish together by that; a model that is off by a third leaves the one kind of warps idle for a tenth of the time.
+// HBM with 400 a step.  All finish together by that; a model that is off by a third leaves the one kind of warps idle for a tenth of the time.  (Measured with heads of 128; those of
+// 64 have the same division.)
 __device__ __forceinline__ void own_chunks(const Shape &s, int units, int line, int &chunk, int &chunk2) {
     chunk2 = 1;
     if (s.own_first == s.own_workers) { chunk = max((line + s.own_workers - 1) / s.own_workers, 1); return; }

@@ -9,7 +9,7 @@
 // 10,000 clocks for 64 KB - where HBM gives an SM 64 KB in 2,850.  Four such warps run beside the others, so that HBM and tensor
 // cores are both in use, and the softmax warps join them when the shared items are done.
 //
-// By itself, cold caches: 128 sequences over 32768 shared keys, 32 / 8 heads of 128 (70 GFLOP, 405 MB) 95 us: 28 shared units of 4,300 clocks a CTA, in which the tensor cores
+// By itself, cold caches: 128 sequences over 32768 shared keys, 32 / 8 heads of 128 (70 GFLOP, 405 MB) 97 us: 28 shared units of 4,300 clocks a CTA, in which the tensor cores
 // and the exponentials would each take 2,050, beside some 220 own steps; 64 over 8191 (9 GFLOP, 185 MB) 41 us.
 //
 // In both m is the row's maximum so far, kept until a score passes it by 2^8 (weights up to 256 are as good as any, the sum has the same
