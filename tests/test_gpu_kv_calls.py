@@ -49,7 +49,7 @@ KINDS = {"slot": "out of range", "twice": "named twice", "long": "position", "ro
 @pytest.mark.parametrize("batch,t,page,hkv,hq", [(3, 1, 16, 1, 1), (3, 40, 16, 3, 5), (3, 3000, 64, 4, 4), (3, 3000, 16, 1, 2), (300, 1, 16, 2, 2), (600, 2, 16, 1, 1)])
 def test_a_faulted_append_does_nothing(cuda_dev, kind, where, batch, t, page, hkv, hq):
     """One slot of many cannot be stored, the first or the last: nothing is stored, no query given, whoever finds it; a second call does nothing either; the state is as it was, and
-    once the fault is taken the call without that slot does all.  From one check to one a thread, several a thread (300 and 141 of them), and more (564, 1200)."""
+    once the fault is taken the call without that slot does all.  From one check to one a thread, several a thread (144 and 300 of them), and more than a CTA makes itself (567, 1200)."""
     if kind == "rotary" and where == 0:
         pytest.skip("the tables end for the longest sequence")
     per = -(-(t + 40) // page)
